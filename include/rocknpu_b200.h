@@ -1,6 +1,6 @@
 /*
  * rocknpu_b200.h -- what librocknpu.so adds beside the reference C ABI
- * (rocknpu.h).  Five groups:
+ * (rocknpu.h).  Six groups:
  *
  *  1. The ggml plugin's host rules (adapters/ggml-rocknpu), exported so a
  *     plugin built against ggml can call them and tests can check them
@@ -17,6 +17,9 @@
  *     outputs are unspecified (later kernels of the call may have run on
  *     scratch the failed step never wrote); only a zero status vouches for
  *     them.
+ *  2b. 8-bit floating point (e4m3) with a scale per block of 128: the
+ *     activation quantiser, weight preparation and product, device pointers
+ *     and status word as in group 2.
  *  3. Multi-GPU N-sharding: the row split, the all-gather layout, and peer
  *     (CUDA IPC) buffers for a GEMM whose epilogue all-gathers over NVLink.
  *  4. W8 sidecar files: the plugin's disk cache of prepared int8 weights.
@@ -43,6 +46,7 @@ enum rocknpu_ggml_type {
     ROCKNPU_GGML_Q4_K = 12,
     ROCKNPU_GGML_Q5_K = 13,
     ROCKNPU_GGML_Q6_K = 14,
+    ROCKNPU_GGML_BF16 = 30, /* dense operands of the e4m3 entry points only */
 };
 
 /* The parts of a ggml MUL_MAT node that supports_op reads: src0 = weights
@@ -315,6 +319,64 @@ int rocknpu_b200_kq_layout(uint32_t kind, const uint8_t *blocks, size_t k, size_
                            rocknpu_stream stream);
 int rocknpu_b200_gemv_kq(uint32_t kind, const uint8_t *layout, size_t k, size_t n, const float *x, float *y,
                          int *status, rocknpu_stream stream);
+
+/* ---- 2b. 8-bit floating point (e4m3) with a scale per block of 128 ------ */
+
+/* Values are e4m3 bytes; a value stands for byte * scale.  Activations have
+ * an f32 scale per row and 128 columns, scales[m][ceil(k / 128)]; weights one
+ * per 128 x 128 block, scales[ceil(n / 128)][ceil(k / 128)] (the last block
+ * of a row or column may be shorter).  A block's scale is amax / 448, at
+ * least 2^-126, or 1 for a block of zeros; a value is fl(x / scale) rounded
+ * to the nearest e4m3 (ties to even).  Products of two scales must be finite.
+ * `type` / `out_type` are ggml ids: ROCKNPU_GGML_F32, _F16 or _BF16; dense
+ * pointers are aligned to their elements (16-byte aligned rows are faster).
+ * A non-finite input sets *status to 1 and leaves the outputs unspecified. */
+
+/* Activation rows a[m][lda] -> a_f8[m][ld_f8] + scales[m][ld_scales]; columns
+ * k..ld_f8 of a_f8 are left as they are. */
+int rocknpu_b200_quantize_rows_f8(uint32_t type, const void *a, size_t m, size_t k, size_t lda, uint8_t *a_f8,
+                                  size_t ld_f8, float *scales, size_t ld_scales, int *status, rocknpu_stream stream);
+
+/* `count` dense weights w[n][ldw], each n * ldw elements behind the last (the
+ * experts of a layer), -> w_f8[n][ld_f8] + scales, `count` times. */
+int rocknpu_b200_prepare_f8(uint32_t type, const void *w, size_t n, size_t k, size_t ldw, size_t count, uint8_t *w_f8,
+                            size_t ld_f8, float *scales, int *status, rocknpu_stream stream);
+
+/* The same from n rows of K-quant superblocks (kind 4/5/6, k % 256 == 0): the
+ * values are ggml's f32 dequantisation.  `blocks` and w_f8 4-byte aligned,
+ * ld_f8 a multiple of 4. */
+int rocknpu_b200_prepare_f8_q(uint32_t kind, const uint8_t *blocks, size_t k, size_t n, uint8_t *w_f8, size_t ld_f8,
+                              float *scales, int *status, rocknpu_stream stream);
+
+/* Bytes of workspace the e4m3 product of this shape can use. */
+size_t rocknpu_b200_gemm_f8_workspace_bytes(size_t m, size_t n, size_t k);
+
+/* out[m][ldo] = sum over blocks b of a_scales[m][b] * w_scales[n / 128][b] *
+ * sum_{k in b} a_f8[m][k] * w_f8[n][k], on tcgen05, in f32, rounded once to
+ * out_type.  a_f8 and w_f8 16-byte aligned, ld_a and ld_w multiples of 16.
+ * `workspace` (optional, device memory, 16-byte aligned) lets shapes with few
+ * tiles split K; NULL or fewer than rocknpu_b200_gemm_f8_workspace_bytes runs
+ * without.  The first 64 KiB must be zero before the first use of a
+ * workspace; every launch that ends with status 0 or 1 leaves them zero, so
+ * one workspace serves calls of any shape, in turn.  Calls that share a
+ * workspace must not overlap on the GPU (two streams, two captured graphs
+ * replayed at once).  Results do not depend on the order in which CTAs
+ * finish. */
+int rocknpu_b200_gemm_f8(const uint8_t *a_f8, size_t ld_a, const float *a_scales, size_t ld_as, const uint8_t *w_f8,
+                         size_t ld_w, const float *w_scales, void *out, uint32_t out_type, size_t ldo, size_t m,
+                         size_t k, size_t n, void *workspace, size_t workspace_bytes, int *status,
+                         rocknpu_stream stream);
+
+/* Quantiser and product in one call: a[m][lda] of `type` times a prepared
+ * weight -> out[m][ldo] of out_type, the same bits as
+ * rocknpu_b200_quantize_rows_f8 followed by rocknpu_b200_gemm_f8 with a
+ * workspace.  `workspace` as above but required, with at least
+ * rocknpu_b200_matmul_f8_workspace_bytes bytes (it also holds the quantised
+ * activations). */
+size_t rocknpu_b200_matmul_f8_workspace_bytes(size_t m, size_t n, size_t k);
+int rocknpu_b200_matmul_f8(const void *a, uint32_t type, size_t lda, const uint8_t *w_f8, size_t ld_w,
+                           const float *w_scales, void *out, uint32_t out_type, size_t ldo, size_t m, size_t k,
+                           size_t n, void *workspace, size_t workspace_bytes, int *status, rocknpu_stream stream);
 
 /* ---- 3. multi-GPU N-sharding (one process per GPU, one node) ----------- */
 

@@ -26,6 +26,7 @@ BLOCK_BYTES = {Q4_K: 144, Q5_K: 176, Q6_K: 210}
 
 # ggml type ids understood by rocknpu_mul_mat_supported
 GGML_F32, GGML_F16, GGML_Q4_K, GGML_Q5_K, GGML_Q6_K = 0, 1, 12, 13, 14
+GGML_BF16 = 30  # dense operands of the e4m3 entry points only
 
 _P = ctypes.c_void_p
 _S = ctypes.c_size_t
@@ -82,6 +83,13 @@ SIGNATURES = {
     "rocknpu_b200_kq_layout_bytes": (_S, [_U32, _S, _S]),
     "rocknpu_b200_kq_layout": (_I, [_U32, _P, _S, _S, _P, _P]),
     "rocknpu_b200_gemv_kq": (_I, [_U32, _P, _S, _S, _P, _P, _P, _P]),
+    "rocknpu_b200_quantize_rows_f8": (_I, [_U32, _P, _S, _S, _S, _P, _S, _P, _S, _P, _P]),
+    "rocknpu_b200_prepare_f8": (_I, [_U32, _P, _S, _S, _S, _S, _P, _S, _P, _P, _P]),
+    "rocknpu_b200_prepare_f8_q": (_I, [_U32, _P, _S, _S, _P, _S, _P, _P, _P]),
+    "rocknpu_b200_gemm_f8_workspace_bytes": (_S, [_S, _S, _S]),
+    "rocknpu_b200_gemm_f8": (_I, [_P, _S, _P, _S, _P, _S, _P, _P, _U32, _S, _S, _S, _S, _P, _S, _P, _P]),
+    "rocknpu_b200_matmul_f8_workspace_bytes": (_S, [_S, _S, _S]),
+    "rocknpu_b200_matmul_f8": (_I, [_P, _U32, _S, _P, _S, _P, _P, _U32, _S, _S, _S, _S, _P, _S, _P, _P]),
     "rocknpu_b200_shard_rows": (_S, [_S, _S, _P, _P]),
     "rocknpu_b200_gather_shards": (_I, [_P, _S, _S, _S, _S, _P, _P, _P, _S, _P]),
     "rocknpu_b200_peer_buffer_create": (_I, [_S, _I, _I, _P, _P]),

@@ -90,6 +90,40 @@ rk::GemmWorkspace gemm_ws_view(void* base, size_t bytes, const rk::GemmPlan& pl)
     return w;
 }
 
+// ---- e4m3 entry points: shared checks ----
+
+bool dim_ok(size_t v) { return v > 0 && v <= 0x7fffff00; }
+size_t f8_blocks(size_t k) { return (k + 127) / 128; }
+
+// A dense pointer of a supported type, aligned to its elements.
+bool dense_ok(uint32_t type, const void* p) {
+    const size_t size = type == ROCKNPU_GGML_F32                                 ? 4
+                        : type == ROCKNPU_GGML_F16 || type == ROCKNPU_GGML_BF16 ? 2
+                                                                                 : 0;
+    return size && p && reinterpret_cast<uintptr_t>(p) % size == 0;
+}
+
+int launch_status(int e) {
+    return e == cudaSuccess ? kOk : (e == cudaErrorInvalidValue ? kInvalid : kExecError);
+}
+
+bool gemm_f8_args(rk::GemmF8* g, const uint8_t* w_f8, size_t ld_w, const float* w_scales, void* out, uint32_t out_type,
+                  size_t ldo, size_t m, size_t k, size_t n) {
+    if (!w_f8 || !w_scales || !dense_ok(out_type, out) || ld_w < k || ld_w % 16 != 0 || ldo < n ||
+        reinterpret_cast<uintptr_t>(w_f8) % 16 != 0)
+        return false;
+    g->w = w_f8;
+    g->ldw = static_cast<long long>(ld_w);
+    g->w_scale = w_scales;
+    g->out = out;
+    g->out_type = static_cast<int>(out_type);
+    g->ldo = static_cast<long long>(ldo);
+    g->m = static_cast<int>(m);
+    g->n = static_cast<int>(n);
+    g->k = static_cast<int>(k);
+    return true;
+}
+
 // Column chunk width of split_wide_mtile (L:2140-2141) for n > 8192.
 size_t wide_chunk(size_t n) {
     const size_t chunks = (n + 8191) / 8192;
@@ -1730,6 +1764,101 @@ int rocknpu_b200_gemv_kq(uint32_t kind, const uint8_t* layout, size_t k, size_t 
                                      status, static_cast<cudaStream_t>(stream));
     if (e == cudaErrorInvalidValue) return kInvalid;
     return cuda_status(static_cast<cudaError_t>(e));
+}
+
+// ---- e4m3 with a scale per block of 128 ------------------------------------
+
+int rocknpu_b200_quantize_rows_f8(uint32_t type, const void* a, size_t m, size_t k, size_t lda, uint8_t* a_f8,
+                                  size_t ld_f8, float* scales, size_t ld_scales, int* status, rocknpu_stream stream) {
+    if (!dense_ok(type, a) || !a_f8 || !scales || !status || !dim_ok(m) || !dim_ok(k) || lda < k || ld_f8 < k ||
+        ld_scales < f8_blocks(k))
+        return kInvalid;
+    return launch_status(rk::launch_quant_rows_f8(static_cast<int>(type), a, static_cast<int>(m), static_cast<int>(k),
+                                                  static_cast<long long>(lda), a_f8, static_cast<long long>(ld_f8),
+                                                  scales, static_cast<long long>(ld_scales), status,
+                                                  static_cast<cudaStream_t>(stream)));
+}
+
+int rocknpu_b200_prepare_f8(uint32_t type, const void* w, size_t n, size_t k, size_t ldw, size_t count, uint8_t* w_f8,
+                            size_t ld_f8, float* scales, int* status, rocknpu_stream stream) {
+    if (!dense_ok(type, w) || !w_f8 || !scales || !status || !dim_ok(n) || !dim_ok(k) || !dim_ok(count) || ldw < k ||
+        ld_f8 < k)
+        return kInvalid;
+    return launch_status(rk::launch_prep_f8(static_cast<int>(type), w, static_cast<int>(n), static_cast<int>(k),
+                                            static_cast<long long>(ldw), static_cast<int>(count), w_f8,
+                                            static_cast<long long>(ld_f8), scales, status,
+                                            static_cast<cudaStream_t>(stream)));
+}
+
+int rocknpu_b200_prepare_f8_q(uint32_t kind, const uint8_t* blocks, size_t k, size_t n, uint8_t* w_f8, size_t ld_f8,
+                              float* scales, int* status, rocknpu_stream stream) {
+    if ((kind != 4 && kind != 5 && kind != 6) || !blocks || !w_f8 || !scales || !status || !dim_ok(n) || !dim_ok(k) ||
+        k % 256 != 0 || ld_f8 < k || ld_f8 % 4 != 0 || reinterpret_cast<uintptr_t>(blocks) % 4 != 0 ||
+        reinterpret_cast<uintptr_t>(w_f8) % 4 != 0)
+        return kInvalid;
+    return launch_status(rk::launch_prep_f8_kq(static_cast<int>(kind), blocks, static_cast<int>(n),
+                                               static_cast<int>(k), w_f8, static_cast<long long>(ld_f8), scales,
+                                               status, static_cast<cudaStream_t>(stream)));
+}
+
+size_t rocknpu_b200_gemm_f8_workspace_bytes(size_t m, size_t n, size_t k) {
+    if (!dim_ok(m) || !dim_ok(n) || !dim_ok(k)) return 0;
+    return rk::kF8CounterBytes +
+           rk::gemm_f8_scratch_bytes(static_cast<int>(m), static_cast<int>(n), static_cast<int>(k));
+}
+
+int rocknpu_b200_gemm_f8(const uint8_t* a_f8, size_t ld_a, const float* a_scales, size_t ld_as, const uint8_t* w_f8,
+                         size_t ld_w, const float* w_scales, void* out, uint32_t out_type, size_t ldo, size_t m,
+                         size_t k, size_t n, void* workspace, size_t workspace_bytes, int* status,
+                         rocknpu_stream stream) {
+    if (!a_f8 || !a_scales || !status || ld_as < f8_blocks(k) || ld_a < k || !dim_ok(m) || !dim_ok(k) || !dim_ok(n) ||
+        ld_a % 16 != 0 || reinterpret_cast<uintptr_t>(a_f8) % 16 != 0 || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+        return kInvalid;
+    rk::GemmF8 g;
+    if (!gemm_f8_args(&g, w_f8, ld_w, w_scales, out, out_type, ldo, m, k, n)) return kInvalid;
+    g.a = a_f8;
+    g.lda = static_cast<long long>(ld_a);
+    g.a_scale = a_scales;
+    g.ld_as = static_cast<long long>(ld_as);
+    if (workspace && workspace_bytes >= rk::kF8CounterBytes) {
+        g.counters = static_cast<unsigned*>(workspace);
+        g.scratch = static_cast<char*>(workspace) + rk::kF8CounterBytes;
+        g.scratch_bytes = workspace_bytes - rk::kF8CounterBytes;
+    }
+    return launch_status(rk::launch_gemm_f8(g, status, static_cast<cudaStream_t>(stream)));
+}
+
+size_t rocknpu_b200_matmul_f8_workspace_bytes(size_t m, size_t n, size_t k) {
+    if (!dim_ok(m) || !dim_ok(n) || !dim_ok(k)) return 0;
+    return round_up(rocknpu_b200_gemm_f8_workspace_bytes(m, n, k), 256) + round_up(m * round_up(k, 16), 256) +
+           m * f8_blocks(k) * sizeof(float);
+}
+
+int rocknpu_b200_matmul_f8(const void* a, uint32_t type, size_t lda, const uint8_t* w_f8, size_t ld_w,
+                           const float* w_scales, void* out, uint32_t out_type, size_t ldo, size_t m, size_t k,
+                           size_t n, void* workspace, size_t workspace_bytes, int* status, rocknpu_stream stream) {
+    if (!dense_ok(type, a) || !workspace || !status || !dim_ok(m) || !dim_ok(k) || !dim_ok(n) || lda < k ||
+        reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
+        workspace_bytes < rocknpu_b200_matmul_f8_workspace_bytes(m, n, k))
+        return kInvalid;
+    rk::GemmF8 g;
+    if (!gemm_f8_args(&g, w_f8, ld_w, w_scales, out, out_type, ldo, m, k, n)) return kInvalid;
+    const size_t head = round_up(rocknpu_b200_gemm_f8_workspace_bytes(m, n, k), 256), ld8 = round_up(k, 16);
+    uint8_t* a8 = static_cast<uint8_t*>(workspace) + head;
+    float* as = reinterpret_cast<float*>(a8 + round_up(m * ld8, 256));
+    g.a = a8;
+    g.lda = static_cast<long long>(ld8);
+    g.a_scale = as;
+    g.ld_as = static_cast<long long>(f8_blocks(k));
+    g.counters = static_cast<unsigned*>(workspace);
+    g.scratch = static_cast<char*>(workspace) + rk::kF8CounterBytes;
+    g.scratch_bytes = head - rk::kF8CounterBytes;
+    g.early_weights = true;  // the quantiser's launch waited for all earlier work on the stream
+    const int st = launch_status(rk::launch_quant_rows_f8(
+        static_cast<int>(type), a, static_cast<int>(m), static_cast<int>(k), static_cast<long long>(lda), a8,
+        static_cast<long long>(ld8), as, g.ld_as, status, static_cast<cudaStream_t>(stream)));
+    if (st != kOk) return st;
+    return launch_status(rk::launch_gemm_f8(g, status, static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

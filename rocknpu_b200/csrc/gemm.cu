@@ -97,6 +97,10 @@ int current_device() {
 
 }  // namespace
 
+bool make_kmajor_map(void* map, const void* base, int elem_bytes, int k, int rows, long long ld_bytes, int box_rows) {
+    return make_map(static_cast<CUtensorMap*>(map), base, elem_bytes, k, rows, ld_bytes, box_rows);
+}
+
 int sm_count() {
     static int count[64] = {};
     const int dev = current_device();

@@ -139,6 +139,52 @@ void launch_hilo_residual(const float* a, int m, int k, long long lda, float* re
 void launch_add_halves(const float* hi, const float* lo, float* out, long long len, cudaStream_t s);
 
 
+// ---- e4m3 with a scale per block of 128 ------------------------------------
+
+// Element types of dense operands (ggml's GGML_TYPE_* ids).
+enum DType : int { kTypeF32 = 0, kTypeF16 = 1, kTypeBF16 = 30 };
+
+// Activation rows a[m][lda] -> e4m3 out[m][ld8] + scales[m][lds], one per 128
+// columns.  Columns k..ld8 are left as they are.  Returns a cudaError_t value.
+int launch_quant_rows_f8(int type, const void* a, int m, int k, long long lda, uint8_t* out, long long ld8,
+                         float* scales, long long lds, int* err, cudaStream_t s);
+// `count` dense matrices w[n][ldw] (each n * ldw elements behind the last) ->
+// e4m3 out[n][ld8] + scales[ceil(n/128)][ceil(k/128)], count times.
+int launch_prep_f8(int type, const void* w, int n, int k, long long ldw, int count, uint8_t* out, long long ld8,
+                   float* scales, int* err, cudaStream_t s);
+// The same from K-quant superblocks (blocks 4-byte, out and ld8 4-byte aligned).
+int launch_prep_f8_kq(int kind, const uint8_t* blocks, int n, int k, uint8_t* out, long long ld8, float* scales,
+                      int* err, cudaStream_t s);
+
+// Scratch of the e4m3 products: kF8Counters counters, all zero between
+// launches (every launch leaves them zero), then bytes with no such rule.
+constexpr size_t kF8Counters = 16384;
+constexpr size_t kF8CounterBytes = kF8Counters * sizeof(unsigned);
+size_t gemm_f8_scratch_bytes(int m, int n, int k);
+struct GemmF8 {
+    const uint8_t* a = nullptr;  // e4m3 [m][lda], lda % 16 == 0
+    long long lda = 0;
+    const float* a_scale = nullptr;  // [m][ld_as]
+    long long ld_as = 0;
+    const uint8_t* w = nullptr;  // e4m3 [n][ldw], ldw % 16 == 0
+    long long ldw = 0;
+    const float* w_scale = nullptr;  // [ceil(n/128)][ceil(k/128)]
+    void* out = nullptr;             // [m][ldo] of out_type
+    int out_type = kTypeF32;
+    long long ldo = 0;
+    int m = 0, n = 0, k = 0;
+    unsigned* counters = nullptr;  // kF8Counters, or null: no split over K
+    void* scratch = nullptr;       // gemm_f8_scratch_bytes
+    size_t scratch_bytes = 0;
+    // the weights were complete before the preceding launch on the stream
+    // began: stream them ahead of that launch's end
+    bool early_weights = false;
+};
+int launch_gemm_f8(const GemmF8& g, int* err, cudaStream_t s);
+
 int sm_count();
+// 2-D K-major tensor map (gemm.cu): rows x k elements of 1 or 2 bytes, row
+// pitch ld_bytes, box of 128 bytes x box_rows, 128-byte swizzle, zero fill.
+bool make_kmajor_map(void* map, const void* base, int elem_bytes, int k, int rows, long long ld_bytes, int box_rows);
 
 }  // namespace rk

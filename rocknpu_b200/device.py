@@ -8,7 +8,10 @@ from __future__ import annotations
 
 import torch
 
-from .capi import lib
+from .capi import BLOCK_BYTES, GGML_BF16, GGML_F16, GGML_F32, lib
+
+_TYPES = {torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16}
+F8_BLOCK = 128
 
 
 def _stream(stream) -> int:
@@ -133,4 +136,170 @@ def matmul_w8a8(ctx, a: torch.Tensor, w8: torch.Tensor, w_scales: torch.Tensor, 
     n = w8.shape[0]
     _check(lib().rocknpu_b200_matmul_w8a8(ctx.handle, a.data_ptr(), w8.data_ptr(), w_scales.data_ptr(),
                                           out.data_ptr(), m, k, n, _stream(stream)), "matmul_w8a8")
+    return out
+
+
+# ---- e4m3 with a scale per block of 128 --------------------------------------
+#
+# e4m3 tensors are torch.float8_e4m3fn; scales are f32, per row and 128 columns
+# for activations, per 128 x 128 block for weights.  These calls queue on the
+# operands' own device (its current torch stream unless one is given).
+
+def _f8_blocks(n: int) -> int:
+    return (n + F8_BLOCK - 1) // F8_BLOCK
+
+
+def _require(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _operands(first: torch.Tensor, *others) -> None:
+    _require(first.is_cuda, "operands are CUDA tensors")
+    for t in others:
+        _require(t is None or t.device == first.device, "all operands are on one device")
+
+
+def _status_word(status: torch.Tensor) -> None:
+    _require(status.dtype == torch.int32 and status.numel() >= 1, "status is an int32 tensor (new_status)")
+
+
+def _launch(name: str, device, stream, *args) -> None:
+    """Call entry point `name` with `device` current; the stream goes last."""
+    with torch.cuda.device(device):
+        _check(getattr(lib(), f"rocknpu_b200_{name}")(*args, _stream(stream)), name)
+
+
+def _f8_empty(*shape, device) -> torch.Tensor:
+    """e4m3 tensor whose rows start at multiples of 16 bytes."""
+    k16 = (shape[-1] + 15) // 16 * 16
+    return torch.empty((*shape[:-1], k16), dtype=torch.float8_e4m3fn, device=device)[..., :shape[-1]]
+
+
+def _f8_weight(w8: torch.Tensor, scales: torch.Tensor, what: str) -> None:
+    n, k = w8.shape[-2:]
+    _require(w8.dtype == torch.float8_e4m3fn and w8.stride(-1) == 1 and w8.stride(-2) >= k,
+             f"{what} is an e4m3 tensor of whole rows")
+    _require(scales.dtype == torch.float32 and scales.is_contiguous() and
+             tuple(scales.shape) == (*w8.shape[:-2], _f8_blocks(n), _f8_blocks(k)),
+             f"{what} scales are a contiguous f32 tensor, one per 128 x 128 block")
+
+
+def quantize_rows_f8(a: torch.Tensor, status: torch.Tensor, out: torch.Tensor | None = None,
+                     scales: torch.Tensor | None = None, stream=None):
+    """f32 / f16 / bf16 [m, k] -> (e4m3 [m, k], f32 scales [m, ceil(k / 128)])."""
+    _operands(a, status, out, scales)
+    _status_word(status)
+    _require(a.dim() == 2 and a.dtype in _TYPES and a.stride(1) == 1, "a is an f32, f16 or bf16 matrix of whole rows")
+    m, k = a.shape
+    _require(m > 0 and k > 0, "a is not empty")
+    out = _f8_empty(m, k, device=a.device) if out is None else out
+    scales = torch.empty((m, _f8_blocks(k)), dtype=torch.float32, device=a.device) if scales is None else scales
+    _require(out.dtype == torch.float8_e4m3fn and out.shape == a.shape and out.stride(1) == 1,
+             "out is an e4m3 matrix of a's shape")
+    _require(scales.dtype == torch.float32 and tuple(scales.shape) == (m, _f8_blocks(k)) and
+             (scales.stride(1) == 1 or scales.shape[1] == 1), "scales are f32 [m, ceil(k / 128)]")
+    _launch("quantize_rows_f8", a.device, stream, _TYPES[a.dtype], a.data_ptr(), m, k, _pitch(a), out.data_ptr(),
+            _pitch(out), scales.data_ptr(), _pitch(scales), status.data_ptr())
+    return out, scales
+
+
+def _pitch(t: torch.Tensor) -> int:
+    """Row pitch in elements; a single row's stride says nothing."""
+    return t.stride(-2) if t.shape[-2] > 1 else max(t.shape[-1], t.stride(-2))
+
+
+def prepare_f8(w: torch.Tensor, status: torch.Tensor, stream=None):
+    """Dense weight(s) [n, k] or [experts, n, k] -> (e4m3 of the same shape,
+    f32 scales [..., ceil(n / 128), ceil(k / 128)])."""
+    _operands(w, status)
+    _status_word(status)
+    _require(w.dim() in (2, 3) and w.dtype in _TYPES and w.stride(-1) == 1 and w.numel() > 0,
+             "w is an f32, f16 or bf16 matrix, or a stack of them, of whole rows")
+    n, k = w.shape[-2:]
+    count = w.shape[0] if w.dim() == 3 else 1
+    ldw = _pitch(w)
+    _require(count == 1 or w.stride(0) == n * ldw, "a stack of weights has no gaps between them")
+    out = _f8_empty(*w.shape, device=w.device)
+    scales = torch.empty((*w.shape[:-2], _f8_blocks(n), _f8_blocks(k)), dtype=torch.float32, device=w.device)
+    _launch("prepare_f8", w.device, stream, _TYPES[w.dtype], w.data_ptr(), n, k, ldw, count, out.data_ptr(),
+            (k + 15) // 16 * 16, scales.data_ptr(), status.data_ptr())
+    return out, scales
+
+
+def prepare_f8_q(kind: int, blocks: torch.Tensor, k: int, n: int, status: torch.Tensor, stream=None):
+    """K-quant rows -> (e4m3 [n, k], f32 scales [ceil(n / 128), k / 128])."""
+    _operands(blocks, status)
+    _status_word(status)
+    _require(blocks.dtype == torch.uint8 and blocks.is_contiguous(), "blocks are contiguous uint8")
+    _require(kind in BLOCK_BYTES and k > 0 and n > 0 and k % 256 == 0 and
+             blocks.numel() >= n * (k // 256) * BLOCK_BYTES[kind], "blocks hold n rows of k / 256 superblocks")
+    out = torch.empty((n, k), dtype=torch.float8_e4m3fn, device=blocks.device)
+    scales = torch.empty((_f8_blocks(n), _f8_blocks(k)), dtype=torch.float32, device=blocks.device)
+    _launch("prepare_f8_q", blocks.device, stream, kind, blocks.data_ptr(), k, n, out.data_ptr(), k,
+            scales.data_ptr(), status.data_ptr())
+    return out, scales
+
+
+def gemm_f8_workspace_bytes(m: int, n: int, k: int) -> int:
+    return int(lib().rocknpu_b200_gemm_f8_workspace_bytes(m, n, k))
+
+
+def matmul_f8_workspace_bytes(m: int, n: int, k: int) -> int:
+    return int(lib().rocknpu_b200_matmul_f8_workspace_bytes(m, n, k))
+
+
+def _f8_out(out, m: int, n: int, dtype, device) -> torch.Tensor:
+    out = torch.empty((m, n), dtype=dtype, device=device) if out is None else out
+    _require(out.dtype in _TYPES and tuple(out.shape) == (m, n) and (out.stride(1) == 1 or n == 1),
+             f"out is an f32, f16 or bf16 matrix of shape {(m, n)}")
+    return out
+
+
+def gemm_f8(a8: torch.Tensor, a_scales: torch.Tensor, w8: torch.Tensor, w_scales: torch.Tensor,
+            status: torch.Tensor, out: torch.Tensor | None = None, out_dtype=torch.float32,
+            workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Block-scaled e4m3 product a8 [m, k] . w8 [n, k]^T (quantize_rows_f8,
+    prepare_f8).  Rows start at multiples of 16 bytes."""
+    _operands(a8, a_scales, w8, w_scales, status, out, workspace)
+    _status_word(status)
+    _require(a8.dim() == 2 and a8.dtype == torch.float8_e4m3fn and a8.stride(1) == 1 and a8.numel() > 0,
+             "a8 is an e4m3 matrix of whole rows")
+    m, k = a8.shape
+    _require(w8.dim() == 2 and w8.shape[1] == k and w8.numel() > 0, "w8 is [n, k]")
+    _f8_weight(w8, w_scales, "w8")
+    _require(a_scales.dtype == torch.float32 and tuple(a_scales.shape) == (m, _f8_blocks(k)) and
+             (a_scales.stride(1) == 1 or a_scales.shape[1] == 1), "a_scales are f32 [m, ceil(k / 128)]")
+    n = w8.shape[0]
+    out = _f8_out(out, m, n, out_dtype, a8.device)
+    _launch("gemm_f8", a8.device, stream, a8.data_ptr(), _pitch16(a8), a_scales.data_ptr(), _pitch(a_scales),
+            w8.data_ptr(), _pitch16(w8), w_scales.data_ptr(), out.data_ptr(), _TYPES[out.dtype], _pitch(out), m, k, n,
+            workspace.data_ptr() if workspace is not None else None,
+            workspace.numel() * workspace.element_size() if workspace is not None else 0, status.data_ptr())
+    return out
+
+
+def _pitch16(t: torch.Tensor) -> int:
+    """Row pitch of an e4m3 operand; a single row has none, and may end at k."""
+    return t.stride(-2) if t.shape[-2] > 1 else (t.shape[-1] + 15) // 16 * 16
+
+
+def matmul_f8(a: torch.Tensor, w8: torch.Tensor, w_scales: torch.Tensor, status: torch.Tensor,
+              workspace: torch.Tensor, out: torch.Tensor | None = None, out_dtype=None, stream=None) -> torch.Tensor:
+    """quantize_rows_f8 + gemm_f8: f32 / f16 / bf16 a [m, k] times a prepared
+    weight; the result has a's type unless `out` or `out_dtype` says another.
+    `workspace` (new_workspace of matmul_f8_workspace_bytes) is kept by the
+    caller, one per stream on which calls may be in flight."""
+    _operands(a, w8, w_scales, status, workspace, out)
+    _status_word(status)
+    _require(a.dim() == 2 and a.dtype in _TYPES and a.stride(1) == 1 and a.numel() > 0,
+             "a is an f32, f16 or bf16 matrix of whole rows")
+    m, k = a.shape
+    _require(w8.dim() == 2 and w8.shape[1] == k and w8.numel() > 0, "w8 is [n, k]")
+    _f8_weight(w8, w_scales, "w8")
+    n = w8.shape[0]
+    out = _f8_out(out, m, n, out_dtype or a.dtype, a.device)
+    _launch("matmul_f8", a.device, stream, a.data_ptr(), _TYPES[a.dtype], _pitch(a), w8.data_ptr(), _pitch16(w8),
+            w_scales.data_ptr(), out.data_ptr(), _TYPES[out.dtype], _pitch(out), m, k, n, workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), status.data_ptr())
     return out
