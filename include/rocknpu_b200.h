@@ -12,7 +12,8 @@
  *     a device pointer on the context's GPU, work is queued on `stream`
  *     (NULL = the context's own stream) and the call returns without
  *     waiting.  Kernels report errors in the device word `status`
- *     (0 = ok, 1 = non-finite input, >1 = a device-side wait ran out).
+ *     (0 = ok, 1 = non-finite input, 9 = an index out of range, any other:
+ *     a device-side wait ran out).
  *     Whenever that word is non-zero after the work has run, the call's
  *     outputs are unspecified (later kernels of the call may have run on
  *     scratch the failed step never wrote); only a zero status vouches for
@@ -197,8 +198,8 @@ typedef struct rocknpu_b200_prompt_cache_stats {
 int rocknpu_b200_context_prompt_cache_stats(const rocknpu_context *context, rocknpu_b200_prompt_cache_stats *out);
 
 /* The status code of a device status word, as the host-pointer entry points
- * return it: 0 -> ROCKNPU_STATUS_OK, 1 (non-finite input) ->
- * ROCKNPU_STATUS_INVALID_ARGUMENT, any other value (a device-side wait that
+ * return it: 0 -> ROCKNPU_STATUS_OK, 1 (non-finite input)
+ * or 9 (index out of range) -> ROCKNPU_STATUS_INVALID_ARGUMENT, any other value (a device-side wait that
  * ran out) -> ROCKNPU_STATUS_EXECUTION_ERROR. */
 int rocknpu_b200_status_code(int device_status);
 
@@ -325,9 +326,9 @@ int rocknpu_b200_gemv_kq(uint32_t kind, const uint8_t *layout, size_t k, size_t 
 /* Values are e4m3 bytes; a value stands for byte * scale.  Activations have
  * an f32 scale per row and 128 columns, scales[m][ceil(k / 128)]; weights one
  * per 128 x 128 block, scales[ceil(n / 128)][ceil(k / 128)] (the last block
- * of a row or column may be shorter).  A block's scale is amax / 448, at
- * least 2^-126, or 1 for a block of zeros; a value is fl(x / scale) rounded
- * to the nearest e4m3 (ties to even).  Products of two scales must be finite.
+ * of a row or column may be shorter).  A block's scale is amax times
+ * 1 / 448 (both f32), at least 2^-126, or 1 for a block of zeros; a value is
+ * fl(x / scale) rounded to the nearest e4m3 (ties to even).  Products of two scales must be finite.
  * `type` / `out_type` are ggml ids: ROCKNPU_GGML_F32, _F16 or _BF16; dense
  * pointers are aligned to their elements (16-byte aligned rows are faster).
  * A non-finite input sets *status to 1 and leaves the outputs unspecified. */
@@ -377,6 +378,56 @@ size_t rocknpu_b200_matmul_f8_workspace_bytes(size_t m, size_t n, size_t k);
 int rocknpu_b200_matmul_f8(const void *a, uint32_t type, size_t lda, const uint8_t *w_f8, size_t ld_w,
                            const float *w_scales, void *out, uint32_t out_type, size_t ldo, size_t m, size_t k,
                            size_t n, void *workspace, size_t workspace_bytes, int *status, rocknpu_stream stream);
+
+/* A stack of prepared weights: expert i's e4m3 rows at w_f8 + i * stride, row
+ * pitch ld (16-byte aligned, ld and stride multiples of 16), its block scales
+ * at scales + i * scale_stride.  With one expert the strides are not read. */
+typedef struct rocknpu_b200_f8_experts {
+    const uint8_t *w_f8;
+    size_t ld, stride;
+    const float *scales;
+    size_t scale_stride;
+} rocknpu_b200_f8_experts;
+
+/* A mixture-of-experts layer for up to 64 tokens:
+ *   the top_k experts of each token by x . router^T (ties to the lower
+ *   expert), weighted by the softmax over all experts, or over the chosen
+ *   ones (renormalize);
+ *   out = sum over slots of weight * down(silu(gate(x)) * up(x)).
+ * With a router, ids and weights [tokens][top_k] are outputs (slots in order
+ * of falling logits).  Without (NULL) they are inputs: a negative id is an
+ * empty slot, whatever its weight; a token with only empty slots gets a row
+ * of zeros; an id may occur twice; an id >= experts sets *status to 9
+ * (INVALID_ARGUMENT by rocknpu_b200_status_code) and counts as empty.
+ * Activations are not quantised: f32 ones (and the hidden values) enter the
+ * products with 22 bits relative to the largest of their block of 128, f16
+ * and bf16 ones exactly, with hidden values of 11 bits; sums are f32.
+ * hidden and ffn are multiples of 16, top_k <= 16, experts <= 256. */
+typedef struct rocknpu_b200_moe_f8_args {
+    size_t tokens, hidden, ffn, experts, top_k;
+    uint32_t type;        /* of x and out */
+    const void *x;        /* [tokens][ld_x] */
+    void *out;            /* [tokens][ld_out] */
+    size_t ld_x, ld_out;
+    rocknpu_b200_f8_experts gate, up; /* [experts][ffn][hidden] */
+    rocknpu_b200_f8_experts down;     /* [experts][hidden][ffn] */
+    const void *router;   /* [experts][ld_router] of router_type, or NULL */
+    uint32_t router_type;
+    size_t ld_router;
+    int32_t renormalize;
+    int32_t *ids;
+    float *weights;
+} rocknpu_b200_moe_f8_args;
+
+/* Bytes of workspace (0 for a shape outside the limits above), and the layer.
+ * One cooperative launch: it needs every SM of the GPU for one CTA, waits for
+ * other kernels that hold them, and can be captured into a graph.  The
+ * workspace follows rocknpu_b200_gemm_f8's rules and can be shared with those
+ * calls, in turn.  Results do not depend on the order in which CTAs finish. */
+size_t rocknpu_b200_moe_f8_workspace_bytes(size_t tokens, size_t hidden, size_t ffn, size_t experts, size_t top_k,
+                                           uint32_t type);
+int rocknpu_b200_moe_f8(const rocknpu_b200_moe_f8_args *args, void *workspace, size_t workspace_bytes, int *status,
+                        rocknpu_stream stream);
 
 /* ---- 3. multi-GPU N-sharding (one process per GPU, one node) ----------- */
 

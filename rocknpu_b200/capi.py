@@ -90,6 +90,8 @@ SIGNATURES = {
     "rocknpu_b200_gemm_f8": (_I, [_P, _S, _P, _S, _P, _S, _P, _P, _U32, _S, _S, _S, _S, _P, _S, _P, _P]),
     "rocknpu_b200_matmul_f8_workspace_bytes": (_S, [_S, _S, _S]),
     "rocknpu_b200_matmul_f8": (_I, [_P, _U32, _S, _P, _S, _P, _P, _U32, _S, _S, _S, _S, _P, _S, _P, _P]),
+    "rocknpu_b200_moe_f8_workspace_bytes": (_S, [_S, _S, _S, _S, _S, _U32]),
+    "rocknpu_b200_moe_f8": (_I, [_P, _P, _S, _P, _P]),
     "rocknpu_b200_shard_rows": (_S, [_S, _S, _P, _P]),
     "rocknpu_b200_gather_shards": (_I, [_P, _S, _S, _S, _S, _P, _P, _P, _S, _P]),
     "rocknpu_b200_peer_buffer_create": (_I, [_S, _I, _I, _P, _P]),
@@ -107,6 +109,19 @@ SIGNATURES = {
 }
 
 _lib = None
+
+
+class F8Experts(ctypes.Structure):
+    """rocknpu_b200_f8_experts."""
+    _fields_ = [("w_f8", _P), ("ld", _S), ("stride", _S), ("scales", _P), ("scale_stride", _S)]
+
+
+class MoeF8Args(ctypes.Structure):
+    """rocknpu_b200_moe_f8_args."""
+    _fields_ = [("tokens", _S), ("hidden", _S), ("ffn", _S), ("experts", _S), ("top_k", _S), ("type", _U32),
+                ("x", _P), ("out", _P), ("ld_x", _S), ("ld_out", _S), ("gate", F8Experts), ("up", F8Experts),
+                ("down", F8Experts), ("router", _P), ("router_type", _U32), ("ld_router", _S),
+                ("renormalize", ctypes.c_int32), ("ids", _P), ("weights", _P)]
 
 
 class CacheStats(ctypes.Structure):

@@ -124,6 +124,27 @@ bool gemm_f8_args(rk::GemmF8* g, const uint8_t* w_f8, size_t ld_w, const float* 
     return true;
 }
 
+bool moe_shape_ok(const rocknpu_b200_moe_f8_args& a) {
+    return a.tokens >= 1 && a.tokens <= static_cast<size_t>(rk::kMoeMaxTokens) && a.experts >= 1 &&
+           a.experts <= static_cast<size_t>(rk::kMoeMaxExperts) && a.top_k >= 1 &&
+           a.top_k <= static_cast<size_t>(rk::kMoeMaxTop) && a.top_k <= a.experts && dim_ok(a.hidden) &&
+           dim_ok(a.ffn) && a.hidden % 16 == 0 && a.ffn % 16 == 0 && a.hidden <= (1u << 20) && a.ffn <= (1u << 20) &&
+           (a.type == ROCKNPU_GGML_F32 || a.type == ROCKNPU_GGML_F16 || a.type == ROCKNPU_GGML_BF16);
+}
+
+bool moe_weight(rk::MoeWeight* o, const rocknpu_b200_f8_experts& w, size_t rows, size_t k, size_t experts) {
+    if (!w.w_f8 || !w.scales || reinterpret_cast<uintptr_t>(w.w_f8) % 16 != 0 || w.ld < k || w.ld % 16 != 0 ||
+        (experts > 1 && (w.stride < (rows - 1) * w.ld + k || w.stride % 16 != 0 ||
+                         w.scale_stride < f8_blocks(rows) * f8_blocks(k))))
+        return false;
+    o->w = w.w_f8;
+    o->ld = static_cast<long long>(w.ld);
+    o->stride = experts > 1 ? static_cast<long long>(w.stride) : static_cast<long long>(rows * w.ld);
+    o->scales = w.scales;
+    o->scale_stride = static_cast<long long>(w.scale_stride);
+    return true;
+}
+
 // Column chunk width of split_wide_mtile (L:2140-2141) for n > 8192.
 size_t wide_chunk(size_t n) {
     const size_t chunks = (n + 8191) / 8192;
@@ -1594,7 +1615,7 @@ int rocknpu_b200_context_prompt_cache_stats(const rocknpu_context* context, rock
 
 int rocknpu_b200_status_code(int device_status) {
     if (device_status == rk::kErrNone) return kOk;
-    return device_status == rk::kErrNonFinite ? kInvalid : kExecError;
+    return device_status == rk::kErrNonFinite || device_status == rk::kErrBadIndex ? kInvalid : kExecError;
 }
 
 int rocknpu_b200_context_check(rocknpu_context* context) {
@@ -1859,6 +1880,55 @@ int rocknpu_b200_matmul_f8(const void* a, uint32_t type, size_t lda, const uint8
         static_cast<long long>(ld8), as, g.ld_as, status, static_cast<cudaStream_t>(stream)));
     if (st != kOk) return st;
     return launch_status(rk::launch_gemm_f8(g, status, static_cast<cudaStream_t>(stream)));
+}
+
+size_t rocknpu_b200_moe_f8_workspace_bytes(size_t tokens, size_t hidden, size_t ffn, size_t experts, size_t top_k,
+                                           uint32_t type) {
+    rocknpu_b200_moe_f8_args a{};
+    a.tokens = tokens;
+    a.hidden = hidden;
+    a.ffn = ffn;
+    a.experts = experts;
+    a.top_k = top_k;
+    a.type = type;
+    if (!moe_shape_ok(a)) return 0;
+    return rk::kF8CounterBytes + rk::moe_f8_scratch_bytes(static_cast<int>(tokens), static_cast<int>(hidden),
+                                                          static_cast<int>(ffn), static_cast<int>(experts),
+                                                          static_cast<int>(top_k), static_cast<int>(type));
+}
+
+int rocknpu_b200_moe_f8(const rocknpu_b200_moe_f8_args* args, void* workspace, size_t workspace_bytes, int* status,
+                        rocknpu_stream stream) {
+    if (!args || !workspace || !status || !moe_shape_ok(*args)) return kInvalid;
+    const rocknpu_b200_moe_f8_args& a = *args;
+    rk::MoeF8 m;
+    if (!dense_ok(a.type, a.x) || !dense_ok(a.type, a.out) || a.ld_x < a.hidden || a.ld_out < a.hidden || !a.ids ||
+        !a.weights || (a.router && (!dense_ok(a.router_type, a.router) || a.ld_router < a.hidden)) ||
+        !moe_weight(&m.gate, a.gate, a.ffn, a.hidden, a.experts) ||
+        !moe_weight(&m.up, a.up, a.ffn, a.hidden, a.experts) ||
+        !moe_weight(&m.down, a.down, a.hidden, a.ffn, a.experts) || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
+        workspace_bytes < rocknpu_b200_moe_f8_workspace_bytes(a.tokens, a.hidden, a.ffn, a.experts, a.top_k, a.type))
+        return kInvalid;
+    m.x = a.x;
+    m.out = a.out;
+    m.type = static_cast<int>(a.type);
+    m.ldx = static_cast<long long>(a.ld_x);
+    m.ldo = static_cast<long long>(a.ld_out);
+    m.router = a.router;
+    m.router_type = static_cast<int>(a.router_type);
+    m.ld_router = static_cast<long long>(a.ld_router);
+    m.ids = a.ids;
+    m.weights = a.weights;
+    m.t = static_cast<int>(a.tokens);
+    m.h = static_cast<int>(a.hidden);
+    m.f = static_cast<int>(a.ffn);
+    m.e = static_cast<int>(a.experts);
+    m.top = static_cast<int>(a.top_k);
+    m.renorm = a.renormalize ? 1 : 0;
+    m.counters = static_cast<unsigned*>(workspace);
+    m.scratch = static_cast<char*>(workspace) + rk::kF8CounterBytes;
+    m.scratch_bytes = workspace_bytes - rk::kF8CounterBytes;
+    return launch_status(rk::launch_moe_f8(m, status, static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

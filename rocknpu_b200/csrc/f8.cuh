@@ -1,10 +1,10 @@
 // e4m3 values with one f32 scale per block of 128: the arithmetic shared by
 // the activation quantiser, the weight preparation and the products.
 //
-// Block scale: s = amax / 448 (the IEEE quotient), at least 2^-126 so that it
-// is a normal number; 1 for a block of zeros.  Value: q = e4m3(fl(x / s)),
-// round to nearest even; |x / s| <= 448 (1 + 2^-23), which rounds to at most
-// 448, so nothing saturates.
+// Block scale: s = fl(amax * fl(1 / 448)), at least 2^-126 so that it is a
+// normal number; 1 for a block of zeros.  Value: q = e4m3(fl(x / s)), round to
+// nearest even; |x / s| <= 448 (1 + 2^-21), which rounds to at most 448, so
+// nothing saturates.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -17,7 +17,7 @@ namespace rk {
 constexpr int kF8Block = 128;
 
 __device__ __forceinline__ float f8_scale(float amax) {
-    return amax == 0.0f ? 1.0f : fmaxf(__fdiv_rn(amax, 448.0f), 1.17549435e-38f);
+    return amax == 0.0f ? 1.0f : fmaxf(__fmul_rn(amax, 1.0f / 448.0f), 1.17549435e-38f);
 }
 
 // Two f32 -> two e4m3 bytes (a in the low byte).

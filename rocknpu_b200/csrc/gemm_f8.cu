@@ -122,6 +122,22 @@ __device__ __forceinline__ void fail(int* err, volatile uint32_t* abort, int cod
     *abort = 1u;
 }
 
+// The epilogue warps' barrier; whether any of their threads passed true.
+__device__ __forceinline__ bool epi_any(bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n"
+        " .reg .pred p, q;\n"
+        " setp.ne.u32 p, %1, 0;\n"
+        " bar.red.or.pred q, 1, %2, p;\n"
+        " selp.u32 %0, 1, 0, q;\n"
+        "}\n"
+        : "=r"(r)
+        : "r"(v ? 1u : 0u), "n"(kEpiThreads)
+        : "memory");
+    return r != 0;
+}
+
 __device__ __forceinline__ void epi_bar() { asm volatile("bar.sync 1, %0;" ::"n"(kEpiThreads) : "memory"); }
 
 template <int N>
@@ -283,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_f8_kernel(const __grid_const
         Seg t;
         int g = 0;
         bool ok = true;
-        while (ok && walk.next(p, t)) {
+        while (walk.next(p, t)) {
             const float* ws = p.w_scale + static_cast<long long>(t.n0 / kWRows) * p.num_kb;
             const int m0 = t.m0 + half * COLS;
             const float* as[kPer];
@@ -296,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_f8_kernel(const __grid_const
             float acc[COLS];
 #pragma unroll
             for (int c = 0; c < COLS; ++c) acc[c] = 0.0f;
-            for (int kb = t.kb0; kb < t.kb1; ++kb, ++g) {
+            for (int kb = t.kb0; ok && kb < t.kb1; ++kb, ++g) {
                 const int b = g % B;
                 float* sc = slice + (g & 1) * COLS;
 #pragma unroll
@@ -312,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_f8_kernel(const __grid_const
                 ready = __shfl_sync(0xffffffffu, ready, 0);
                 if (!ready) {
                     if (lane == 0 && !*abort) fail(p.err, abort, kErrTimeoutAccum);
-                    ok = false;
+                    ok = false;  // this warp stores nothing more, but joins the others' barriers
                     break;
                 }
                 tc_fence_after();
@@ -335,10 +351,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_f8_kernel(const __grid_const
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&tempty[b]);
             }
-            if (!ok) break;
             const int col = t.n0 + q * 32 + lane;
             if (t.kb1 - t.kb0 == p.num_kb) {
-                store_tile<COLS>(p, acc, m0, col);
+                if (ok) store_tile<COLS>(p, acc, m0, col);
                 continue;
             }
             // a cut tile: this CTA's partial sums, then the last contributor adds all
@@ -349,11 +364,15 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_f8_kernel(const __grid_const
             const int x0 = t.tile * p.num_kb;
             const int first = range_of(p, x0), last = range_of(p, x0 + p.num_kb - 1);
             __threadfence();
-            epi_bar();
+            if (epi_any(!ok)) {
+                ok = false;
+                continue;
+            }
             if (etid == 0) {
-                const unsigned prev = atomicAdd(p.counters + t.tile, 1u);
+                // a tile that is cut is the last of its first CTA
+                const unsigned prev = atomicAdd(p.counters + first, 1u);
                 *last_flag = prev == static_cast<unsigned>(last - first) ? 1u : 0u;
-                if (*last_flag) p.counters[t.tile] = 0u;
+                if (*last_flag) p.counters[first] = 0u;
             }
             epi_bar();
             if (*last_flag) {
@@ -361,8 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_f8_kernel(const __grid_const
 #pragma unroll
                 for (int c = 0; c < COLS; ++c) acc[c] = 0.0f;
                 for (int cta = first; cta <= last; ++cta) {
-                    const float* theirs =
-                        p.part + (2ll * cta + (range_start(p, cta) <= x0 ? 1 : 0)) * kPart + etid;
+                    const float* theirs = p.part + (2ll * cta + (cta == first ? 1 : 0)) * kPart + etid;
 #pragma unroll
                     for (int c = 0; c < COLS; ++c) acc[c] += __ldcg(theirs + c * kEpiThreads);
                 }
@@ -403,7 +421,7 @@ F8Plan plan_f8(int m, int n, int k) {
         const double whole = static_cast<double>((tiles + sms - 1) / sms) * kb * block;
         const long long total = tiles * kb;
         const double cut = static_cast<double>((total + sms - 1) / sms) * block + 1500.0 + kWRows * bt * 8 / 30.0;
-        const bool can_cut = tiles <= static_cast<long long>(kF8Counters) && total < 0x7fffffffll && tiles % sms != 0;
+        const bool can_cut = total < 0x7fffffffll && tiles % sms != 0;
         const bool stream = can_cut && cut < whole;
         const double cost = stream ? cut : whole;
         if (cost < best) {

@@ -182,6 +182,33 @@ struct GemmF8 {
 };
 int launch_gemm_f8(const GemmF8& g, int* err, cudaStream_t s);
 
+// A mixture-of-experts layer (moe_f8.cu) over stacks of prepared weights.
+constexpr int kMoeMaxTokens = 64, kMoeMaxTop = 16, kMoeMaxExperts = 256;
+struct MoeWeight {
+    const uint8_t* w = nullptr;  // e4m3 [experts][rows][ld], 16-byte aligned, ld and stride multiples of 16
+    long long ld = 0, stride = 0;
+    const float* scales = nullptr;  // [experts][ceil(rows/128)][ceil(k/128)]
+    long long scale_stride = 0;
+};
+struct MoeF8 {
+    const void* x = nullptr;  // [t][ldx] of type
+    void* out = nullptr;      // [t][ldo] of type
+    int type = kTypeF32;
+    long long ldx = 0, ldo = 0;
+    MoeWeight gate, up, down;      // [e][f][h], [e][f][h], [e][h][f]
+    const void* router = nullptr;  // [e][ld_router] of router_type; null: ids and weights are inputs
+    int router_type = kTypeF32;
+    long long ld_router = 0;
+    int* ids = nullptr;        // [t][top], -1: empty slot
+    float* weights = nullptr;  // [t][top]
+    int t = 0, h = 0, f = 0, e = 0, top = 0, renorm = 0;
+    unsigned* counters = nullptr;  // kF8Counters words
+    void* scratch = nullptr;       // moe_f8_scratch_bytes
+    size_t scratch_bytes = 0;
+};
+size_t moe_f8_scratch_bytes(int t, int h, int f, int e, int top, int type);
+int launch_moe_f8(const MoeF8& m, int* err, cudaStream_t s);
+
 int sm_count();
 // 2-D K-major tensor map (gemm.cu): rows x k elements of 1 or 2 bytes, row
 // pitch ld_bytes, box of 128 bytes x box_rows, 128-byte swizzle, zero fill.

@@ -19,6 +19,8 @@ enum DeviceError : int {
     kErrTimeoutDrain = 5,   // teardown: in-flight copies did not drain
     kErrTimeoutPeer = 6,    // peer barrier: another rank never arrived
     kErrTimeoutQuant = 7,   // GEMM with fused quantiser: token rows never published
+    kErrTimeoutGrid = 8,    // grid barrier: a CTA of the launch never arrived
+    kErrBadIndex = 9,       // an index out of range in a device operand
 };
 
 // Wait limit of every spin in the library (the reference's NPU completion

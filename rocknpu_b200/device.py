@@ -6,9 +6,11 @@ on the current torch stream (or the given one) and returns without waiting.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
-from .capi import BLOCK_BYTES, GGML_BF16, GGML_F16, GGML_F32, lib
+from .capi import BLOCK_BYTES, GGML_BF16, GGML_F16, GGML_F32, F8Experts, MoeF8Args, lib
 
 _TYPES = {torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16}
 F8_BLOCK = 128
@@ -303,3 +305,59 @@ def matmul_f8(a: torch.Tensor, w8: torch.Tensor, w_scales: torch.Tensor, status:
             w_scales.data_ptr(), out.data_ptr(), _TYPES[out.dtype], _pitch(out), m, k, n, workspace.data_ptr(),
             workspace.numel() * workspace.element_size(), status.data_ptr())
     return out
+
+
+def moe_f8_workspace_bytes(tokens: int, hidden: int, ffn: int, experts: int, top_k: int, dtype) -> int:
+    """0 for a shape that moe_f8 does not take."""
+    return int(lib().rocknpu_b200_moe_f8_workspace_bytes(tokens, hidden, ffn, experts, top_k, _TYPES[dtype]))
+
+
+def _f8_experts(w8: torch.Tensor, scales: torch.Tensor, shape, what: str) -> F8Experts:
+    _require(tuple(w8.shape) == shape, f"{what} is an e4m3 tensor of shape {shape}")
+    _f8_weight(w8, scales, what)
+    return F8Experts(w8.data_ptr(), _pitch16(w8), w8.stride(0), scales.data_ptr(), scales.stride(0))
+
+
+def moe_f8(x: torch.Tensor, gate, up, down, status: torch.Tensor, workspace: torch.Tensor, *,
+           router: torch.Tensor | None = None, top_k: int | None = None, renormalize: bool = True,
+           ids: torch.Tensor | None = None, weights: torch.Tensor | None = None, out: torch.Tensor | None = None,
+           stream=None):
+    """A mixture-of-experts layer for up to 64 tokens x [t, hidden].
+
+    gate, up and down are (e4m3, scales) pairs of stacked weights as
+    prepare_f8 returns them, [e, ffn, hidden], [e, ffn, hidden] and
+    [e, hidden, ffn].  With `router` [e, hidden] the layer picks top_k experts
+    per token (softmax over the chosen ones, or over all with
+    renormalize=False); without, int32 `ids` (negative: empty slot) and f32
+    `weights` [t, top_k] say them.  Returns (out, ids, weights).
+    `workspace`: new_workspace(moe_f8_workspace_bytes(...)), kept by the
+    caller, one per stream on which calls may be in flight."""
+    _operands(x, *gate, *up, *down, status, workspace, router, ids, weights, out)
+    _status_word(status)
+    _require(x.dim() == 2 and x.dtype in _TYPES and x.stride(1) == 1 and x.numel() > 0,
+             "x is an f32, f16 or bf16 matrix of whole rows")
+    t, h = x.shape
+    _require(gate[0].dim() == 3, "gate is [experts, ffn, hidden]")
+    e, f = gate[0].shape[:2]
+    if router is not None:
+        _require(top_k is not None and ids is None and weights is None, "a router goes with top_k, ids and weights without")
+        _require(router.dtype in _TYPES and tuple(router.shape) == (e, h) and router.stride(1) == 1,
+                 "router is an f32, f16 or bf16 matrix [experts, hidden]")
+        ids = torch.empty((t, top_k), dtype=torch.int32, device=x.device)
+        weights = torch.empty((t, top_k), dtype=torch.float32, device=x.device)
+    else:
+        _require(ids is not None and weights is not None, "without a router, ids and weights are given")
+        top_k = ids.shape[1] if ids.dim() == 2 else 0
+        _require(ids.dtype == torch.int32 and weights.dtype == torch.float32 and tuple(ids.shape) == (t, top_k) and
+                 ids.shape == weights.shape and ids.is_contiguous() and weights.is_contiguous(),
+                 "ids and weights are contiguous int32 and f32 [tokens, top_k]")
+    out = _f8_out(out, t, h, x.dtype, x.device)
+    _require(out.dtype == x.dtype, "out has x's type")
+    args = MoeF8Args(t, h, f, e, top_k, _TYPES[x.dtype], x.data_ptr(), out.data_ptr(), _pitch(x), _pitch(out),
+                     _f8_experts(*gate, (e, f, h), "gate"), _f8_experts(*up, (e, f, h), "up"),
+                     _f8_experts(*down, (e, h, f), "down"), None if router is None else router.data_ptr(),
+                     _TYPES[torch.float32 if router is None else router.dtype], 0 if router is None else _pitch(router),
+                     1 if renormalize else 0, ids.data_ptr(), weights.data_ptr())
+    _launch("moe_f8", x.device, stream, ctypes.byref(args), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), status.data_ptr())
+    return out, ids, weights

@@ -29,7 +29,7 @@ def blocks_of(n):
 
 
 def scale_of(amax):
-    return torch.where(amax == 0, torch.ones_like(amax), (amax / 448.0).clamp_min(2.0 ** -126))
+    return torch.where(amax == 0, torch.ones_like(amax), (amax * torch.tensor(1.0 / 448.0)).clamp_min(2.0 ** -126))
 
 
 def ref_rows(a):
