@@ -6,11 +6,11 @@ on the current torch stream (or the given one) and returns without waiting.
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
-from .capi import BLOCK_BYTES, GGML_BF16, GGML_F16, GGML_F32, F8Experts, MoeF8Args, lib
+from .capi import BLOCK_BYTES, GGML_BF16, GGML_F16, GGML_F32, lib
 
 _TYPES = {torch.float32: GGML_F32, torch.float16: GGML_F16, torch.bfloat16: GGML_BF16}
 F8_BLOCK = 128
@@ -145,101 +145,152 @@ def matmul_w8a8(ctx, a: torch.Tensor, w8: torch.Tensor, w_scales: torch.Tensor, 
 #
 # e4m3 tensors are torch.float8_e4m3fn; scales are f32, per row and 128 columns
 # for activations, per 128 x 128 block for weights.  These calls queue on the
-# operands' own device (its current torch stream unless one is given).
+# operands' own device (its current torch stream unless one is given).  A
+# decode call's kernels take a few microseconds, so the checks are written to
+# cost about as much: sizes and strides are read once, and messages are made
+# only for an error.
 
 def _f8_blocks(n: int) -> int:
     return (n + F8_BLOCK - 1) // F8_BLOCK
 
 
-def _require(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
-def _operands(first: torch.Tensor, *others) -> None:
-    _require(first.is_cuda, "operands are CUDA tensors")
+def _device_of(first: torch.Tensor, *others) -> int:
+    dev = first.get_device()
+    if dev < 0:
+        raise ValueError("operands are CUDA tensors")
     for t in others:
-        _require(t is None or t.device == first.device, "all operands are on one device")
+        if t is not None and t.get_device() != dev:
+            raise ValueError("all operands are on one device")
+    return dev
 
 
-def _status_word(status: torch.Tensor) -> None:
-    _require(status.dtype == torch.int32 and status.numel() >= 1, "status is an int32 tensor (new_status)")
+_ENTRY = {}
 
 
-def _launch(name: str, device, stream, *args) -> None:
-    """Call entry point `name` with `device` current; the stream goes last."""
-    with torch.cuda.device(device):
-        _check(getattr(lib(), f"rocknpu_b200_{name}")(*args, _stream(stream)), name)
+def _launch(name: str, dev: int, stream, *args) -> None:
+    """Call entry point `name` with device `dev` current; the stream goes last."""
+    fn = _ENTRY.get(name)
+    if fn is None:
+        fn = _ENTRY[name] = getattr(lib(), "rocknpu_b200_" + name)
+    handle = torch._C._cuda_getCurrentRawStream(dev) if stream is None else _stream(stream)
+    if torch._C._cuda_getDevice() == dev:
+        st = fn(*args, handle)
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, handle)
+    if st != 0:
+        raise RuntimeError(f"{name} failed with status {st}")
+
+
+def _status_ptr(status: torch.Tensor) -> int:
+    if status.dtype is not torch.int32 or status.numel() < 1:
+        raise ValueError("status is an int32 tensor (new_status)")
+    return status.data_ptr()
 
 
 def _f8_empty(*shape, device) -> torch.Tensor:
     """e4m3 tensor whose rows start at multiples of 16 bytes."""
-    k16 = (shape[-1] + 15) // 16 * 16
-    return torch.empty((*shape[:-1], k16), dtype=torch.float8_e4m3fn, device=device)[..., :shape[-1]]
+    k = shape[-1]
+    if k % 16 == 0:
+        return torch.empty(shape, dtype=torch.float8_e4m3fn, device=device)
+    return torch.empty((*shape[:-1], (k + 15) // 16 * 16), dtype=torch.float8_e4m3fn, device=device)[..., :k]
 
 
-def _f8_weight(w8: torch.Tensor, scales: torch.Tensor, what: str) -> None:
-    n, k = w8.shape[-2:]
-    _require(w8.dtype == torch.float8_e4m3fn and w8.stride(-1) == 1 and w8.stride(-2) >= k,
-             f"{what} is an e4m3 tensor of whole rows")
-    _require(scales.dtype == torch.float32 and scales.is_contiguous() and
-             tuple(scales.shape) == (*w8.shape[:-2], _f8_blocks(n), _f8_blocks(k)),
-             f"{what} scales are a contiguous f32 tensor, one per 128 x 128 block")
+def _dense_rows(t: torch.Tensor, what: str):
+    """(rows, columns, row pitch, type id) of a dense matrix of whole rows.  A
+    single row's stride says nothing."""
+    type_ = _TYPES.get(t.dtype)
+    if type_ is None or t.dim() != 2 or t.numel() == 0:
+        raise ValueError(f"{what} is an f32, f16 or bf16 matrix, not empty")
+    (m, k), (ld, step) = t.shape, t.stride()
+    if step != 1 and k > 1:
+        raise ValueError(f"{what} is a matrix of whole rows")
+    return m, k, ld if m > 1 else max(k, ld), type_
+
+
+def _f8_rows(t: torch.Tensor, what: str):
+    """(rows, columns, row pitch) of an e4m3 operand; a single row may end at k."""
+    if t.dtype is not torch.float8_e4m3fn or t.dim() != 2 or t.numel() == 0:
+        raise ValueError(f"{what} is an e4m3 matrix, not empty")
+    (m, k), (ld, step) = t.shape, t.stride()
+    if step != 1 and k > 1:
+        raise ValueError(f"{what} is a matrix of whole rows")
+    return m, k, ld if m > 1 else (k + 15) // 16 * 16
+
+
+def _row_scales(s: torch.Tensor, m: int, k: int, what: str) -> int:
+    """Row pitch of activation scales [m, ceil(k / 128)]."""
+    kb = _f8_blocks(k)
+    if s.dtype is not torch.float32 or s.shape != (m, kb):
+        raise ValueError(f"{what} are f32 [m, ceil(k / 128)]")
+    ld, step = s.stride()
+    if step != 1 and kb > 1:
+        raise ValueError(f"{what} are a matrix of whole rows")
+    return ld if m > 1 else max(kb, ld)
+
+
+def _weight_scales(s: torch.Tensor, shape, what: str) -> None:
+    if s.dtype is not torch.float32 or s.shape != shape or not s.is_contiguous():
+        raise ValueError(f"{what} scales are contiguous f32 {tuple(shape)}, one per 128 x 128 block")
+
+
+def _dense_out(out, m: int, n: int, dtype, device):
+    """(out, type id, row pitch), made when None."""
+    if out is None:
+        if dtype not in _TYPES:
+            raise ValueError("results are f32, f16 or bf16")
+        return torch.empty((m, n), dtype=dtype, device=device), _TYPES[dtype], n
+    rows, cols, ld, type_ = _dense_rows(out, "out")
+    if rows != m or cols != n:
+        raise ValueError(f"out has shape {(m, n)}")
+    return out, type_, ld
 
 
 def quantize_rows_f8(a: torch.Tensor, status: torch.Tensor, out: torch.Tensor | None = None,
                      scales: torch.Tensor | None = None, stream=None):
     """f32 / f16 / bf16 [m, k] -> (e4m3 [m, k], f32 scales [m, ceil(k / 128)])."""
-    _operands(a, status, out, scales)
-    _status_word(status)
-    _require(a.dim() == 2 and a.dtype in _TYPES and a.stride(1) == 1, "a is an f32, f16 or bf16 matrix of whole rows")
-    m, k = a.shape
-    _require(m > 0 and k > 0, "a is not empty")
-    out = _f8_empty(m, k, device=a.device) if out is None else out
-    scales = torch.empty((m, _f8_blocks(k)), dtype=torch.float32, device=a.device) if scales is None else scales
-    _require(out.dtype == torch.float8_e4m3fn and out.shape == a.shape and out.stride(1) == 1,
-             "out is an e4m3 matrix of a's shape")
-    _require(scales.dtype == torch.float32 and tuple(scales.shape) == (m, _f8_blocks(k)) and
-             (scales.stride(1) == 1 or scales.shape[1] == 1), "scales are f32 [m, ceil(k / 128)]")
-    _launch("quantize_rows_f8", a.device, stream, _TYPES[a.dtype], a.data_ptr(), m, k, _pitch(a), out.data_ptr(),
-            _pitch(out), scales.data_ptr(), _pitch(scales), status.data_ptr())
+    dev = _device_of(a, status, out, scales)
+    m, k, lda, type_ = _dense_rows(a, "a")
+    if out is None:
+        out = _f8_empty(m, k, device=a.device)
+    if scales is None:
+        scales = torch.empty((m, _f8_blocks(k)), dtype=torch.float32, device=a.device)
+    rows, cols, ld8 = _f8_rows(out, "out")
+    if rows != m or cols != k:
+        raise ValueError("out has a's shape")
+    _launch("quantize_rows_f8", dev, stream, type_, a.data_ptr(), m, k, lda, out.data_ptr(), ld8, scales.data_ptr(),
+            _row_scales(scales, m, k, "scales"), _status_ptr(status))
     return out, scales
-
-
-def _pitch(t: torch.Tensor) -> int:
-    """Row pitch in elements; a single row's stride says nothing."""
-    return t.stride(-2) if t.shape[-2] > 1 else max(t.shape[-1], t.stride(-2))
 
 
 def prepare_f8(w: torch.Tensor, status: torch.Tensor, stream=None):
     """Dense weight(s) [n, k] or [experts, n, k] -> (e4m3 of the same shape,
     f32 scales [..., ceil(n / 128), ceil(k / 128)])."""
-    _operands(w, status)
-    _status_word(status)
-    _require(w.dim() in (2, 3) and w.dtype in _TYPES and w.stride(-1) == 1 and w.numel() > 0,
-             "w is an f32, f16 or bf16 matrix, or a stack of them, of whole rows")
-    n, k = w.shape[-2:]
+    dev = _device_of(w, status)
+    if w.dim() not in (2, 3):
+        raise ValueError("w is a matrix or a stack of them")
+    n, k, ldw, type_ = _dense_rows(w if w.dim() == 2 else w[0] if w.shape[0] else w.flatten(0, 1), "w")
     count = w.shape[0] if w.dim() == 3 else 1
-    ldw = _pitch(w)
-    _require(count == 1 or w.stride(0) == n * ldw, "a stack of weights has no gaps between them")
+    if count > 1 and w.stride(0) != n * ldw:
+        raise ValueError("a stack of weights has no gaps between them")
     out = _f8_empty(*w.shape, device=w.device)
     scales = torch.empty((*w.shape[:-2], _f8_blocks(n), _f8_blocks(k)), dtype=torch.float32, device=w.device)
-    _launch("prepare_f8", w.device, stream, _TYPES[w.dtype], w.data_ptr(), n, k, ldw, count, out.data_ptr(),
-            (k + 15) // 16 * 16, scales.data_ptr(), status.data_ptr())
+    _launch("prepare_f8", dev, stream, type_, w.data_ptr(), n, k, ldw, count, out.data_ptr(), (k + 15) // 16 * 16,
+            scales.data_ptr(), _status_ptr(status))
     return out, scales
 
 
 def prepare_f8_q(kind: int, blocks: torch.Tensor, k: int, n: int, status: torch.Tensor, stream=None):
     """K-quant rows -> (e4m3 [n, k], f32 scales [ceil(n / 128), k / 128])."""
-    _operands(blocks, status)
-    _status_word(status)
-    _require(blocks.dtype == torch.uint8 and blocks.is_contiguous(), "blocks are contiguous uint8")
-    _require(kind in BLOCK_BYTES and k > 0 and n > 0 and k % 256 == 0 and
-             blocks.numel() >= n * (k // 256) * BLOCK_BYTES[kind], "blocks hold n rows of k / 256 superblocks")
+    dev = _device_of(blocks, status)
+    if blocks.dtype is not torch.uint8 or not blocks.is_contiguous():
+        raise ValueError("blocks are contiguous uint8")
+    if kind not in BLOCK_BYTES or k <= 0 or n <= 0 or k % 256 or blocks.numel() < n * (k // 256) * BLOCK_BYTES[kind]:
+        raise ValueError("blocks hold n rows of k / 256 superblocks")
     out = torch.empty((n, k), dtype=torch.float8_e4m3fn, device=blocks.device)
     scales = torch.empty((_f8_blocks(n), _f8_blocks(k)), dtype=torch.float32, device=blocks.device)
-    _launch("prepare_f8_q", blocks.device, stream, kind, blocks.data_ptr(), k, n, out.data_ptr(), k,
-            scales.data_ptr(), status.data_ptr())
+    _launch("prepare_f8_q", dev, stream, kind, blocks.data_ptr(), k, n, out.data_ptr(), k, scales.data_ptr(),
+            _status_ptr(status))
     return out, scales
 
 
@@ -251,39 +302,23 @@ def matmul_f8_workspace_bytes(m: int, n: int, k: int) -> int:
     return int(lib().rocknpu_b200_matmul_f8_workspace_bytes(m, n, k))
 
 
-def _f8_out(out, m: int, n: int, dtype, device) -> torch.Tensor:
-    out = torch.empty((m, n), dtype=dtype, device=device) if out is None else out
-    _require(out.dtype in _TYPES and tuple(out.shape) == (m, n) and (out.stride(1) == 1 or n == 1),
-             f"out is an f32, f16 or bf16 matrix of shape {(m, n)}")
-    return out
-
-
 def gemm_f8(a8: torch.Tensor, a_scales: torch.Tensor, w8: torch.Tensor, w_scales: torch.Tensor,
             status: torch.Tensor, out: torch.Tensor | None = None, out_dtype=torch.float32,
             workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """Block-scaled e4m3 product a8 [m, k] . w8 [n, k]^T (quantize_rows_f8,
     prepare_f8).  Rows start at multiples of 16 bytes."""
-    _operands(a8, a_scales, w8, w_scales, status, out, workspace)
-    _status_word(status)
-    _require(a8.dim() == 2 and a8.dtype == torch.float8_e4m3fn and a8.stride(1) == 1 and a8.numel() > 0,
-             "a8 is an e4m3 matrix of whole rows")
-    m, k = a8.shape
-    _require(w8.dim() == 2 and w8.shape[1] == k and w8.numel() > 0, "w8 is [n, k]")
-    _f8_weight(w8, w_scales, "w8")
-    _require(a_scales.dtype == torch.float32 and tuple(a_scales.shape) == (m, _f8_blocks(k)) and
-             (a_scales.stride(1) == 1 or a_scales.shape[1] == 1), "a_scales are f32 [m, ceil(k / 128)]")
-    n = w8.shape[0]
-    out = _f8_out(out, m, n, out_dtype, a8.device)
-    _launch("gemm_f8", a8.device, stream, a8.data_ptr(), _pitch16(a8), a_scales.data_ptr(), _pitch(a_scales),
-            w8.data_ptr(), _pitch16(w8), w_scales.data_ptr(), out.data_ptr(), _TYPES[out.dtype], _pitch(out), m, k, n,
-            workspace.data_ptr() if workspace is not None else None,
-            workspace.numel() * workspace.element_size() if workspace is not None else 0, status.data_ptr())
+    dev = _device_of(a8, a_scales, w8, w_scales, status, out, workspace)
+    m, k, lda = _f8_rows(a8, "a8")
+    n, kw, ldw = _f8_rows(w8, "w8")
+    if kw != k:
+        raise ValueError("w8 is [n, k]")
+    _weight_scales(w_scales, (_f8_blocks(n), _f8_blocks(k)), "w8")
+    out, out_type, ldo = _dense_out(out, m, n, out_dtype, a8.device)
+    _launch("gemm_f8", dev, stream, a8.data_ptr(), lda, a_scales.data_ptr(), _row_scales(a_scales, m, k, "a_scales"),
+            w8.data_ptr(), ldw, w_scales.data_ptr(), out.data_ptr(), out_type, ldo, m, k, n,
+            None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.nbytes,
+            _status_ptr(status))
     return out
-
-
-def _pitch16(t: torch.Tensor) -> int:
-    """Row pitch of an e4m3 operand; a single row has none, and may end at k."""
-    return t.stride(-2) if t.shape[-2] > 1 else (t.shape[-1] + 15) // 16 * 16
 
 
 def matmul_f8(a: torch.Tensor, w8: torch.Tensor, w_scales: torch.Tensor, status: torch.Tensor,
@@ -292,18 +327,15 @@ def matmul_f8(a: torch.Tensor, w8: torch.Tensor, w_scales: torch.Tensor, status:
     weight; the result has a's type unless `out` or `out_dtype` says another.
     `workspace` (new_workspace of matmul_f8_workspace_bytes) is kept by the
     caller, one per stream on which calls may be in flight."""
-    _operands(a, w8, w_scales, status, workspace, out)
-    _status_word(status)
-    _require(a.dim() == 2 and a.dtype in _TYPES and a.stride(1) == 1 and a.numel() > 0,
-             "a is an f32, f16 or bf16 matrix of whole rows")
-    m, k = a.shape
-    _require(w8.dim() == 2 and w8.shape[1] == k and w8.numel() > 0, "w8 is [n, k]")
-    _f8_weight(w8, w_scales, "w8")
-    n = w8.shape[0]
-    out = _f8_out(out, m, n, out_dtype or a.dtype, a.device)
-    _launch("matmul_f8", a.device, stream, a.data_ptr(), _TYPES[a.dtype], _pitch(a), w8.data_ptr(), _pitch16(w8),
-            w_scales.data_ptr(), out.data_ptr(), _TYPES[out.dtype], _pitch(out), m, k, n, workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), status.data_ptr())
+    dev = _device_of(a, w8, w_scales, status, workspace, out)
+    m, k, lda, type_ = _dense_rows(a, "a")
+    n, kw, ldw = _f8_rows(w8, "w8")
+    if kw != k:
+        raise ValueError("w8 is [n, k]")
+    _weight_scales(w_scales, (_f8_blocks(n), _f8_blocks(k)), "w8")
+    out, out_type, ldo = _dense_out(out, m, n, out_dtype or a.dtype, a.device)
+    _launch("matmul_f8", dev, stream, a.data_ptr(), type_, lda, w8.data_ptr(), ldw, w_scales.data_ptr(),
+            out.data_ptr(), out_type, ldo, m, k, n, workspace.data_ptr(), workspace.nbytes, _status_ptr(status))
     return out
 
 
@@ -312,10 +344,21 @@ def moe_f8_workspace_bytes(tokens: int, hidden: int, ffn: int, experts: int, top
     return int(lib().rocknpu_b200_moe_f8_workspace_bytes(tokens, hidden, ffn, experts, top_k, _TYPES[dtype]))
 
 
-def _f8_experts(w8: torch.Tensor, scales: torch.Tensor, shape, what: str) -> F8Experts:
-    _require(tuple(w8.shape) == shape, f"{what} is an e4m3 tensor of shape {shape}")
-    _f8_weight(w8, scales, what)
-    return F8Experts(w8.data_ptr(), _pitch16(w8), w8.stride(0), scales.data_ptr(), scales.stride(0))
+# The bytes of a rocknpu_b200_moe_f8_args (capi.MoeF8Args names its fields).
+_MOE_ARGS = struct.Struct("@5N I PPNN PNNPN PNNPN PNNPN P I N i PP")
+
+
+def _experts(weight, shape, what: str):
+    """The fields of a rocknpu_b200_f8_experts."""
+    w8, scales = weight
+    if w8.dtype is not torch.float8_e4m3fn or w8.shape != shape:
+        raise ValueError(f"{what} is an e4m3 tensor of shape {shape}")
+    e, n, k = shape
+    stride, ld, step = w8.stride()
+    if step != 1 and k > 1:
+        raise ValueError(f"{what} is a stack of matrices of whole rows")
+    _weight_scales(scales, (e, _f8_blocks(n), _f8_blocks(k)), what)
+    return w8.data_ptr(), ld if n > 1 else (k + 15) // 16 * 16, stride, scales.data_ptr(), scales.stride(0)
 
 
 def moe_f8(x: torch.Tensor, gate, up, down, status: torch.Tensor, workspace: torch.Tensor, *,
@@ -332,32 +375,34 @@ def moe_f8(x: torch.Tensor, gate, up, down, status: torch.Tensor, workspace: tor
     `weights` [t, top_k] say them.  Returns (out, ids, weights).
     `workspace`: new_workspace(moe_f8_workspace_bytes(...)), kept by the
     caller, one per stream on which calls may be in flight."""
-    _operands(x, *gate, *up, *down, status, workspace, router, ids, weights, out)
-    _status_word(status)
-    _require(x.dim() == 2 and x.dtype in _TYPES and x.stride(1) == 1 and x.numel() > 0,
-             "x is an f32, f16 or bf16 matrix of whole rows")
-    t, h = x.shape
-    _require(gate[0].dim() == 3, "gate is [experts, ffn, hidden]")
-    e, f = gate[0].shape[:2]
+    dev = _device_of(x, *gate, *up, *down, status, workspace, router, ids, weights, out)
+    t, h, ldx, type_ = _dense_rows(x, "x")
+    if gate[0].dim() != 3:
+        raise ValueError("gate is [experts, ffn, hidden]")
+    e, f, _ = gate[0].shape
     if router is not None:
-        _require(top_k is not None and ids is None and weights is None, "a router goes with top_k, ids and weights without")
-        _require(router.dtype in _TYPES and tuple(router.shape) == (e, h) and router.stride(1) == 1,
-                 "router is an f32, f16 or bf16 matrix [experts, hidden]")
+        if top_k is None or top_k < 1 or ids is not None or weights is not None:
+            raise ValueError("a router goes with top_k, ids and weights without")
+        rows, cols, ld_router, router_type = _dense_rows(router, "router")
+        if rows != e or cols != h:
+            raise ValueError("router is [experts, hidden]")
         ids = torch.empty((t, top_k), dtype=torch.int32, device=x.device)
         weights = torch.empty((t, top_k), dtype=torch.float32, device=x.device)
     else:
-        _require(ids is not None and weights is not None, "without a router, ids and weights are given")
-        top_k = ids.shape[1] if ids.dim() == 2 else 0
-        _require(ids.dtype == torch.int32 and weights.dtype == torch.float32 and tuple(ids.shape) == (t, top_k) and
-                 ids.shape == weights.shape and ids.is_contiguous() and weights.is_contiguous(),
-                 "ids and weights are contiguous int32 and f32 [tokens, top_k]")
-    out = _f8_out(out, t, h, x.dtype, x.device)
-    _require(out.dtype == x.dtype, "out has x's type")
-    args = MoeF8Args(t, h, f, e, top_k, _TYPES[x.dtype], x.data_ptr(), out.data_ptr(), _pitch(x), _pitch(out),
-                     _f8_experts(*gate, (e, f, h), "gate"), _f8_experts(*up, (e, f, h), "up"),
-                     _f8_experts(*down, (e, h, f), "down"), None if router is None else router.data_ptr(),
-                     _TYPES[torch.float32 if router is None else router.dtype], 0 if router is None else _pitch(router),
-                     1 if renormalize else 0, ids.data_ptr(), weights.data_ptr())
-    _launch("moe_f8", x.device, stream, ctypes.byref(args), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), status.data_ptr())
+        ld_router = router_type = 0
+        if ids is None or weights is None or ids.dim() != 2 or ids.shape[0] != t or ids.shape != weights.shape or \
+                ids.dtype is not torch.int32 or weights.dtype is not torch.float32 or \
+                not ids.is_contiguous() or not weights.is_contiguous():
+            raise ValueError("without a router, ids and weights are contiguous int32 and f32 [tokens, top_k]")
+        if top_k is not None and top_k != ids.shape[1]:
+            raise ValueError("ids and weights are [tokens, top_k]")
+        top_k = ids.shape[1]
+    out, out_type, ldo = _dense_out(out, t, h, x.dtype, x.device)
+    if out_type != type_:
+        raise ValueError("out has x's type")
+    args = _MOE_ARGS.pack(t, h, f, e, top_k, type_, x.data_ptr(), out.data_ptr(), ldx, ldo,
+                          *_experts(gate, (e, f, h), "gate"), *_experts(up, (e, f, h), "up"),
+                          *_experts(down, (e, h, f), "down"), 0 if router is None else router.data_ptr(), router_type,
+                          ld_router, 1 if renormalize else 0, ids.data_ptr(), weights.data_ptr())
+    _launch("moe_f8", dev, stream, args, workspace.data_ptr(), workspace.nbytes, _status_ptr(status))
     return out, ids, weights
