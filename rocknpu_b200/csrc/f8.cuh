@@ -31,6 +31,45 @@ __device__ __forceinline__ uint32_t f8_pack4(float a, float b, float c, float d)
     return f8_pack2(a, b) | (f8_pack2(c, d) << 16);
 }
 
+// fl(x / s) for the values of a block whose scale is s.  Markstein's method
+// (IBM J. Res. Dev. 34, 1990): with y = RN(1 / s), a quotient q off by less
+// than a unit in the last place and its exact remainder r = x - q s (one
+// fused multiply-add), q + r y rounds to the IEEE quotient.  x y is off by at
+// most 1.5 units, so a first step brings it within one and a second makes it
+// exact: five multiply-adds where the IEEE division takes about thirty
+// instructions.  The remainder of a quotient that matters (2^-11 and more;
+// smaller ones are 0 in e4m3) is exact for s >= 2^-100; below that, and in no
+// real tensor, the division itself.
+__device__ __forceinline__ float f8_quotient(float x, float s, float y) {
+    float q = __fmul_rn(x, y);
+    q = __fmaf_rn(__fmaf_rn(-q, s, x), y, q);
+    q = __fmaf_rn(__fmaf_rn(-q, s, x), y, q);
+    return copysignf(q, x);  // a quotient of -0 came out as 0
+}
+
+// e4m3 codes of a thread's values of one block (N a multiple of 4), four per
+// word.  The rare scale is decided once for all of them.
+template <int N>
+__device__ __forceinline__ void f8_codes(const float (&v)[N], float s, uint32_t (&code)[N / 4]) {
+    float q[N];
+    if (s >= 7.88860905e-31f) {
+        const float y = __frcp_rn(s);
+#pragma unroll
+        for (int i = 0; i < N; ++i) q[i] = f8_quotient(v[i], s, y);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) q[i] = __fdiv_rn(v[i], s);
+    }
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) code[i] = f8_pack4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
+}
+
+// Largest magnitude as an integer: f32 bits without the sign order like the
+// magnitudes, infinities and NaN above every finite value, so one maximum
+// both finds the scale and shows a non-finite value.
+__device__ __forceinline__ uint32_t mag_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+__device__ __forceinline__ bool mag_finite(uint32_t m) { return m < 0x7F800000u; }
+
 template <class T>
 __device__ __forceinline__ float to_f32(T v);
 template <>
@@ -61,29 +100,53 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
     return __float2bfloat16_rn(v);
 }
 
-// Eight consecutive values at a 16-byte boundary.
+// Eight consecutive values as they lie in memory.
 template <class T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-        v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+struct Raw8 {
+    static constexpr int kWords = sizeof(T) * 2;
+    uint32_t w[kWords];
+    // p at a 16-byte boundary
+    __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            T lo, hi;
-            const unsigned short l = static_cast<unsigned short>(w[i] & 0xFFFFu),
-                                 h = static_cast<unsigned short>(w[i] >> 16);
-            if constexpr (sizeof(T) == 2) {
-                memcpy(&lo, &l, 2);
-                memcpy(&hi, &h, 2);
-            }
-            v[2 * i] = to_f32<T>(lo);
-            v[2 * i + 1] = to_f32<T>(hi);
+        for (int i = 0; i < kWords / 4; ++i) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
         }
     }
-}
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0u;
+    }
+    // up to n of them, at any boundary; 0 behind
+    __device__ __forceinline__ void load_some(const T* p, int n) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            uint32_t b = 0u;
+            if (i < n) {
+                if constexpr (sizeof(T) == 4)
+                    b = __float_as_uint(p[i]);
+                else
+                    b = reinterpret_cast<const unsigned short*>(p)[i];
+            }
+            if constexpr (sizeof(T) == 4)
+                w[i] = b;
+            else
+                w[i / 2] = (i & 1) ? (w[i / 2] | (b << 16)) : b;
+        }
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                v[i] = __uint_as_float(w[i]);
+            } else {
+                const unsigned short b = static_cast<unsigned short>((i & 1) ? w[i / 2] >> 16 : w[i / 2] & 0xFFFFu);
+                T x;
+                memcpy(&x, &b, 2);
+                v[i] = to_f32<T>(x);
+            }
+        }
+    }
+};
 
 }  // namespace rk

@@ -16,82 +16,116 @@ namespace rk {
 namespace {
 
 constexpr int kRowsThreads = 256;
-constexpr int kUnroll = 4;  // blocks of 128 that a half-warp has in flight
+constexpr int kRowsUnroll = 2;  // blocks of 128 per half-warp and step
+template <class T>
+constexpr int kRowsCtas = sizeof(T) == 4 ? 4 : 5;  // per SM
 
-__device__ __forceinline__ float half_warp_max(float v) {
+__device__ __forceinline__ uint32_t half_warp_max(uint32_t v) {
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    for (int o = 8; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
+}
+
+template <int N>
+__device__ __forceinline__ uint32_t mag_max(const float (&v)[N]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = max(m, mag_bits(v[i]));
+    return m;
 }
 
 // Values col..col+7 of a row that ends at k; 0 behind it.
 template <class T, bool VEC>
-__device__ __forceinline__ void row_load8(const T* row, int col, int k, float (&v)[8]) {
-    if (VEC && col + 8 <= k) {
-        load8(row + col, v);
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = col + i < k ? to_f32<T>(row[col + i]) : 0.0f;
+__device__ __forceinline__ void row_load8(const T* row, int col, int k, Raw8<T>& v) {
+    if (VEC && col + 8 <= k)
+        v.load(row + col);
+    else
+        v.load_some(row + col, k - col);
 }
 
 template <bool VEC>
 __device__ __forceinline__ void row_store8(uint8_t* row, int col, int k, const float (&v)[8], float s) {
-    float q[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = __fdiv_rn(v[i], s);
-    const uint32_t lo = f8_pack4(q[0], q[1], q[2], q[3]), hi = f8_pack4(q[4], q[5], q[6], q[7]);
+    uint32_t code[2];
+    f8_codes(v, s, code);
     if (VEC && col + 8 <= k) {
-        *reinterpret_cast<uint2*>(row + col) = make_uint2(lo, hi);
+        *reinterpret_cast<uint2*>(row + col) = make_uint2(code[0], code[1]);
         return;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        if (col + i < k) row[col + i] = static_cast<uint8_t>((i < 4 ? lo : hi) >> (8 * (i & 3)));
+        if (col + i < k) row[col + i] = static_cast<uint8_t>(code[i / 4] >> (8 * (i & 3)));
 }
 
-// A half-warp per block, 8 consecutive values per lane, kUnroll blocks per
-// half-warp with all their loads in flight.  Triggers the dependent product
-// at its start: that reads nothing of this kernel's before its own wait.
+// Block b of the walk: column block c of row r.
+struct At {
+    unsigned b, r, c;
+    __device__ __forceinline__ void set(unsigned to, unsigned kb) {
+        b = to;
+        r = to / kb;
+        c = to - r * kb;
+    }
+    __device__ __forceinline__ void on(const At& by, unsigned kb) {
+        b += by.b;
+        r += by.r;
+        c += by.c;
+        if (c >= kb) {
+            c -= kb;
+            ++r;
+        }
+    }
+};
+
+// A half-warp per kRowsUnroll consecutive blocks, 8 consecutive values per
+// lane and block; a step's loads are issued before the step before it is
+// quantised.  Triggers the dependent product at its start: that reads nothing
+// of this kernel's before its own wait.
 template <class T, bool VEC>
-__global__ void __launch_bounds__(kRowsThreads) rows_f8_kernel(const T* __restrict__ a, int k, long long lda,
-                                                               unsigned kb, unsigned blocks,
-                                                               uint8_t* __restrict__ out, long long ld8,
-                                                               float* __restrict__ scales, long long lds, int* err) {
+__global__ void __launch_bounds__(kRowsThreads, kRowsCtas<T>)
+    rows_f8_kernel(const T* __restrict__ a, int k, long long lda, unsigned kb, unsigned blocks,
+                   uint8_t* __restrict__ out, long long ld8, float* __restrict__ scales, long long lds, int* err) {
+    constexpr int U = kRowsUnroll;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const unsigned half = (blockIdx.x * kRowsThreads + threadIdx.x) >> 4;
-    const unsigned halves = gridDim.x * (kRowsThreads / 16);
     const int lane = threadIdx.x & 15;
-    float v[kUnroll][8];
+    At at, step, one;
+    one.set(1, kb);
+    step.set(gridDim.x * (kRowsThreads / 16) * U, kb);
+    at.set((blockIdx.x * (kRowsThreads / 16) + (threadIdx.x >> 4)) * U, kb);
+    auto load = [&](At p, Raw8<T>(&v)[U]) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-        const unsigned b = half + u * halves;
-        const unsigned r = b / kb;
-        if (b < blocks) {
-            row_load8<T, VEC>(a + r * lda, static_cast<int>(b - r * kb) * kF8Block + lane * 8, k, v[u]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
+        for (int u = 0; u < U; ++u) {
+            if (p.b < blocks)
+                row_load8<T, VEC>(a + p.r * lda, static_cast<int>(p.c) * kF8Block + lane * 8, k, v[u]);
+            else
+                v[u].clear();
+            p.on(one, kb);
         }
+    };
+    Raw8<T> cur[U];
+    load(at, cur);
+    const unsigned odd = (threadIdx.x >> 4 & 1) * U;  // the two halves of a warp take the same steps
+    uint32_t most = 0;
+    while (at.b - odd < blocks) {
+        Raw8<T> next[U];
+        At then = at;
+        then.on(step, kb);
+        load(then, next);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float v[8];
+            cur[u].values(v);
+            const uint32_t m = half_warp_max(mag_max(v));
+            most = max(most, m);
+            const float s = f8_scale(__uint_as_float(m));
+            if (at.b < blocks) {
+                row_store8<VEC>(out + at.r * ld8, static_cast<int>(at.c) * kF8Block + lane * 8, k, v, s);
+                if (lane == 0) scales[at.r * lds + at.c] = s;
+            }
+            at.on(one, kb);
+            cur[u] = next[u];
+        }
+        at = then;
     }
-    bool finite = true;
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-        const unsigned b = half + u * halves;
-        const unsigned r = b / kb, c = b - r * kb;
-        float amax = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            amax = fmaxf(amax, fabsf(v[u][i]));
-            finite &= isfinite(v[u][i]);
-        }
-        const float s = f8_scale(half_warp_max(amax));
-        if (b < blocks) {
-            row_store8<VEC>(out + r * ld8, static_cast<int>(c) * kF8Block + lane * 8, k, v[u], s);
-            if (lane == 0) scales[r * lds + c] = s;
-        }
-    }
-    if (!finite) atomicExch(err, kErrNonFinite);
+    if (!mag_finite(most)) atomicExch(err, kErrNonFinite);
 }
 
 template <class T>
@@ -100,8 +134,8 @@ int rows_f8(const T* a, int m, int k, long long lda, uint8_t* out, long long ld8
     const unsigned kb = static_cast<unsigned>((k + kF8Block - 1) / kF8Block);
     const unsigned long long total = static_cast<unsigned long long>(m) * kb;
     if (total > 0xF0000000ull) return cudaErrorInvalidValue;
-    const unsigned per = kRowsThreads / 16 * kUnroll;
-    const unsigned grid = static_cast<unsigned>((total + per - 1) / per);
+    const unsigned per = kRowsThreads / 16 * kRowsUnroll;
+    const unsigned grid = static_cast<unsigned>(std::min<unsigned long long>((total + per - 1) / per, sm_count() * kRowsCtas<T>));
     const bool vec = (reinterpret_cast<uintptr_t>(a) % 16 == 0) && (lda * sizeof(T)) % 16 == 0 &&
                      (reinterpret_cast<uintptr_t>(out) % 8 == 0) && ld8 % 8 == 0;
     auto kern = vec ? rows_f8_kernel<T, true> : rows_f8_kernel<T, false>;
@@ -123,24 +157,24 @@ int rows_f8(const T* a, int m, int k, long long lda, uint8_t* out, long long ld8
 constexpr int kPrepThreads = 256;
 
 template <int THREADS>
-__device__ __forceinline__ float cta_max(float v, float* red) {
-    v = warp_max(v);
+__device__ __forceinline__ uint32_t cta_max(uint32_t v, uint32_t* red) {
+    v = __reduce_max_sync(0xffffffffu, v);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
-    float r = red[0];
+    uint32_t r = red[0];
 #pragma unroll
-    for (int w = 1; w < THREADS / 32; ++w) r = fmaxf(r, red[w]);
+    for (int w = 1; w < THREADS / 32; ++w) r = max(r, red[w]);
     return r;
 }
 
 // One CTA per block: 16 lanes of 8 values per row, 16 rows per pass, 8 passes
 // held in registers.
 template <class T, bool VEC>
-__global__ void __launch_bounds__(kPrepThreads) prep_f8_dense_kernel(const T* __restrict__ w, int n, int k,
+__global__ void __launch_bounds__(kPrepThreads, sizeof(T) == 4 ? 2 : 4) prep_f8_dense_kernel(const T* __restrict__ w, int n, int k,
                                                                      long long ldw, unsigned nb, unsigned kb,
                                                                      uint8_t* __restrict__ out, long long ld8,
                                                                      float* __restrict__ scales, int* err) {
-    __shared__ float red[kPrepThreads / 32];
+    __shared__ uint32_t red[kPrepThreads / 32];
     const unsigned per = nb * kb;
     const unsigned mat = blockIdx.x / per, b = blockIdx.x - mat * per;
     const unsigned rb = b / kb, cb = b - rb * kb;
@@ -148,33 +182,34 @@ __global__ void __launch_bounds__(kPrepThreads) prep_f8_dense_kernel(const T* __
     const int row0 = static_cast<int>(rb) * kF8Block + (threadIdx.x >> 4);
     w += static_cast<long long>(mat) * n * ldw;
     out += static_cast<long long>(mat) * n * ld8;
-    float v[8][8];
+    Raw8<T> raw[8];
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
         const int r = row0 + 16 * p;
-        if (r < n) {
-            row_load8<T, VEC>(w + r * ldw, col, k, v[p]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[p][i] = 0.0f;
-        }
+        if (r < n)
+            row_load8<T, VEC>(w + r * ldw, col, k, raw[p]);
+        else
+            raw[p].clear();
     }
-    float amax = 0.0f;
-    bool finite = true;
+    uint32_t m = 0;
 #pragma unroll
-    for (int p = 0; p < 8; ++p)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            amax = fmaxf(amax, fabsf(v[p][i]));
-            finite &= isfinite(v[p][i]);
-        }
-    if (!finite) atomicExch(err, kErrNonFinite);
-    const float s = f8_scale(cta_max<kPrepThreads>(amax, red));
-    if (threadIdx.x == 0) scales[blockIdx.x] = s;
+    for (int p = 0; p < 8; ++p) {
+        float v[8];
+        raw[p].values(v);
+        m = max(m, mag_max(v));
+    }
+    m = cta_max<kPrepThreads>(m, red);
+    const float s = f8_scale(__uint_as_float(m));
+    if (threadIdx.x == 0) {
+        if (!mag_finite(m)) atomicExch(err, kErrNonFinite);
+        scales[blockIdx.x] = s;
+    }
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
         const int r = row0 + 16 * p;
-        if (r < n) row_store8<VEC>(out + r * ld8, col, k, v[p], s);
+        float v[8];
+        raw[p].values(v);
+        if (r < n) row_store8<VEC>(out + r * ld8, col, k, v, s);
     }
 }
 
@@ -188,33 +223,31 @@ __global__ void __launch_bounds__(kKqThreads) prep_f8_kq_kernel(const uint8_t* _
                                                                 unsigned sb, uint8_t* __restrict__ out,
                                                                 long long ld8, float* __restrict__ scales, int* err) {
     constexpr int kBytes = KIND == kQ4K ? 144 : KIND == kQ5K ? 176 : 210;
-    __shared__ float red[2][kKqThreads / 32];
+    __shared__ uint32_t red[2][kKqThreads / 32];
     const unsigned rb = blockIdx.x / sb, cb = blockIdx.x - rb * sb;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float v[4][8];
-    float amax = 0.0f;
-    bool finite = true;
+    uint32_t m = 0;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
         const long long r = static_cast<long long>(rb) * kF8Block + warp * 4 + p;
         if (r < n) {
             dequant8<KIND>(blocks + (r * sb + cb) * kBytes, lane, [&](int slot, int, float x) {
                 v[p][slot] = x;
-                amax = fmaxf(amax, fabsf(x));
-                finite &= isfinite(x);
+                m = max(m, mag_bits(x));
             });
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[p][i] = 0.0f;
         }
     }
-    if (!finite) atomicExch(err, kErrNonFinite);
-    amax = half_warp_max(amax);
+    m = half_warp_max(m);
+    if (!mag_finite(m)) atomicExch(err, kErrNonFinite);
     static_assert(kKqThreads / 32 == 32, "two maxima per lane below");
-    if ((lane & 15) == 0) red[lane >> 4][warp] = amax;
+    if ((lane & 15) == 0) red[lane >> 4][warp] = m;
     __syncthreads();
     // two reads of 16 maxima by each half-warp, then a shuffle
-    const float s = f8_scale(half_warp_max(fmaxf(red[lane >> 4][lane & 15], red[lane >> 4][16 + (lane & 15)])));
+    const float s = f8_scale(__uint_as_float(half_warp_max(max(red[lane >> 4][lane & 15], red[lane >> 4][16 + (lane & 15)]))));
     if (warp == 0 && (lane & 15) == 0)
         scales[static_cast<long long>(rb) * 2 * sb + 2 * cb + (lane >> 4)] = s;
 #pragma unroll
@@ -222,18 +255,19 @@ __global__ void __launch_bounds__(kKqThreads) prep_f8_kq_kernel(const uint8_t* _
         const long long r = static_cast<long long>(rb) * kF8Block + warp * 4 + p;
         if (r >= n) continue;
         uint8_t* dst = out + r * ld8 + cb * 256;
-        float q[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = __fdiv_rn(v[p][i], s);
+        uint32_t code[2];
+        f8_codes(v[p], s, code);
         if constexpr (KIND == kQ6K) {
+            // slots t and 4 + t are neighbours
             const int base = 128 * (lane >> 4) + (lane & 15) * 2;
 #pragma unroll
             for (int t = 0; t < 4; ++t)
-                *reinterpret_cast<uint16_t*>(dst + base + 32 * t) = static_cast<uint16_t>(f8_pack2(q[t], q[4 + t]));
+                *reinterpret_cast<uint16_t*>(dst + base + 32 * t) =
+                    static_cast<uint16_t>(__byte_perm(code[0], code[1], t | ((4 + t) << 4)));
         } else {
             const int base = 64 * (lane >> 3) + (lane & 7) * 4;
-            *reinterpret_cast<uint32_t*>(dst + base) = f8_pack4(q[0], q[1], q[2], q[3]);
-            *reinterpret_cast<uint32_t*>(dst + base + 32) = f8_pack4(q[4], q[5], q[6], q[7]);
+            *reinterpret_cast<uint32_t*>(dst + base) = code[0];
+            *reinterpret_cast<uint32_t*>(dst + base + 32) = code[1];
         }
     }
 }
