@@ -20,40 +20,21 @@
 //
 // Launch: programmatic dependent launch behind the quantiser.  Every wait is
 // bounded as in the int8 GEMM.
-#include <cuda.h>
-
 #include <algorithm>
 
-#include "f8.cuh"
-#include "kernels.h"
-#include "ptx.cuh"
+#include "gemm_f8.cuh"
 
 namespace rk {
 namespace {
+
+using f8_detail::F8Params;
+using f8_detail::fail;
 
 constexpr int kEpiWarps = 8;
 constexpr int kEpiThreads = kEpiWarps * 32;
 constexpr int kThreads = (3 + kEpiWarps) * 32;
 constexpr int kWRows = 128;
 constexpr int kWBox = kWRows * kF8Block;
-
-struct F8Params {
-    CUtensorMap tmap_w, tmap_a;
-    const float* w_scale;
-    const float* a_scale;
-    long long ld_as;
-    void* out;
-    long long ldo;
-    int out_type;
-    int m, n, num_kb;
-    int tiles_n, tiles_m, group_m;
-    int stream;   // blocks of all tiles in one line, cut evenly
-    int total;    // stream: blocks; else tiles
-    int early_weights;
-    float* part;  // [CTA][2][BT / 2][kEpiThreads] partial tiles
-    unsigned* counters;
-    int* err;
-};
 
 template <int BT>
 struct F8Cfg {
@@ -116,11 +97,6 @@ struct Walk {
         return true;
     }
 };
-
-__device__ __forceinline__ void fail(int* err, volatile uint32_t* abort, int code) {
-    atomicCAS(err, 0, code);
-    *abort = 1u;
-}
 
 // The epilogue warps' barrier; whether any of their threads passed true.
 __device__ __forceinline__ bool epi_any(bool v) {
@@ -400,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_f8_kernel(const __grid_const
 
 struct F8Plan {
     int bt = 16, grid = 1, tiles = 1;
-    bool stream = false;
+    bool stream = false, pair = false;
     size_t scratch = 0;
 };
 
@@ -431,6 +407,19 @@ F8Plan plan_f8(int m, int n, int k) {
             pl.tiles = static_cast<int>(std::min<long long>(tiles, 0x7fffffff));
             pl.grid = static_cast<int>(std::min<long long>(stream ? total : tiles, sms));
             pl.scratch = stream ? static_cast<size_t>(pl.grid) * 2 * kWRows * bt * sizeof(float) : 0;
+        }
+    }
+    // two-SM tiles: 512 cycles of MMAs per block and 256 x 256 outputs
+    const long long pairs = static_cast<long long>((n + 255) / 256) * ((m + 255) / 256);
+    const int slots = m > 128 ? f8_detail::pair_slots() : 0;
+    if (slots > 0) {
+        const double cost = static_cast<double>((pairs + slots - 1) / slots) * (kb * 600.0 + 4000.0);
+        if (cost < best) {
+            pl = F8Plan{};
+            pl.pair = true;
+            pl.bt = 256;
+            pl.tiles = static_cast<int>(std::min<long long>(pairs, 0x7fffffff));
+            pl.grid = static_cast<int>(std::min<long long>(pairs, slots));
         }
     }
     return pl;
@@ -481,7 +470,8 @@ int launch_gemm_f8(const GemmF8& g, int* err, cudaStream_t s) {
     p.m = g.m;
     p.n = g.n;
     p.num_kb = (g.k + kF8Block - 1) / kF8Block;
-    p.tiles_n = (g.n + kWRows - 1) / kWRows;
+    const int wt = pl.pair ? 256 : kWRows;
+    p.tiles_n = (g.n + wt - 1) / wt;
     p.tiles_m = (g.m + pl.bt - 1) / pl.bt;
     if (static_cast<long long>(p.tiles_n) * p.tiles_m > 0x7fffffffll) return cudaErrorInvalidValue;
     p.group_m = std::min(p.tiles_m, 8);
@@ -491,6 +481,13 @@ int launch_gemm_f8(const GemmF8& g, int* err, cudaStream_t s) {
     p.part = static_cast<float*>(g.scratch);
     p.counters = g.counters;
     p.err = err;
+    if (pl.pair) {
+        // each CTA of a pair loads 128 rows of either operand
+        if (!make_kmajor_map(&p.tmap_w, g.w, 1, g.k, g.n, g.ldw, 128) ||
+            !make_kmajor_map(&p.tmap_a, g.a, 1, g.k, g.m, g.lda, 128))
+            return cudaErrorInvalidValue;
+        return f8_detail::launch_pair(p, pl.grid, s);
+    }
     if (!make_kmajor_map(&p.tmap_w, g.w, 1, g.k, g.n, g.ldw, kWRows)) return cudaErrorInvalidValue;
     if (!make_kmajor_map(&p.tmap_a, g.a, 1, g.k, g.m, g.lda, pl.bt)) return cudaErrorInvalidValue;
     switch (pl.bt) {
