@@ -11,13 +11,25 @@
 // Tokens are the TMEM lanes, so the scale of a block is one number per thread
 // (its token's times its 128 columns', one weight scale block): an epilogue
 // thread adds 128 columns with 64 two-wide multiply-adds and reads no shared
-// memory, which the MMA's operands fill to half.  The totals are 128 registers
+// memory, which the MMA's operands fill to half.  Two-wide, because plain f32
+// multiply-adds slow the tensor core (measured: an MMA of 128 cycles takes 223
+// beside a stream of them, 128 beside two-wide ones).  The totals are 128 registers
 // per thread, so the epilogue warps take registers from the others
 // (setmaxnreg: 384 threads x 168 = 128 x 40 + 256 x 232).  At a tile's end each warp
 // turns its 32 tokens through shared memory, 128 bytes of columns at a time,
 // and stores whole lines.
 //
-// Barriers and bounded waits as in the int8 pair kernel (gemm_pair.cu).
+// MMA issue.  Whatever a warp reads from shared memory, a barrier included, it
+// gets only after the tensor core has accepted the MMAs it issued before
+// (about 200 cycles per look, measured with 4 MMAs between looks: 720 cycles
+// per block instead of 512), so one warp that waits and issues in turn starves
+// the tensor core.  Two warps take turns: one waits for its block's operands
+// and TMEM buffer while the other's MMAs run, then for its turn.  One barrier
+// per stage, done[s], says both that a block's operands may be overwritten and
+// that its sums are in TMEM; the epilogue is never more than the two TMEM
+// buffers behind, less than the stages, so it cannot miss a phase.
+//
+// Bounded waits as in the int8 pair kernel (gemm_pair.cu).
 #include <algorithm>
 
 #include "gemm_f8.cuh"
@@ -40,32 +52,6 @@ constexpr int kStageOffset = (kBarOffset + kNumBars * 8 + 32 + 127) / 128 * 128;
 constexpr int kBytes = kStageOffset + kEpiWarps * kStaging + 1024;  // + alignment slack
 static_assert(kBytes <= 232448, "shared memory");
 
-__device__ __forceinline__ bool wait_cluster_or_abort(uint64_t* bar, uint32_t parity, volatile uint32_t* abort) {
-    if (mbar_try_wait_cluster(bar, parity)) return true;
-    const uint64_t t0 = globaltimer_ns();
-    while (true) {
-#pragma unroll 1
-        for (int i = 0; i < 32; ++i)
-            if (mbar_try_wait_cluster(bar, parity)) return true;
-        if (*abort) return false;
-        if (globaltimer_ns() - t0 > kWaitLimitNs) return false;
-    }
-}
-
-// (a, b) * (s, s) + (c, d)
-__device__ __forceinline__ void fma2(float& c, float& d, uint32_t a, uint32_t b, float s) {
-    asm("{\n"
-        " .reg .b64 x, y, z;\n"
-        " mov.b64 x, {%2, %3};\n"
-        " mov.b64 y, {%4, %4};\n"
-        " mov.b64 z, {%0, %1};\n"
-        " fma.rn.f32x2 z, x, y, z;\n"
-        " mov.b64 {%0, %1}, z;\n"
-        "}\n"
-        : "+f"(c), "+f"(d)
-        : "r"(a), "r"(b), "f"(s));
-}
-
 struct Tile {
     int n0, m0;
     __device__ __forceinline__ Tile(const F8Params& p, int u) {
@@ -80,8 +66,11 @@ struct Tile {
 
 // A warp's 32 tokens x 128 columns (one token per lane) to memory.
 template <class T>
-__device__ __forceinline__ void store_rows(const F8Params& p, const float (&acc)[128], int m0, int n0, uint8_t* staging,
+__device__ __forceinline__ void store_rows(const F8Params& p, const float2 (&acc2)[64], int m0, int n0, uint8_t* staging,
                                            int lane) {
+    float acc[128];
+#pragma unroll
+    for (int c = 0; c < 64; ++c) acc[2 * c] = acc2[c].x, acc[2 * c + 1] = acc2[c].y;
     constexpr int kPer = 128 / sizeof(T);  // columns per 128-byte piece
     T* out = static_cast<T*>(p.out);
     const bool whole = reinterpret_cast<uintptr_t>(out) % 16 == 0 && p.ldo * sizeof(T) % 16 == 0;
@@ -131,10 +120,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // same offset in both CTAs: the MMA addresses the peer's half by it
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + kBarOffset);
-    uint64_t* empty = full + S;
-    uint64_t* tfull = empty + S;
-    uint64_t* tempty = tfull + 2;
-    uint64_t* drain = tempty + 2;
+    uint64_t* done = full + S;
+    uint64_t* tempty = done + S;
+    uint64_t* turn = tempty + 2;
+    uint64_t* drain = turn + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile uint32_t* abort = tmem_slot + 1;
 
@@ -144,13 +133,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
             mbar_init(&full[s], 2);  // the leader's two producers
-            mbar_init(&empty[s], 1);
+            mbar_init(&done[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
-            mbar_init(&tfull[b], 1);
+            mbar_init(&turn[b], 1);
             mbar_init(&tempty[b], 2 * kEpiWarps);  // epilogue warps of both CTAs
         }
-        mbar_init(drain, 1);
+        mbar_init(drain, 2);  // the two issuers
         *abort = 0u;
         fence_mbar_init();
         prefetch_tmap(&p.tmap_w);
@@ -181,7 +170,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int row = (is_w ? t.n0 : t.m0) + 128 * static_cast<int>(rank);
                 for (int kb = 0; kb < p.num_kb; ++kb, ++g) {
                     const int s = g % S;
-                    if (g >= S && !wait_or_abort(&empty[s], ((g / S) & 1) ^ 1, abort)) {
+                    if (g >= S && !wait_or_abort(&done[s], ((g / S) & 1) ^ 1, abort)) {
                         if (!*abort) fail(p.err, abort, kErrTimeoutEmpty);
                         ok = false;
                         break;
@@ -194,38 +183,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
             // every stage filled here must be consumed (so its copy has landed) before the CTA leaves
             for (int i = max(0, g - S); i < g; ++i) {
-                if (!mbar_wait(&empty[i % S], (i / S) & 1)) {
+                if (!mbar_wait(&done[i % S], (i / S) & 1)) {
                     atomicCAS(p.err, 0, kErrTimeoutDrain);
                     break;
                 }
             }
-        } else if (warp == 2 && lane == 0 && leader) {
-            // ---- MMA issuer (even CTA): one TMEM buffer per block ----
+        } else if (warp >= 2 && lane == 0 && leader) {
+            // ---- MMA issuers (even CTA), taking turns: warp 2 the even blocks
+            // with TMEM buffer 0, warp 3 the odd ones with buffer 1 ----
             constexpr uint32_t idesc = make_idesc<2>(kTile, kTile);
-            int g = 0;
-            bool ok = true;
-            for (int u = pair; ok && u < p.total; u += npairs) {
-                for (int kb = 0; kb < p.num_kb; ++kb, ++g) {
-                    const int s = g % S, b = g & 1;
-                    if (g >= 2 && !wait_cluster_or_abort(&tempty[b], ((g >> 1) & 1) ^ 1, abort)) {
-                        if (!*abort) fail(p.err, abort, kErrTimeoutAccum);
-                        ok = false;
-                        break;
-                    }
-                    if (!wait_or_abort(&full[s], (g / S) & 1, abort)) {
-                        if (!*abort) fail(p.err, abort, kErrTimeoutFull);
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t ta = smem_u32(smem + s * kStage);
-#pragma unroll
-                    for (int ks = 0; ks < kF8Block / 32; ++ks)
-                        tc_mma_pair<2>(tmem_base + b * kTile, smem_desc_k128(ta + ks * 32),
-                                       smem_desc_k128(ta + kBox + ks * 32), idesc, ks != 0 ? 1u : 0u);
-                    tc_commit_pair(&empty[s], 0x3);
-                    tc_commit_pair(&tfull[b], 0x3);
+            const int b = warp - 2;
+            const int blocks = (p.total - pair + npairs - 1) / npairs * p.num_kb;
+            for (int g = b; g < blocks; g += 2) {
+                const int s = g % S;
+                if (!wait_or_abort(&full[s], (g / S) & 1, abort)) {
+                    if (!*abort) fail(p.err, abort, kErrTimeoutFull);
+                    break;
                 }
+                // the other warp has issued block g - 1
+                if (g > 0 && !wait_or_abort(&turn[b], ((g - 1) >> 1) & 1, abort)) {
+                    if (!*abort) fail(p.err, abort, kErrTimeoutFull);
+                    break;
+                }
+                // the last of the three to come: this buffer has been read out
+                if (g >= 2 && !wait_or_abort(&tempty[b], ((g >> 1) & 1) ^ 1, abort)) {
+                    if (!*abort) fail(p.err, abort, kErrTimeoutAccum);
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t ta = smem_u32(smem + s * kStage);
+#pragma unroll
+                for (int ks = 0; ks < kF8Block / 32; ++ks)
+                    tc_mma_pair<2>(tmem_base + b * kTile, smem_desc_k128(ta + ks * 32),
+                                   smem_desc_k128(ta + kBox + ks * 32), idesc, ks != 0 ? 1u : 0u);
+                mbar_arrive(&turn[b ^ 1]);
+                tc_commit_pair(&done[s], 0x3);
             }
             // the pair's MMAs must finish before either CTA releases TMEM
             tc_commit_pair(drain, 0x3);
@@ -250,13 +242,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             // columns past n read a scale that exists; their sums are not stored
             const float* ws = p.w_scale + static_cast<long long>(min(n0, p.n - 1) / kF8Block) * p.num_kb;
             const float* as = p.a_scale + static_cast<long long>(min(m0 + lane, p.m - 1)) * p.ld_as;
-            float acc[128];
+            float2 acc[64];
 #pragma unroll
-            for (int c = 0; c < 128; ++c) acc[c] = 0.0f;
+            for (int c = 0; c < 64; ++c) acc[c] = make_float2(0.0f, 0.0f);
             // A block's 128 columns in four pieces; the next piece is on its way
             // while one is added, the next block's first piece included.
             auto ready = [&](int i) {
-                if (!wait_or_abort(&tfull[i & 1], (i >> 1) & 1, abort)) {
+                if (!wait_or_abort(&done[i % S], (i / S) & 1, abort)) {
                     if (lane == 0 && !*abort) fail(p.err, abort, kErrTimeoutAccum);
                     ok = false;
                 }
@@ -265,8 +257,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             };
             const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * 128);
             auto add = [&](int c, const uint32_t(&r)[32], float s) {
+const float2 ss = make_float2(s, s);
 #pragma unroll
-                for (int j = 0; j < 32; j += 2) fma2(acc[c * 32 + j], acc[c * 32 + j + 1], r[j], r[j + 1], s);
+                for (int j = 0; j < 16; ++j) acc[c * 16 + j] = __ffma2_rn(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), ss, acc[c * 16 + j]);
             };
             // scales two blocks ahead
             const int last = p.num_kb - 1;
@@ -274,7 +267,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             uint32_t r0[32], r1[32];
             ready(g);
             tmem_ld32(lane_base + (g & 1) * kTile, r0);
-#pragma unroll 1
+// unrolled, so that the carried piece stays in place (1089 -> 1015 us at
+            // 4096 x 28672 x 8192)
+#pragma unroll 4
             for (int kb = 0; kb < p.num_kb; ++kb, ++g) {
                 const float a2 = __ldg(as + min(kb + 2, last)), w2 = __ldg(ws + min(kb + 2, last));
                 const uint32_t base = lane_base + (g & 1) * kTile;
@@ -291,7 +286,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 // read out: this CTA's half of the buffer is free
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_remote_relaxed(tempty_leader + (g & 1) * 8);
+                if (lane == 0) {
+                    if (leader)
+                        mbar_arrive(&tempty[g & 1]);
+                    else
+                        mbar_arrive_remote_relaxed(tempty_leader + (g & 1) * 8);
+                }
                 if (kb < last) {
                     ready(g + 1);
                     tmem_ld32(lane_base + ((g + 1) & 1) * kTile, r0);
