@@ -400,8 +400,9 @@ typedef struct rocknpu_b200_f8_experts {
  * of zeros; an id may occur twice; an id >= experts sets *status to 9
  * (INVALID_ARGUMENT by rocknpu_b200_status_code) and counts as empty.
  * Activations are not quantised: f32 ones (and the hidden values) enter the
- * products with 22 bits relative to the largest of their block of 128, f16
- * and bf16 ones exactly, with hidden values of 11 bits; sums are f32.
+ * products with 22 bits relative to the largest of their block of 128 (hidden
+ * values: of 16), f16 and bf16 ones exactly, with hidden values of 11 bits;
+ * sums are f32.
  * hidden and ffn are multiples of 16, top_k <= 16, experts <= 256. */
 typedef struct rocknpu_b200_moe_f8_args {
     size_t tokens, hidden, ffn, experts, top_k;
@@ -420,10 +421,10 @@ typedef struct rocknpu_b200_moe_f8_args {
 } rocknpu_b200_moe_f8_args;
 
 /* Bytes of workspace (0 for a shape outside the limits above), and the layer.
- * One cooperative launch: it needs every SM of the GPU for one CTA, waits for
- * other kernels that hold them, and can be captured into a graph.  The
- * workspace follows rocknpu_b200_gemm_f8's rules and can be shared with those
- * calls, in turn.  Results do not depend on the order in which CTAs finish. */
+ * One launch, without a need for co-resident CTAs; it can be captured into a
+ * graph.  The workspace follows rocknpu_b200_gemm_f8's rules and can be shared
+ * with those calls, in turn.  Results do not depend on the order in which CTAs
+ * finish. */
 size_t rocknpu_b200_moe_f8_workspace_bytes(size_t tokens, size_t hidden, size_t ffn, size_t experts, size_t top_k,
                                            uint32_t type);
 int rocknpu_b200_moe_f8(const rocknpu_b200_moe_f8_args *args, void *workspace, size_t workspace_bytes, int *status,

@@ -9,7 +9,7 @@
 //
 // Products.  Weights go from TMA stages (128-byte swizzle) to registers,
 // e4m3 -> f16 (exact), into mma.sync m16n8k16 with tokens as the 8 columns.
-// Activations are not quantised: a block of 128 is scaled by a power of two
+// Activations are not quantised: a block of them is scaled by a power of two
 // so that its largest magnitude is in [2^14, 2^15) and held in f16; for f32
 // calls a second f16 holds the remainder (22 bits in all), for f16 / bf16
 // calls the inputs fit one f16 and the hidden values are rounded to 11 bits,
@@ -22,19 +22,30 @@
 // the swizzle spreads over all banks) and the activations are laid out in
 // memory in the order in which the threads then need them.
 //
-// Work.  A tile is 256 weight rows (128 gate + 128 up rows, or 256 down
-// rows); the blocks of all tiles of all chosen experts form one line that is
-// cut evenly over the CTAs, one per SM, so no SM idles for a whole tile.  A
-// tile cut by a border is finished by the CTA that arrives last on it, from
-// the contributors' f32 partial tiles in line order (the result does not
-// depend on who that is); the last of a column tile's experts sums the slots
-// in slot order.
+// Work.  A group is 16 gate and 16 up rows (32 down rows) of one chosen
+// expert over the whole of k; the groups of all chosen experts form one line
+// that is cut evenly into as many parts as there are SMs, at most one group
+// apart.  Groups and not larger tiles, because then nothing of gate / up is
+// summed across CTAs (cutting 128-row tiles along k evenly instead left each
+// CTA one or two partial tiles to exchange: 6 us between the two products of
+// a 10 us layer).  A part runs in passes of up to 8 groups, one per warp;
+// with fewer, warps share a group's blocks and add through shared memory.
+// Hidden values are scaled per group of 16; the down product brings the
+// eight groups of a block to the block's largest scale as it reads them
+// (exact but for bits 2^-39 below the block's largest value).
 //
-// Phases: (0) router products and the activations' layout; grid barrier; (1)
-// every CTA picks the experts for itself, gate / up products, SiLU; grid
-// barrier; (2) down products, weighted sum.  The weight copies of phase 2
-// start before its barrier.  The launch is cooperative, so all CTAs are
-// resident; every wait is bounded all the same.
+// The down product may also cut k (a part's groups then divide more evenly);
+// the parts of a sum and the slots of a token are added in a fixed order by
+// the CTA that finishes a group of columns last, so results do not depend on
+// who that is.
+//
+// Phases: (0) router products and the activations' layout; (1) every CTA
+// picks the experts for itself, gate / up products, SiLU; (2) down products,
+// weighted sum.  A CTA takes a part by ticket and does that part of every
+// phase.  One that waits long for the others in phase 0 takes further parts,
+// until all are held by CTAs that run, so the launch needs no co-residency (a
+// cooperative launch cost 16 us more per call).  The weight copies of phase 2
+// start before its wait.  Every wait is bounded.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -48,19 +59,24 @@
 namespace rk {
 namespace {
 
-constexpr int kConsumers = 8;                      // warps
+constexpr int kConsumers = 8;                // warps
 constexpr int kConsThreads = kConsumers * 32;
-constexpr int kThreads = kConsThreads + 32;        // + the producer warp
-constexpr int kBoxRows = 128;
+constexpr int kProducers = 4;                // warps
+constexpr int kThreads = kConsThreads + kProducers * 32;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBoxRows = 16;                 // rows of one TMA box, one MMA tile
 constexpr int kBoxBytes = kBoxRows * kF8Block;
+constexpr int kGroupBytes = 2 * kBoxBytes;   // gate and up, or two boxes of down rows
 constexpr int kMaxPairs = kMoeMaxTokens * kMoeMaxTop;
-constexpr int kRouterTokens = 4;                   // tokens per router task
+constexpr int kRouterTokens = 4;             // tokens per router task
+constexpr int kMaxParts = 512;               // CTAs of a launch
+constexpr uint64_t kHelpNs = 20000;          // wait for the others before taking a further part
 
 // Words of the zeroed header.
-constexpr int kCut1 = 0, kCut2 = 1024, kBarrier = 2048, kExit = 2049, kCombine = 4096;
+constexpr int kTicket = 0, kBarrier = 32, kExit = 64, kCombine = 1024;
 
 struct MoeParams {
-    CUtensorMap tm_gate, tm_up, tm_down;  // (k, rows, expert), box 128 B x 128 rows
+    CUtensorMap tm_gate, tm_up, tm_down;  // (k, rows, expert), box 128 B x 16 rows
     const float *gate_s, *up_s, *down_s;
     long long gate_ss, up_ss, down_ss;  // scales of one expert
     const void* x;
@@ -71,37 +87,40 @@ struct MoeParams {
     int* ids;
     float* weights;
     int t, h, f, e, top, renorm;
-    int kb_h, kb_f, tiles_f, tiles_h;
+    int kb_h, kb_f, max_split;
+    int wide;  // x and router rows can be read 16 bytes at a time
     unsigned* ctrl;
     float* logits;    // [t][e]
     uint8_t* xq;      // [t][kb_h] activation blocks
     uint8_t* hq;      // [pair][kb_f] activation blocks
-    float* part;      // [CTA][2][8 NG][kConsThreads] partial tiles
-    float* pair_out;  // [pair][h]
+    float* pair_out;  // [pair][max_split][h]
     int* err;
 };
 
 // An activation block of 128 values: f16 values (and remainders) in the
-// order of the MMA operands, then the f32 power of two.
+// order of the MMA operands, then eight f32 powers of two, one per 16 values
+// (x: all the first one's).
 template <bool LO>
 struct ActBlock {
     static constexpr int kScaleAt = LO ? 512 : 256;
-    static constexpr int kBytes = kScaleAt + 16;
+    static constexpr int kBytes = kScaleAt + 32;
     // distance of two rows in shared memory: an odd multiple of 64 bytes, so
     // that two rows' 64-byte reads fall into different banks
     static constexpr int kPitch = LO ? 576 : 320;
 };
 
+// Sums that warps exchange: 8 per thread.
+constexpr int kRedBytes = kConsThreads * 8 * 4;
+
 template <int NG, bool LO>
 struct MoeCfg {
     using Act = ActBlock<LO>;
     static constexpr int kAct = (NG * 8 * Act::kPitch + 1023) / 1024 * 1024;
-    static constexpr int kStage = 2 * kBoxBytes + kAct;
-    static constexpr int kStages = (212 * 1024) / kStage;
+    static constexpr int kStage = kConsumers * kGroupBytes + kAct;
+    static constexpr int kStages = (200 * 1024) / kStage;
     static constexpr int kBarOffset = kStages * kStage;
     static constexpr int kTables = kBarOffset + (2 * kStages * 8 + 32 + 15) / 16 * 16;
-    static constexpr int kTableBytes = kMaxPairs * (4 + 2 + 2 + 4) + kMoeMaxExperts * 4 + 16 +
-                                       kConsumers * kMoeMaxTokens * 4;
+    static constexpr int kTableBytes = kMaxPairs * (4 + 4 + 2 + 2) + kMoeMaxExperts * 4 + 16 + kRedBytes + kMaxParts * 2;
     static constexpr int kBytes = kTables + kTableBytes + 1024;  // + alignment slack
     static_assert(kBytes <= 232448, "shared memory");
 };
@@ -114,7 +133,7 @@ struct Tables {
     int* entry;          // [entries] expert << 16 | first position in order
     int* count;          // [expert] pairs
     int* info;           // [0] entries, [1] positions
-    float* red;          // [kConsumers][kMoeMaxTokens]
+    float* red;          // kRedBytes
 };
 
 __device__ __forceinline__ void fail(int* err, volatile uint32_t* abort, int code) {
@@ -144,6 +163,14 @@ __device__ __forceinline__ bool grid_wait(const unsigned* bar, unsigned need, vo
     return true;
 }
 
+// As grid_wait, but for at most ns.
+__device__ __forceinline__ bool grid_wait_some(const unsigned* bar, unsigned need, uint64_t ns) {
+    const uint64_t t0 = globaltimer_ns();
+    while (ld_acquire(bar) < need)
+        if (globaltimer_ns() - t0 > ns) return false;
+    return true;
+}
+
 __device__ __forceinline__ void cons_bar() { asm volatile("bar.sync 2, %0;" ::"n"(kConsThreads) : "memory"); }
 
 // The same barrier; whether any consumer thread passed true.
@@ -168,6 +195,23 @@ __device__ __forceinline__ float load_dense(const void* p, int type, long long i
     return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
 
+// Eight consecutive values at a 16-byte boundary.
+__device__ __forceinline__ void load_dense8(const void* p, int type, long long i, float (&v)[8]) {
+    if (type == kTypeF32) {
+        Raw8<float> r;
+        r.load(static_cast<const float*>(p) + i);
+        r.values(v);
+    } else if (type == kTypeF16) {
+        Raw8<__half> r;
+        r.load(static_cast<const __half*>(p) + i);
+        r.values(v);
+    } else {
+        Raw8<__nv_bfloat16> r;
+        r.load(static_cast<const __nv_bfloat16*>(p) + i);
+        r.values(v);
+    }
+}
+
 __device__ __forceinline__ void store_dense(void* p, int type, long long i, float v) {
     if (type == kTypeF32)
         static_cast<float*>(p)[i] = v;
@@ -177,11 +221,12 @@ __device__ __forceinline__ void store_dense(void* p, int type, long long i, floa
         static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
-// Power of two s with amax / s in [2^14, 2^15) (1 for a block of zeros, at
-// least 2^-126), and its exact reciprocal.
+// Power of two s with amax / s in [2^14, 2^15), at least 2^-126 (zeros too:
+// next to other groups of a block theirs must not be the largest scale), and
+// its exact reciprocal.
 __device__ __forceinline__ float act_scale(float amax, float& inv) {
     const uint32_t ex = (__float_as_uint(amax) >> 23) & 0xFFu;
-    const uint32_t se = amax == 0.0f ? 127u : (ex > 15u ? ex - 14u : 1u);
+    const uint32_t se = ex > 15u ? ex - 14u : 1u;
     inv = __uint_as_float((254u - se) << 23);
     return __uint_as_float(se << 23);
 }
@@ -190,57 +235,84 @@ __device__ __forceinline__ float act_scale(float amax, float& inv) {
 // 16-byte chunk j = (k % 32) / 8 at (4 j + t) * 16.
 __device__ __forceinline__ int act_at(int k) { return (((k >> 3) & 3) * 4 + (k >> 5)) * 16 + (k & 7) * 2; }
 
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-    const __half2 v = __floats2half2_rn(a, b);
-    uint32_t r;
-    memcpy(&r, &v, 4);
-    return r;
+// Two values as f16 and, with LO, what that leaves as f16.
+template <bool LO>
+__device__ __forceinline__ void split_half2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    memcpy(&hi, &h, 4);
+    if constexpr (LO) {
+        const float2 f = __half22float2(h);
+        const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+        memcpy(&lo, &l, 4);
+    }
 }
 
 // ---- phase 0: activation blocks of x, router products ----------------------
 
+// A half-warp per block, 8 values per lane.
 template <bool LO>
-__device__ __forceinline__ void layout_x(const MoeParams& p, int warp, int warps, int lane) {
-    bool finite = true;
-    for (int task = warp; task < p.t * p.kb_h; task += warps) {
-        const int tok = task / p.kb_h, kb = task - tok * p.kb_h;
-        float v[4], amax = 0.0f;
+__device__ __forceinline__ void layout_x(const MoeParams& p, int half, int halves, int lane) {
+    uint32_t most = 0;
+    const int l = lane & 15;
+    // the two halves of a warp take the same steps
+    for (int task = half; task - (lane >> 4) < p.t * p.kb_h; task += halves) {
+        const bool live = task < p.t * p.kb_h;
+        const int tok = task / p.kb_h, k = (task - tok * p.kb_h) * kF8Block + l * 8;
+        float v[8];
+        if (live && p.wide && k < p.h) {  // h is a multiple of 16
+            load_dense8(p.x, p.type, tok * p.ldx + k, v);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int k = kb * kF8Block + lane * 4 + i;
-            v[i] = k < p.h ? load_dense(p.x, p.type, tok * p.ldx + k) : 0.0f;
-            finite &= isfinite(v[i]);
-            amax = fmaxf(amax, fabsf(v[i]));
+            for (int i = 0; i < 8; ++i) v[i] = live && k + i < p.h ? load_dense(p.x, p.type, tok * p.ldx + k + i) : 0.0f;
         }
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, mag_bits(v[i]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        most = max(most, m);
         float inv;
-        const float s = act_scale(warp_max(amax), inv);
-        uint8_t* blk = p.xq + static_cast<long long>(task) * ActBlock<LO>::kBytes;
-        float hi[4], lo[4];
+        const float s = act_scale(__uint_as_float(m), inv);
+        if (live) {
+            uint8_t* blk = p.xq + static_cast<long long>(task) * ActBlock<LO>::kBytes;
+            uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            hi[i] = __half2float(__float2half_rn(v[i] * inv));
-            lo[i] = v[i] * inv - hi[i];
+            for (int i = 0; i < 4; ++i) split_half2<LO>(v[2 * i] * inv, v[2 * i + 1] * inv, hi[i], lo[i]);
+            *reinterpret_cast<uint4*>(blk + act_at(l * 8)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if constexpr (LO) *reinterpret_cast<uint4*>(blk + 256 + act_at(l * 8)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            if (l == 0) *reinterpret_cast<float*>(blk + ActBlock<LO>::kScaleAt) = s;
         }
-        *reinterpret_cast<uint2*>(blk + act_at(lane * 4)) = make_uint2(pack_half2(hi[0], hi[1]), pack_half2(hi[2], hi[3]));
-        if constexpr (LO)
-            *reinterpret_cast<uint2*>(blk + 256 + act_at(lane * 4)) =
-                make_uint2(pack_half2(lo[0], lo[1]), pack_half2(lo[2], lo[3]));
-        if (lane == 0) *reinterpret_cast<float*>(blk + ActBlock<LO>::kScaleAt) = s;
     }
-    if (!finite) atomicExch(p.err, kErrNonFinite);
+    if (!mag_finite(most)) atomicExch(p.err, kErrNonFinite);
 }
 
-// Partial sums over k0..k1 of one expert's row with kRouterTokens tokens.
+// Sums over k0..k1 of one expert's row with kRouterTokens tokens.
 __device__ __forceinline__ void router_dot(const MoeParams& p, int ex, int tok0, int k0, int k1, int lane,
                                            float (&s)[kRouterTokens]) {
 #pragma unroll
     for (int i = 0; i < kRouterTokens; ++i) s[i] = 0.0f;
-#pragma unroll 4
-    for (int k = k0 + lane; k < k1; k += 32) {
-        const float r = load_dense(p.router, p.router_type, ex * p.ld_router + k);
+    if (p.wide) {  // k0 and k1 are multiples of 8
+#pragma unroll 2
+        for (int k = k0 + lane * 8; k < k1; k += 256) {
+            float r[8];
+            load_dense8(p.router, p.router_type, ex * p.ld_router + k, r);
 #pragma unroll
-        for (int i = 0; i < kRouterTokens; ++i)
-            if (tok0 + i < p.t) s[i] = fmaf(r, load_dense(p.x, p.type, (tok0 + i) * p.ldx + k), s[i]);
+            for (int i = 0; i < kRouterTokens; ++i) {
+                if (tok0 + i >= p.t) break;
+                float x[8];
+                load_dense8(p.x, p.type, (tok0 + i) * p.ldx + k, x);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[i] = fmaf(r[j], x[j], s[i]);
+            }
+        }
+    } else {
+#pragma unroll 4
+        for (int k = k0 + lane; k < k1; k += 32) {
+            const float r = load_dense(p.router, p.router_type, ex * p.ld_router + k);
+#pragma unroll
+            for (int i = 0; i < kRouterTokens; ++i)
+                if (tok0 + i < p.t) s[i] = fmaf(r, load_dense(p.x, p.type, (tok0 + i) * p.ldx + k), s[i]);
+        }
     }
 #pragma unroll
     for (int i = 0; i < kRouterTokens; ++i)
@@ -248,13 +320,14 @@ __device__ __forceinline__ void router_dot(const MoeParams& p, int ex, int tok0,
         for (int o = 16; o > 0; o >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
 }
 
-// Few tasks: a CTA's consumer warps share a task's k range; many: a warp each.
-__device__ __forceinline__ void router_products(const MoeParams& p, const Tables& tb, int warp, int lane) {
+// Part `part` of the router products.  Few tasks: a CTA's consumer warps share
+// a task's k range; many: a warp each.
+__device__ __forceinline__ void router_products(const MoeParams& p, const Tables& tb, int part, int warp, int lane) {
     const int groups = (p.t + kRouterTokens - 1) / kRouterTokens, tasks = p.e * groups;
     float s[kRouterTokens];
     if (tasks <= 2 * static_cast<int>(gridDim.x)) {
-        const int per = (p.h + kConsumers - 1) / kConsumers;
-        for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
+        const int per = (p.h / 8 + kConsumers - 1) / kConsumers * 8;
+        for (int task = part; task < tasks; task += gridDim.x) {
             const int ex = task / groups, tok0 = (task - ex * groups) * kRouterTokens;
             if (warp < kConsumers) {
                 router_dot(p, ex, tok0, warp * per, min(p.h, (warp + 1) * per), lane, s);
@@ -265,14 +338,14 @@ __device__ __forceinline__ void router_products(const MoeParams& p, const Tables
             __syncthreads();
             if (threadIdx.x < kRouterTokens && tok0 + static_cast<int>(threadIdx.x) < p.t) {
                 float sum = 0.0f;
+#pragma unroll
                 for (int w = 0; w < kConsumers; ++w) sum += tb.red[w * kRouterTokens + threadIdx.x];
                 __stcg(p.logits + (tok0 + threadIdx.x) * p.e + ex, sum);
             }
             __syncthreads();
         }
     } else {
-        const int warps = gridDim.x * (kThreads / 32);
-        for (int task = blockIdx.x * (kThreads / 32) + warp; task < tasks; task += warps) {
+        for (int task = part * kWarps + warp; task < tasks; task += gridDim.x * kWarps) {
             const int ex = task / groups, tok0 = (task - ex * groups) * kRouterTokens;
             router_dot(p, ex, tok0, 0, p.h, lane, s);
             if (lane == 0)
@@ -292,15 +365,16 @@ __device__ __forceinline__ uint32_t sort_key(float v) {
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// One token: its `top` largest logits, ties to the lower expert.
+// One token: its `top` largest logits, ties to the lower expert.  PER: experts
+// per lane.
+template <int PER>
 __device__ __forceinline__ void choose(const MoeParams& p, const Tables& tb, int tok, int lane) {
-    constexpr int kPer = kMoeMaxExperts / 32;
-    float v[kPer];
-    uint32_t key[kPer];
+    float v[PER];
+    uint32_t key[PER];
     float vmax = -INFINITY;
     bool finite = true;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
+    for (int j = 0; j < PER; ++j) {
         const int ex = lane + 32 * j;
         v[j] = ex < p.e ? __ldcg(p.logits + tok * p.e + ex) : -INFINITY;
         finite &= ex >= p.e || isfinite(v[j]);
@@ -309,9 +383,12 @@ __device__ __forceinline__ void choose(const MoeParams& p, const Tables& tb, int
     }
     if (!finite) atomicExch(p.err, kErrNonFinite);
     vmax = warp_max(vmax);
-    float sum = 0.0f;
+    float ev[PER], sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) sum += lane + 32 * j < p.e ? expf(v[j] - vmax) : 0.0f;
+    for (int j = 0; j < PER; ++j) {
+        ev[j] = lane + 32 * j < p.e ? expf(v[j] - vmax) : 0.0f;
+        sum += ev[j];
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     float chosen = 0.0f, mine = 0.0f;  // lane k keeps slot k
@@ -319,24 +396,24 @@ __device__ __forceinline__ void choose(const MoeParams& p, const Tables& tb, int
     for (int k = 0; k < p.top; ++k) {
         uint32_t best = 0;
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) best = max(best, key[j]);
+        for (int j = 0; j < PER; ++j) best = max(best, key[j]);
         best = __reduce_max_sync(0xffffffffu, best);
         uint32_t at = 0xffffffffu;
 #pragma unroll
-        for (int j = kPer - 1; j >= 0; --j)
+        for (int j = PER - 1; j >= 0; --j)
             if (key[j] == best) at = lane + 32 * j;
         at = __reduce_min_sync(0xffffffffu, at);
-        float ev = 0.0f;
+        float w = 0.0f;
 #pragma unroll
-        for (int j = 0; j < kPer; ++j)
+        for (int j = 0; j < PER; ++j)
             if (static_cast<uint32_t>(lane + 32 * j) == at) {
-                ev = expf(v[j] - vmax);
+                w = ev[j];
                 key[j] = 0u;
             }
-        ev = __shfl_sync(0xffffffffu, ev, at & 31);
-        chosen += ev;
+        w = __shfl_sync(0xffffffffu, w, at & 31);
+        chosen += w;
         if (lane == k) {
-            mine = ev;
+            mine = w;
             mine_e = static_cast<int>(at);
         }
     }
@@ -355,10 +432,18 @@ __device__ __forceinline__ void choose(const MoeParams& p, const Tables& tb, int
 // Pairs sorted by expert (then token); experts with pairs become entries of
 // at most `cap` pairs each.
 __device__ __forceinline__ void build_tables(const MoeParams& p, const Tables& tb, int cap) {
-    const int pairs = p.t * p.top;
+    // eight pairs per read; those behind the last are empty
+    const int eights = (p.t * p.top + 7) / 8;
+    const uint4* all = reinterpret_cast<const uint4*>(tb.pair_e);
     for (int ex = threadIdx.x; ex < p.e; ex += kThreads) {
         int n = 0;
-        for (int i = 0; i < pairs; ++i) n += tb.pair_e[i] == ex;
+#pragma unroll 4
+        for (int i = 0; i < eights; ++i) {
+            const uint4 v = all[i];
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) n += (static_cast<int>(w[j] & 0xFFFFu) == ex) + (static_cast<int>(w[j] >> 16) == ex);
+        }
         tb.count[ex] = n;
     }
     __syncthreads();
@@ -374,7 +459,7 @@ __device__ __forceinline__ void build_tables(const MoeParams& p, const Tables& t
                 if (lane >= o) sp += a, se += b;
             }
             for (int i = 0; i < ne; ++i) tb.entry[ents + se - ne + i] = (ex << 16) | (pos + sp - n + i * cap);
-            if (ex < p.e) tb.count[ex] = pos + sp - n;  // now the expert's first position
+            if (ex < p.e) tb.count[ex] = n ? pos + sp - n : -1;  // now the expert's first position
             pos += __shfl_sync(0xffffffffu, sp, 31);
             ents += __shfl_sync(0xffffffffu, se, 31);
         }
@@ -383,8 +468,16 @@ __device__ __forceinline__ void build_tables(const MoeParams& p, const Tables& t
     __syncthreads();
     for (int ex = threadIdx.x; ex < p.e; ex += kThreads) {
         int at = tb.count[ex];
-        for (int i = 0; i < pairs; ++i)
-            if (tb.pair_e[i] == ex) tb.order[at++] = static_cast<short>(i);
+        if (at < 0) continue;
+        for (int i = 0; i < eights; ++i) {
+            const uint4 v = all[i];
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (static_cast<int>(w[j] & 0xFFFFu) == ex) tb.order[at++] = static_cast<short>(8 * i + 2 * j);
+                if (static_cast<int>(w[j] >> 16) == ex) tb.order[at++] = static_cast<short>(8 * i + 2 * j + 1);
+            }
+        }
     }
     __syncthreads();
 }
@@ -398,43 +491,52 @@ __device__ __forceinline__ void entry_pairs(const Tables& tb, int i, int cap, in
     n = min(cap, end - first);
 }
 
-// ---- the line of blocks ----------------------------------------------------
+// ---- the line of groups ----------------------------------------------------
 
 struct Line {
-    int tiles, nkb, total;  // tiles per entry, blocks per tile, blocks in all
-    int parts;              // CTAs that share it: all, or one per block
-    __device__ __forceinline__ Line(int entries, int tiles_, int nkb_)
-        : tiles(tiles_), nkb(nkb_), total(entries * tiles_ * nkb_), parts(min(static_cast<int>(gridDim.x), total)) {}
-    // First block of CTA cta's part; the CTA whose part holds block x.
-    __device__ __forceinline__ int start(int cta) const {
-        return static_cast<int>(static_cast<long long>(cta) * total / parts);
-    }
-    __device__ __forceinline__ int owner(int x) const {
-        return static_cast<int>(((static_cast<long long>(x) + 1) * parts - 1) / total);
+    int groups, splits, nkb, total;  // groups per (entry, split), splits of k, blocks of k, groups in all
+    __device__ __forceinline__ int start(int part) const {
+        return static_cast<int>(static_cast<long long>(part) * total / static_cast<int>(gridDim.x));
     }
 };
 
-struct Seg {
-    int entry, tile, kb0, kb1, x0;  // x0: the tile's first block in the line
+// Splits of k for the down product: a part takes q = ceil(groups / parts)
+// groups of ceil(kb / splits) blocks.  A stage of q groups takes q blocks'
+// time, but at least about three: it holds one block of k of each group, and
+// five stages in flight have to cover the latency of memory.
+__device__ __forceinline__ int choose_splits(const MoeParams& p, int entries, int groups) {
+    int best = 1;
+    long long least = 0x7fffffffffffffffll;
+    for (int s = 1; s <= p.max_split && s <= p.kb_f; s *= 2) {
+        const long long q = (static_cast<long long>(entries) * groups * s + gridDim.x - 1) / gridDim.x;
+        const long long cost = max(q, 3ll) * ((p.kb_f + s - 1) / s);
+        if (cost < least) {
+            least = cost;
+            best = s;
+        }
+    }
+    return best;
+}
+
+// Up to 8 groups of one entry and split.
+struct Pass {
+    int entry, split, g0, n, k0, k1;
 };
 
 struct Walk {
     int cur, end;
-    __device__ __forceinline__ explicit Walk(const Line& l) : cur(0), end(0) {
-        if (static_cast<int>(blockIdx.x) < l.parts) {
-            cur = l.start(blockIdx.x);
-            end = l.start(blockIdx.x + 1);
-        }
-    }
-    __device__ __forceinline__ bool next(const Line& l, Seg& s) {
+    __device__ __forceinline__ Walk(const Line& l, int part) : cur(l.start(part)), end(l.start(part + 1)) {}
+    __device__ __forceinline__ bool next(const Line& l, Pass& s) {
         if (cur >= end) return false;
-        const int ft = cur / l.nkb;
-        s.x0 = ft * l.nkb;
-        s.kb0 = cur - s.x0;
-        s.kb1 = min(l.nkb, s.kb0 + (end - cur));
-        s.entry = ft / l.tiles;
-        s.tile = ft - s.entry * l.tiles;
-        cur += s.kb1 - s.kb0;
+        const int es = cur / l.groups;
+        s.g0 = cur - es * l.groups;
+        s.entry = es / l.splits;
+        s.split = es - s.entry * l.splits;
+        const int avail = min(l.groups - s.g0, end - cur), passes = (avail + kConsumers - 1) / kConsumers;
+        s.n = (avail + passes - 1) / passes;  // passes of about one size
+        s.k0 = static_cast<int>(static_cast<long long>(s.split) * l.nkb / l.splits);
+        s.k1 = static_cast<int>(static_cast<long long>(s.split + 1) * l.nkb / l.splits);
+        cur += s.n;
         return true;
     }
 };
@@ -471,11 +573,19 @@ __device__ __forceinline__ uint32_t e4m3_to_half2(uint32_t two) {
 
 // ---- the kernel ------------------------------------------------------------
 
+__device__ __forceinline__ uint32_t mul_half2(uint32_t v, __half2 s) {
+    __half2 x;
+    memcpy(&x, &v, 4);
+    x = __hmul2(x, s);
+    memcpy(&v, &x, 4);
+    return v;
+}
+
 template <int NG, bool LO>
 struct Consumer {
-    using C = MoeCfg<NG, LO>;
     using Act = ActBlock<LO>;
-    // gate / up (or the two halves of 256 down rows) x token groups x fragment
+    static constexpr int kChains = LO ? 4 : 2;
+    // gate / up (or the two boxes of down rows) x token groups x fragment
     float acc[2][NG][4];
 
     __device__ __forceinline__ void clear() {
@@ -487,13 +597,17 @@ struct Consumer {
                 for (int i = 0; i < 4; ++i) acc[b][n][i] = 0.0f;
     }
 
-    // One block of 128: this warp's 16 rows of both boxes times ng token groups.
-    __device__ __forceinline__ void block(const uint8_t* stage, int warp, int lane, int ng, float s0, float s1) {
+    // One block of 128: a group's 16 rows of both boxes times ng token groups.
+    // GROUPED: a scale per 16 values (thread t's two 16s are its own).
+    // PACKED (LO, at most 4 tokens): column 2c is token c's f16 values and
+    // column 2c + 1 their remainders, in one MMA; unpack() adds them.
+    template <bool GROUPED, bool PACKED>
+    __device__ __forceinline__ void block(const uint8_t* rows, const uint8_t* act, int lane, int ng, float s0, float s1) {
         const int g = lane >> 2, t = lane & 3;
         uint32_t a[2][8][4];  // box, k step, fragment
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            const uint8_t* row = stage + b * kBoxBytes + (warp * 16 + g) * kF8Block;
+            const uint8_t* row = rows + b * kBoxBytes + g * kF8Block;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int at = ((2 * t + c) ^ g) * 16;
@@ -509,81 +623,231 @@ struct Consumer {
                 }
             }
         }
-        const uint8_t* act = stage + 2 * kBoxBytes;
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
-            if (n >= ng) break;
-            const uint8_t* row = act + (n * 8 + g) * Act::kPitch + t * 16;
-            float d[2][4] = {};
+            if (n >= (PACKED ? 1 : ng)) break;
+            const uint8_t* row = act + (PACKED ? g >> 1 : n * 8 + g) * Act::kPitch;
+            float xs;  // the block's power of two for column g
+            __half2 f[2];
+            if constexpr (GROUPED) {
+                const float2 s = *reinterpret_cast<const float2*>(row + Act::kScaleAt + t * 8);
+                xs = fmaxf(s.x, s.y);
+                xs = fmaxf(xs, __shfl_xor_sync(0xffffffffu, xs, 1));
+                xs = fmaxf(xs, __shfl_xor_sync(0xffffffffu, xs, 2));
+                const float inv = __uint_as_float((254u << 23) - __float_as_uint(xs));  // powers of two up to 2^114
+                f[0] = __float2half2_rn(s.x * inv);
+                f[1] = __float2half2_rn(s.y * inv);
+            } else {
+                xs = *reinterpret_cast<const float*>(row + Act::kScaleAt);
+            }
+            // independent accumulators: eight MMAs one behind the other would
+            // take longer than the block's copy
+            float d[2][kChains][4] = {};
 #pragma unroll
-            for (int part = 0; part < (LO ? 2 : 1); ++part)
+            for (int part = 0; part < (LO && !PACKED ? 2 : 1); ++part)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(row + part * 256 + j * 64);
-                    mma_f16(d[0], a[0][2 * j], v.x, v.y);
-                    mma_f16(d[1], a[1][2 * j], v.x, v.y);
-                    mma_f16(d[0], a[0][2 * j + 1], v.z, v.w);
-                    mma_f16(d[1], a[1][2 * j + 1], v.z, v.w);
+                    uint4 v = *reinterpret_cast<const uint4*>(row + (PACKED ? g & 1 : part) * 256 + j * 64 + t * 16);
+                    if constexpr (GROUPED) {
+                        v.x = mul_half2(v.x, f[j >> 1]);
+                        v.y = mul_half2(v.y, f[j >> 1]);
+                        v.z = mul_half2(v.z, f[j >> 1]);
+                        v.w = mul_half2(v.w, f[j >> 1]);
+                    }
+                    const int c0 = (PACKED ? 2 * (j & 1) : 2 * part) % kChains, c1 = (c0 + 1) % kChains;
+                    mma_f16(d[0][c0], a[0][2 * j], v.x, v.y);
+                    mma_f16(d[1][c0], a[1][2 * j], v.x, v.y);
+                    mma_f16(d[0][c1], a[0][2 * j + 1], v.z, v.w);
+                    mma_f16(d[1][c1], a[1][2 * j + 1], v.z, v.w);
+                }
+#pragma unroll
+            for (int c = 1; c < kChains; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    d[0][0][i] += d[0][c][i];
+                    d[1][0][i] += d[1][c][i];
                 }
             // columns 2t and 2t + 1
-            const uint8_t* sc = act + (n * 8 + 2 * t) * Act::kPitch + Act::kScaleAt;
-            const float x0 = *reinterpret_cast<const float*>(sc), x1 = *reinterpret_cast<const float*>(sc + Act::kPitch);
+            const float x0 = __shfl_sync(0xffffffffu, xs, 8 * t), x1 = __shfl_sync(0xffffffffu, xs, 8 * t + 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float xs = (i & 1) ? x1 : x0;
-                acc[0][n][i] = fmaf(d[0][i], s0 * xs, acc[0][n][i]);
-                acc[1][n][i] = fmaf(d[1][i], s1 * xs, acc[1][n][i]);
+                const float x = (i & 1) ? x1 : x0;
+                acc[0][n][i] = fmaf(d[0][0][i], s0 * x, acc[0][n][i]);
+                acc[1][n][i] = fmaf(d[1][0][i], s1 * x, acc[1][n][i]);
             }
         }
     }
 
-    __device__ __forceinline__ void put_part(float* to, int ng) const {
+    // PACKED sums to the plain layout: token c = 2t + j in thread t's column j.
+    __device__ __forceinline__ void unpack(int lane) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int n = 0; n < NG; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (n < ng) __stcg(to + ((n * 2 + b) * 4 + i) * kConsThreads, acc[b][n][i]);
+            for (int r = 0; r < 2; ++r) {
+                const float sum = acc[b][0][2 * r] + acc[b][0][2 * r + 1];  // token t
+                const int from = (lane & ~3) | ((2 * lane) & 3);
+                acc[b][0][2 * r] = __shfl_sync(0xffffffffu, sum, from);
+                acc[b][0][2 * r + 1] = __shfl_sync(0xffffffffu, sum, from | 1);
+            }
     }
 
-    __device__ __forceinline__ void add_part(const float* from, int ng) {
+    // Adds the sums of the warps that share this one's group (ways of them,
+    // n2 warps apart) to the first one's, in order.
+    __device__ __forceinline__ void reduce(float* red, int warp, int lane, int ng, int n2, int ways) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int n = 0; n < NG; ++n) {
+            if (n >= ng) break;
+            float4* mine = reinterpret_cast<float4*>(red) + (warp * 2) * 32 + lane;
+            if (warp >= n2) {
+                mine[0] = make_float4(acc[0][n][0], acc[0][n][1], acc[0][n][2], acc[0][n][3]);
+                mine[32] = make_float4(acc[1][n][0], acc[1][n][1], acc[1][n][2], acc[1][n][3]);
+            }
+            cons_bar();
+            if (warp < n2)
+                for (int w = 1; w < ways; ++w) {
+                    const float4 u = mine[w * n2 * 64], v = mine[w * n2 * 64 + 32];
+                    acc[0][n][0] += u.x, acc[0][n][1] += u.y, acc[0][n][2] += u.z, acc[0][n][3] += u.w;
+                    acc[1][n][0] += v.x, acc[1][n][1] += v.y, acc[1][n][2] += v.z, acc[1][n][3] += v.w;
+                }
+            cons_bar();
+        }
+    }
+
+    // This group's 16 hidden values per token, from gate and up.
+    __device__ __forceinline__ void hidden(const MoeParams& p, int group, int first, int n, int ng, int lane) const {
+        const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-            for (int n = 0; n < NG; ++n)
+        for (int i = 0; i < NG; ++i) {
+            if (i >= ng) break;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (n < ng) acc[b][n][i] += __ldcg(from + ((n * 2 + b) * 4 + i) * kConsThreads);
+            for (int j = 0; j < 2; ++j) {
+                float h[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float gate = acc[0][i][j + 2 * r];
+                    h[r] = gate / (1.0f + expf(-gate)) * acc[1][i][j + 2 * r];
+                }
+                float m = fmaxf(fabsf(h[0]), fabsf(h[1])), inv;
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                const float sc = act_scale(m, inv);
+                const int col = i * 8 + 2 * t + j;
+                if (col < n) {
+                    uint8_t* blk = p.hq + (static_cast<long long>(first + col) * p.kb_f + (group >> 3)) * Act::kBytes;
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float v = h[r] * inv;
+                        const __half hi = __float2half_rn(v);
+                        const int at = act_at((group & 7) * 16 + g + 8 * r);
+                        *reinterpret_cast<__half*>(blk + at) = hi;
+                        if constexpr (LO) *reinterpret_cast<__half*>(blk + 256 + at) = __float2half_rn(v - __half2float(hi));
+                    }
+                    if (g == 0) reinterpret_cast<float*>(blk + Act::kScaleAt)[group & 7] = sc;
+                    // the rest of the last block: zeros
+                    if ((group + 1) * kBoxRows == p.f)
+                        for (int rest = (group & 7) + 1; rest < 8; ++rest) {
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                const int at = act_at(rest * 16 + g + 8 * r);
+                                *reinterpret_cast<__half*>(blk + at) = __half(0.0f);
+                                if constexpr (LO) *reinterpret_cast<__half*>(blk + 256 + at) = __half(0.0f);
+                            }
+                            if (g == 0) reinterpret_cast<float*>(blk + Act::kScaleAt)[rest] = 1.17549435e-38f;
+                        }
+                }
+            }
+        }
+    }
+
+    // This group's 32 down rows of its slots.
+    __device__ __forceinline__ void slot_rows(const MoeParams& p, const Tables& tb, int group, int split, int splits,
+                                              int first, int n, int ng, int lane) const {
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            if (i >= ng) break;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int col = i * 8 + 2 * t + j;
+                if (col < n) {
+                    float* o = p.pair_out + (static_cast<long long>(tb.order[first + col]) * splits + split) * p.h;
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const int row = group * 32 + b * kBoxRows + g + 8 * r;
+                            if (row < p.h) __stcg(o + row, acc[b][i][j + 2 * r]);
+                        }
+                }
+            }
+        }
     }
 };
+
+// The weighted sums of the columns of the groups in `mask` (bit i: group
+// g0 + i), a warp per group and token; slots and splits in order.
+__device__ __forceinline__ void combine(const MoeParams& p, const Tables& tb, int g0, uint32_t mask, int splits, int warp,
+                                        int lane) {
+    const int items = __popc(mask) * p.t;
+    for (int item = warp; item < items; item += kConsumers) {
+        const int nth = item / p.t, tok = item - nth * p.t;
+        const int row = (g0 + static_cast<int>(__fns(mask, 0, nth + 1))) * 32 + lane;
+        if (row >= p.h) continue;
+        float y = 0.0f;
+        if (splits == 1) {
+#pragma unroll 4
+            for (int k = 0; k < p.top; ++k) {
+                const int pair = tok * p.top + k;
+                const float w = tb.pair_e[pair] < 0 ? 0.0f : tb.pair_w[pair];
+                const float d = tb.pair_e[pair] < 0 ? 0.0f : __ldcg(p.pair_out + static_cast<long long>(pair) * p.h + row);
+                y = fmaf(w, d, y);
+            }
+        } else {
+            for (int k = 0; k < p.top; ++k) {
+                const int pair = tok * p.top + k;
+                if (tb.pair_e[pair] < 0) continue;
+                const float* from = p.pair_out + static_cast<long long>(pair) * splits * p.h + row;
+                float d[8];
+#pragma unroll
+                for (int s = 0; s < 8; ++s) d[s] = s < splits ? __ldcg(from + static_cast<long long>(s) * p.h) : 0.0f;
+                float sum = 0.0f;
+#pragma unroll
+                for (int s = 0; s < 8; ++s) sum += d[s];
+                y = fmaf(tb.pair_w[pair], sum, y);
+            }
+        }
+        store_dense(p.out, p.type, tok * p.ldo + row, y);
+    }
+}
 
 template <int NG, bool LO>
 __global__ void __launch_bounds__(kThreads, 1) moe_f8_kernel(const __grid_constant__ MoeParams p) {
     using C = MoeCfg<NG, LO>;
     using Act = ActBlock<LO>;
     constexpr int S = C::kStages, kCap = NG * 8;
-    constexpr int kPart = 8 * NG * kConsThreads;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOffset);
     uint64_t* empty = full + S;
     volatile uint32_t* abort = reinterpret_cast<uint32_t*>(empty + S);
-    uint32_t* last_flag = reinterpret_cast<uint32_t*>(empty + S) + 1;
+    volatile uint32_t* last_mask = abort + 1;
+    volatile int* ticket = reinterpret_cast<int*>(empty + S) + 2;
     Tables tb;
-    tb.pair_w = reinterpret_cast<float*>(smem + C::kTables);
+    tb.red = reinterpret_cast<float*>(smem + C::kTables);
+    tb.pair_w = tb.red + kRedBytes / 4;
     tb.entry = reinterpret_cast<int*>(tb.pair_w + kMaxPairs);
     tb.count = tb.entry + kMaxPairs;
     tb.info = tb.count + kMoeMaxExperts;
-    tb.red = reinterpret_cast<float*>(tb.info + 4);
-    tb.pair_e = reinterpret_cast<short*>(tb.red + kConsumers * kMoeMaxTokens);
+    tb.pair_e = reinterpret_cast<short*>(tb.info + 4);
     tb.order = tb.pair_e + kMaxPairs;
+    short* held = tb.order + kMaxPairs;  // this CTA's parts
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const unsigned grid = gridDim.x;
+    const int parts = static_cast<int>(gridDim.x);
     if (threadIdx.x == 0) {
+        *ticket = static_cast<int>(atomicAdd(p.ctrl + kTicket, 1u));
         for (int s = 0; s < S; ++s) {
-            mbar_init(&full[s], 2);  // weights, activations
+            mbar_init(&full[s], kProducers);  // three for weights, one for activations
             mbar_init(&empty[s], kConsumers);
         }
         *abort = 0u;
@@ -592,20 +856,46 @@ __global__ void __launch_bounds__(kThreads, 1) moe_f8_kernel(const __grid_consta
         prefetch_tmap(&p.tm_up);
         prefetch_tmap(&p.tm_down);
     }
+    __syncthreads();
 
     // ---- phase 0 ----
-    layout_x<LO>(p, blockIdx.x * (kThreads / 32) + warp, grid * (kThreads / 32), lane);
-    if (p.router) router_products(p, tb, warp, lane);
-    asm volatile("fence.proxy.async.global;" ::: "memory");
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        grid_arrive(p.ctrl + kBarrier);
-        if (!grid_wait(p.ctrl + kBarrier, grid, abort)) fail(p.err, abort, kErrTimeoutGrid);
+    int nheld = 0;
+    bool ready = false;
+    while (!ready) {
+        const int part = *ticket;
+        if (part < parts) {
+            layout_x<LO>(p, (part * kWarps + warp) * 2 + (lane >> 4), parts * kWarps * 2, lane);
+            if (p.router) router_products(p, tb, part, warp, lane);
+            asm volatile("fence.proxy.async.global;" ::: "memory");
+            if (threadIdx.x == 0) held[nheld] = static_cast<short>(part);
+            ++nheld;
+        }
+        __syncthreads();
+        bool here = false;
+        if (threadIdx.x == 0) {
+            if (part < parts) {
+                grid_arrive(p.ctrl + kBarrier);
+                here = grid_wait_some(p.ctrl + kBarrier, parts, kHelpNs);
+                if (!here) *ticket = static_cast<int>(atomicAdd(p.ctrl + kTicket, 1u));
+            } else {
+                // every part is held by a CTA that runs
+                here = true;
+                if (!grid_wait(p.ctrl + kBarrier, parts, abort)) fail(p.err, abort, kErrTimeoutGrid);
+            }
+        }
+        ready = __syncthreads_or(here);
     }
     if (!__syncthreads_or(threadIdx.x == 0 && *abort != 0u)) {
         // ---- routing, by every CTA for itself ----
         if (p.router) {
-            for (int tok = warp; tok < p.t; tok += kThreads / 32) choose(p, tb, tok, lane);
+            for (int tok = warp; tok < p.t; tok += kWarps) {
+                if (p.e <= 32)
+                    choose<1>(p, tb, tok, lane);
+                else if (p.e <= 64)
+                    choose<2>(p, tb, tok, lane);
+                else
+                    choose<kMoeMaxExperts / 32>(p, tb, tok, lane);
+            }
         } else {
             for (int i = threadIdx.x; i < p.t * p.top; i += kThreads) {
                 int ex = p.ids[i];
@@ -617,274 +907,209 @@ __global__ void __launch_bounds__(kThreads, 1) moe_f8_kernel(const __grid_consta
                 tb.pair_w[i] = p.weights[i];
             }
         }
+        // pairs are read eight at a time
+        for (int i = p.t * p.top + threadIdx.x; i < (p.t * p.top + 7) / 8 * 8; i += kThreads) tb.pair_e[i] = -1;
         __syncthreads();
         build_tables(p, tb, kCap);
         const int entries = tb.info[0];
-        const Line line1(entries, p.tiles_f, p.kb_h), line2(entries, p.tiles_h, p.kb_f);
+        const int groups1 = p.f / kBoxRows, groups2 = (p.h + 31) / 32;
+        const int splits = choose_splits(p, entries, groups2);
+        const Line line1{groups1, 1, p.kb_h, entries * groups1};
+        const Line line2{groups2, splits, p.kb_f, entries * groups2 * splits};
 
-        if (entries == 0) {
-            // no slot names an expert: the sums are empty
-            for (long long i = blockIdx.x * kThreads + threadIdx.x; i < static_cast<long long>(p.t) * p.h;
-                 i += grid * kThreads)
-                store_dense(p.out, p.type, i / p.h * p.ldo + i % p.h, 0.0f);
-        } else if (warp == kConsumers) {
-            // ---- producer warp ----
+        if (warp >= kConsumers) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+            // ---- producers: three threads for the weights, each every third box of
+            // a stage, and a warp for the activations (an issued copy costs its
+            // thread about 150 cycles; one thread for all took longer over a stage
+            // than the copies themselves) ----
+            const int pw = warp - kConsumers;
             asm volatile("fence.proxy.async.global;" ::: "memory");
-            int gw = 0, ga = 0;  // stages whose weights / activations were issued
+            int g = 0;  // stages issued
             bool ok = true;
-            auto issue_w = [&](int phase, const Seg& s, int kb) {
-                const int st = gw % S;
+            auto stage_free = [&] {
+                if (g >= S && !wait_or_abort(&empty[g % S], ((g / S) & 1) ^ 1, abort)) {
+                    if (!*abort) fail(p.err, abort, kErrTimeoutEmpty);
+                    ok = false;
+                }
+                return ok;
+            };
+            if (pw < kProducers - 1) {
                 if (lane == 0) {
-                    if (gw >= S && !wait_or_abort(&empty[st], ((gw / S) & 1) ^ 1, abort)) {
-                        if (!*abort) fail(p.err, abort, kErrTimeoutEmpty);
-                        ok = false;
-                    } else {
-                        uint8_t* dst = smem + st * C::kStage;
-                        const int ex = tb.entry[s.entry] >> 16;
-                        mbar_arrive_expect_tx(&full[st], 2 * kBoxBytes);
-                        if (phase == 1) {
-                            tma_load_3d(dst, &p.tm_gate, &full[st], kb * kF8Block, s.tile * kBoxRows, ex);
-                            tma_load_3d(dst + kBoxBytes, &p.tm_up, &full[st], kb * kF8Block, s.tile * kBoxRows, ex);
-                        } else {
-                            tma_load_3d(dst, &p.tm_down, &full[st], kb * kF8Block, s.tile * 2 * kBoxRows, ex);
-                            tma_load_3d(dst + kBoxBytes, &p.tm_down, &full[st], kb * kF8Block,
-                                        s.tile * 2 * kBoxRows + kBoxRows, ex);
+                    for (int step = 0; ok && step < 2 * nheld; ++step) {
+                        const int phase = step < nheld ? 1 : 2;
+                        const Line& line = phase == 1 ? line1 : line2;
+                        Walk walk(line, held[phase == 1 ? step : step - nheld]);
+                        Pass s;
+                        while (ok && walk.next(line, s)) {
+                            const int ex = tb.entry[s.entry] >> 16, boxes = 2 * s.n;
+                            const uint32_t bytes = (boxes - pw + kProducers - 2) / (kProducers - 1) * kBoxBytes;
+                            for (int kb = s.k0; kb < s.k1 && stage_free(); ++kb, ++g) {
+                                uint64_t* bar = &full[g % S];
+                                uint8_t* dst = smem + g % S * C::kStage;
+                                mbar_arrive_expect_tx(bar, bytes);
+                                for (int i = pw; i < boxes; i += kProducers - 1) {
+                                    const int grp = s.g0 + (i >> 1), box = i & 1;
+                                    if (phase == 1)
+                                        tma_load_3d(dst + i * kBoxBytes, box ? &p.tm_up : &p.tm_gate, bar,
+                                                    kb * kF8Block, grp * kBoxRows, ex);
+                                    else
+                                        tma_load_3d(dst + i * kBoxBytes, &p.tm_down, bar, kb * kF8Block,
+                                                    grp * 32 + box * kBoxRows, ex);
+                                }
+                            }
                         }
                     }
                 }
-                ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-                if (ok) ++gw;
-            };
-            auto issue_a = [&](int phase, const Seg& s, int kb) {
-                const int st = ga % S;
-                int first, n;
-                entry_pairs(tb, s.entry, kCap, first, n);
-                uint8_t* dst = smem + st * C::kStage + 2 * kBoxBytes;
-                if (lane == 0) mbar_arrive_expect_tx(&full[st], n * Act::kBytes);
-                __syncwarp();
-                for (int i = lane; i < n; i += 32) {
-                    const uint8_t* src =
-                        phase == 1
-                            ? p.xq + (static_cast<long long>(tb.order[first + i] / p.top) * p.kb_h + kb) * Act::kBytes
-                            : p.hq + (static_cast<long long>(first + i) * p.kb_f + kb) * Act::kBytes;
-                    bulk_load(dst + i * Act::kPitch, src, Act::kBytes, &full[st]);
-                }
-                ++ga;
-            };
-            Seg s;
-            {
-                Walk walk(line1);
-                while (ok && walk.next(line1, s))
-                    for (int kb = s.kb0; ok && kb < s.kb1; ++kb) {
-                        issue_w(1, s, kb);
-                        if (ok) issue_a(1, s, kb);
+            } else {
+                for (int step = 0; ok && step < 2 * nheld; ++step) {
+                    const int phase = step < nheld ? 1 : 2;
+                    const Line& line = phase == 1 ? line1 : line2;
+                    Walk walk(line, held[phase == 1 ? step : step - nheld]);
+                    if (step == nheld) {
+                        // the hidden values of all CTAs; the other producers' weights
+                        // are on their way meanwhile
+                        if (!grid_wait(p.ctrl + kBarrier, 2 * parts, abort)) {
+                            if (lane == 0 && !*abort) fail(p.err, abort, kErrTimeoutGrid);
+                            ok = false;
+                        }
+                        asm volatile("fence.proxy.async.global;" ::: "memory");
+                        ok = __all_sync(0xffffffffu, ok);
                     }
-            }
-            // phase 2: up to S stages of weights ahead of the barrier
-            {
-                Walk walk(line2), walk_a(line2);
-                Seg sa;
-                bool more = walk.next(line2, s), more_a = walk_a.next(line2, sa);
-                int kb = more ? s.kb0 : 0, kba = more_a ? sa.kb0 : 0;
-                auto step_w = [&] {
-                    issue_w(2, s, kb);
-                    if (ok && ++kb == s.kb1) {
-                        more = walk.next(line2, s);
-                        kb = s.kb0;
-                    }
-                };
-                for (int i = 0; ok && more && i < S; ++i) step_w();
-                if (ok && more_a) {
-                    if (lane == 0 && !grid_wait(p.ctrl + kBarrier, 2 * grid, abort)) {
-                        if (!*abort) fail(p.err, abort, kErrTimeoutGrid);
-                        ok = false;
-                    }
-                    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-                    asm volatile("fence.proxy.async.global;" ::: "memory");
-                }
-                while (ok && more_a) {
-                    if (ga == gw) step_w();  // past the weights issued ahead
-                    if (!ok) break;
-                    issue_a(2, sa, kba);
-                    if (++kba == sa.kb1) {
-                        more_a = walk_a.next(line2, sa);
-                        kba = sa.kb0;
+                    Pass s;
+                    while (ok && walk.next(line, s)) {
+                        int first, n;
+                        entry_pairs(tb, s.entry, kCap, first, n);
+                        // this lane's rows (the second with more than 32 tokens)
+                        const uint8_t* src[2];
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const int i = min(lane + 32 * r, n - 1);
+                            src[r] = phase == 1 ? p.xq + static_cast<long long>(tb.order[first + i] / p.top) * p.kb_h * Act::kBytes
+                                                : p.hq + static_cast<long long>(first + i) * p.kb_f * Act::kBytes;
+                        }
+                        for (int kb = s.k0; kb < s.k1; ++kb, ++g) {
+                            if (lane == 0 && stage_free()) mbar_arrive_expect_tx(&full[g % S], n * Act::kBytes);
+                            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+                            if (!ok) break;
+                            uint8_t* dst = smem + g % S * C::kStage + kConsumers * kGroupBytes;
+#pragma unroll
+                            for (int r = 0; r < 2; ++r)
+                                if (lane + 32 * r < n)
+                                    bulk_load(dst + (lane + 32 * r) * Act::kPitch, src[r] + kb * Act::kBytes, Act::kBytes,
+                                              &full[g % S]);
+                        }
                     }
                 }
             }
+            __syncwarp();
             // copies in flight must land before the CTA exits
             if (lane == 0)
-                for (int i = max(0, gw - S); i < gw; ++i)
+                for (int i = max(0, g - S); i < g; ++i)
                     if (!mbar_wait(&full[i % S], (i / S) & 1)) {
                         atomicCAS(p.err, 0, kErrTimeoutDrain);
                         break;
                     }
             __syncwarp();
         } else {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
             // ---- consumer warps ----
-            const int g = lane >> 2, t = lane & 3;
             Consumer<NG, LO> c;
             int stage = 0;
             bool ok = true;
-            for (int phase = 1; ok && phase <= 2; ++phase) {
+            for (int step = 0; ok && step < 2 * nheld; ++step) {
+                const int phase = step < nheld ? 1 : 2, part = held[step < nheld ? step : step - nheld];
                 const Line& line = phase == 1 ? line1 : line2;
-                Walk walk(line);
-                Seg s;
+                if (entries == 0 && phase == 2) {
+                    // no slot names an expert: the sums are empty
+                    for (long long i = part * kConsThreads + threadIdx.x; i < static_cast<long long>(p.t) * p.h;
+                         i += parts * kConsThreads)
+                        store_dense(p.out, p.type, i / p.h * p.ldo + i % p.h, 0.0f);
+                }
+                Walk walk(line, part);
+                Pass s;
                 while (ok && walk.next(line, s)) {
                     int first, n;
                     entry_pairs(tb, s.entry, kCap, first, n);
                     const int ng = (n + 7) / 8, ex = tb.entry[s.entry] >> 16;
+                    // n2 warps with a group each, `ways` of them sharing its blocks
+                    const int n2 = s.n > 4 ? 8 : s.n > 2 ? 4 : s.n, ways = kConsumers / n2;
+                    const int gi = warp & (n2 - 1), way = warp / n2;
+                    const bool mine = gi < s.n, packed = n <= 4;
+                    const int group = s.g0 + (mine ? gi : 0);
                     const float *s0, *s1;
                     if (phase == 1) {
-                        s0 = p.gate_s + ex * p.gate_ss + static_cast<long long>(s.tile) * p.kb_h;
-                        s1 = p.up_s + ex * p.up_ss + static_cast<long long>(s.tile) * p.kb_h;
+                        s0 = p.gate_s + ex * p.gate_ss + static_cast<long long>(group >> 3) * p.kb_h;
+                        s1 = p.up_s + ex * p.up_ss + static_cast<long long>(group >> 3) * p.kb_h;
                     } else {
-                        // the last tile's second half may not exist: any scale, its rows are zero
-                        const int rb = 2 * s.tile, last = (p.h + kF8Block - 1) / kF8Block - 1;
-                        s0 = p.down_s + ex * p.down_ss + static_cast<long long>(rb) * p.kb_f;
-                        s1 = p.down_s + ex * p.down_ss + static_cast<long long>(min(rb + 1, last)) * p.kb_f;
+                        s0 = s1 = p.down_s + ex * p.down_ss + static_cast<long long>(group >> 2) * p.kb_f;
                     }
                     c.clear();
-                    float w0 = __ldg(s0 + s.kb0), w1 = __ldg(s1 + s.kb0);
-                    for (int kb = s.kb0; kb < s.kb1; ++kb, ++stage) {
+                    float w0 = __ldg(s0 + min(s.k0 + way, s.k1 - 1)), w1 = __ldg(s1 + min(s.k0 + way, s.k1 - 1));
+                    for (int kb = s.k0; kb < s.k1; ++kb, ++stage) {
                         const int st = stage % S;
-                        const int nk = min(kb + 1, s.kb1 - 1);
-                        const float n0 = __ldg(s0 + nk), n1 = __ldg(s1 + nk);
-                        int ready = 0;
-                        if (lane == 0) ready = wait_or_abort(&full[st], (stage / S) & 1, abort) ? 1 : 0;
-                        ready = __shfl_sync(0xffffffffu, ready, 0);
-                        if (!ready) {
+                        if (!wait_or_abort(&full[st], (stage / S) & 1, abort)) {
                             if (lane == 0 && !*abort) fail(p.err, abort, kErrTimeoutFull);
                             ok = false;
-                            break;
                         }
-                        c.block(smem + st * C::kStage, warp, lane, ng, w0, w1);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        if (mine && ((kb - s.k0) & (ways - 1)) == way) {
+                            const int nk = min(kb + ways, s.k1 - 1);
+                            const float n0 = __ldg(s0 + nk), n1 = __ldg(s1 + nk);
+                            const uint8_t* at = smem + st * C::kStage;
+                            const uint8_t *rows = at + gi * kGroupBytes, *act = at + kConsumers * kGroupBytes;
+                            if (LO && NG == 1 && packed) {
+                                if (phase == 1)
+                                    c.template block<false, true>(rows, act, lane, ng, w0, w1);
+                                else
+                                    c.template block<true, true>(rows, act, lane, ng, w0, w1);
+                            } else if (phase == 1) {
+                                c.template block<false, false>(rows, act, lane, ng, w0, w1);
+                            } else {
+                                c.template block<true, false>(rows, act, lane, ng, w0, w1);
+                            }
+                            w0 = n0;
+                            w1 = n1;
+                        }
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&empty[st]);
-                        w0 = n0;
-                        w1 = n1;
                     }
                     // one decision for all consumer warps
                     if (cons_any(!ok)) {
                         ok = false;
                         break;
                     }
-                    if (s.kb1 - s.kb0 != line.nkb) {
-                        // a cut tile
-                        float* mine = p.part + (2ll * blockIdx.x + (s.kb0 == 0 ? 1 : 0)) * kPart + threadIdx.x;
-                        c.put_part(mine, ng);
-                        const int a = line.owner(s.x0), b = line.owner(s.x0 + line.nkb - 1);
-                        __threadfence();
-                        cons_bar();
-                        if (threadIdx.x == 0) {
-                            // a tile that is cut is the last of its first CTA
-                            unsigned* cut = p.ctrl + (phase == 1 ? kCut1 : kCut2) + a;
-                            *last_flag = atomicAdd(cut, 1u) == static_cast<unsigned>(b - a) ? 1u : 0u;
-                            if (*last_flag) *cut = 0u;
-                        }
-                        cons_bar();
-                        if (!*last_flag) continue;
-                        __threadfence();
-                        c.clear();
-                        for (int cta = a; cta <= b; ++cta)
-                            c.add_part(p.part + (2ll * cta + (cta == a ? 1 : 0)) * kPart + threadIdx.x, ng);
-                    }
+                    if (LO && NG == 1 && packed) c.unpack(lane);
+                    if (ways > 1) c.reduce(tb.red, warp, lane, ng, n2, ways);
+                    const bool owner = mine && way == 0;
                     if (phase == 1) {
-                        // hidden values of 128 rows; rows behind f are zero (zero weights)
-                        float hv[NG][4], am[NG][2];
-#pragma unroll
-                        for (int i = 0; i < NG; ++i) {
-                            if (i >= ng) break;
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const float gate = c.acc[0][i][j];
-                                hv[i][j] = gate / (1.0f + expf(-gate)) * c.acc[1][i][j];
-                            }
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                float m = fmaxf(fabsf(hv[i][j]), fabsf(hv[i][j + 2]));
-#pragma unroll
-                                for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                                am[i][j] = m;
-                                if (g == 0) tb.red[warp * kMoeMaxTokens + i * 8 + 2 * t + j] = m;
-                            }
-                        }
-                        cons_bar();
-#pragma unroll
-                        for (int i = 0; i < NG; ++i) {
-                            if (i >= ng) break;
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                const int col = i * 8 + 2 * t + j;
-                                float m = 0.0f, inv;
-                                for (int w = 0; w < kConsumers; ++w) m = fmaxf(m, tb.red[w * kMoeMaxTokens + col]);
-                                const float sc = act_scale(m, inv);
-                                if (col < n) {
-                                    uint8_t* blk = p.hq + (static_cast<long long>(first + col) * p.kb_f + s.tile) * Act::kBytes;
-#pragma unroll
-                                    for (int r = 0; r < 2; ++r) {
-                                        const float v = hv[i][j + 2 * r] * inv;
-                                        const __half hi = __float2half_rn(v);
-                                        const int at = act_at(warp * 16 + g + 8 * r);
-                                        *reinterpret_cast<__half*>(blk + at) = hi;
-                                        if constexpr (LO)
-                                            *reinterpret_cast<__half*>(blk + 256 + at) = __float2half_rn(v - __half2float(hi));
-                                    }
-                                    if (warp == 0 && g == 0) *reinterpret_cast<float*>(blk + Act::kScaleAt) = sc;
-                                }
-                            }
-                        }
-                        cons_bar();  // red is free again
+                        if (owner) c.hidden(p, group, first, n, ng, lane);
                     } else {
-                        // this expert's rows of its slots, then the last expert of the column tile sums them
-                        const int row0 = s.tile * 2 * kBoxRows + warp * 16 + g;
-#pragma unroll
-                        for (int i = 0; i < NG; ++i) {
-                            if (i >= ng) break;
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                const int col = i * 8 + 2 * t + j;
-                                if (col < n) {
-                                    float* o = p.pair_out + static_cast<long long>(tb.order[first + col]) * p.h;
-#pragma unroll
-                                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                                        for (int r = 0; r < 2; ++r) {
-                                            const int row = row0 + b * kBoxRows + 8 * r;
-                                            if (row < p.h) __stcg(o + row, c.acc[b][i][j + 2 * r]);
-                                        }
-                                }
-                            }
-                        }
+                        if (owner) c.slot_rows(p, tb, group, s.split, splits, first, n, ng, lane);
+                        // the last to add to 32 columns sums them
                         __threadfence();
                         cons_bar();
-                        if (threadIdx.x == 0) {
-                            unsigned* cnt = p.ctrl + kCombine + s.tile;
-                            *last_flag = atomicAdd(cnt, 1u) == static_cast<unsigned>(entries - 1) ? 1u : 0u;
-                            if (*last_flag) *cnt = 0u;
+                        if (warp == 0) {
+                            bool last = false;
+                            if (lane < s.n) {
+                                unsigned* cnt = p.ctrl + kCombine + s.g0 + lane;
+                                last = atomicAdd(cnt, 1u) == static_cast<unsigned>(entries * splits - 1);
+                                if (last) *cnt = 0u;
+                            }
+                            const uint32_t mask = __ballot_sync(0xffffffffu, last);
+                            if (lane == 0) *last_mask = mask;
                         }
                         cons_bar();
-                        if (*last_flag) {
+                        const uint32_t mask = *last_mask;
+                        if (mask) {
                             __threadfence();
-                            const int row = s.tile * 2 * kBoxRows + threadIdx.x;
-                            if (row < p.h) {
-#pragma unroll 4
-                                for (int tok = 0; tok < p.t; ++tok) {
-                                    float y = 0.0f;
-                                    for (int k = 0; k < p.top; ++k) {
-                                        const int pair = tok * p.top + k;
-                                        if (tb.pair_e[pair] >= 0)
-                                            y = fmaf(tb.pair_w[pair],
-                                                     __ldcg(p.pair_out + static_cast<long long>(pair) * p.h + row), y);
-                                    }
-                                    store_dense(p.out, p.type, tok * p.ldo + row, y);
-                                }
-                            }
+                            combine(p, tb, s.g0, mask, splits, warp, lane);
                         }
-                        cons_bar();  // last_flag is free again
+                        cons_bar();  // last_mask is free again
                     }
                 }
-                if (phase == 1 && ok) {
+                if (ok && phase == 1) {
                     asm volatile("fence.proxy.async.global;" ::: "memory");
                     cons_bar();
                     if (threadIdx.x == 0) grid_arrive(p.ctrl + kBarrier);
@@ -893,17 +1118,18 @@ __global__ void __launch_bounds__(kThreads, 1) moe_f8_kernel(const __grid_consta
         }
     }
     __syncthreads();
-    // the last CTA out returns the barrier words to zero
+    // the last CTA out returns the words to zero
     if (threadIdx.x == 0) {
         __threadfence();
-        if (atomicAdd(p.ctrl + kExit, 1u) == grid - 1) {
+        if (atomicAdd(p.ctrl + kExit, 1u) == static_cast<unsigned>(parts) - 1) {
+            p.ctrl[kTicket] = 0u;
             p.ctrl[kBarrier] = 0u;
             p.ctrl[kExit] = 0u;
         }
     }
 }
 
-// (k, rows, experts) map of an expert stack: box 128 bytes x 128 rows x 1.
+// (k, rows, experts) map of an expert stack: box 128 bytes x 16 rows x 1.
 bool make_expert_map(CUtensorMap* map, const MoeWeight& w, int k, int rows, int experts) {
     static PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
         cudaDriverEntryPointQueryResult q;
@@ -927,18 +1153,20 @@ int token_groups(int t) { return t <= 8 ? 1 : t <= 16 ? 2 : t <= 32 ? 4 : 8; }
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
+// Splits of k (at most 8) that the slots' partial rows have room for: 256 rows.
+int split_limit(int pairs) { return std::max(1, std::min(8, 256 / pairs)); }
+
 // Scratch areas in order, after the zeroed header.
 struct MoeScratch {
-    size_t logits, xq, hq, part, pair_out, total;
+    size_t logits, xq, hq, pair_out, total;
     MoeScratch(int t, int h, int f, int e, int top, int type) {
         const size_t blk = type == kTypeF32 ? ActBlock<true>::kBytes : ActBlock<false>::kBytes;
         const size_t kb_h = (h + 127) / 128, kb_f = (f + 127) / 128, pairs = static_cast<size_t>(t) * top;
         logits = 0;
         xq = logits + up256(static_cast<size_t>(t) * e * 4);
         hq = xq + up256(t * kb_h * blk);
-        part = hq + up256(pairs * kb_f * blk);
-        pair_out = part + up256(static_cast<size_t>(sm_count()) * 2 * 8 * token_groups(t) * kConsThreads * 4);
-        total = pair_out + pairs * h * 4;
+        pair_out = hq + up256(pairs * kb_f * blk);
+        total = pair_out + pairs * split_limit(static_cast<int>(pairs)) * h * 4;
     }
 };
 
@@ -954,17 +1182,8 @@ int launch_cfg(const MoeParams& p, cudaStream_t s) {
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) attr_done[dev] = true;
     }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(sm_count()), 1, 1);
-    cfg.blockDim = dim3(kThreads, 1, 1);
-    cfg.dynamicSmemBytes = C::kBytes;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeCooperative;
-    attr[0].val.cooperative = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kern, p);
+    kern<<<sm_count(), kThreads, C::kBytes, s>>>(p);
+    return cudaGetLastError();
 }
 
 }  // namespace
@@ -1004,19 +1223,20 @@ int launch_moe_f8(const MoeF8& m, int* err, cudaStream_t s) {
     p.renorm = m.renorm;
     p.kb_h = (m.h + kF8Block - 1) / kF8Block;
     p.kb_f = (m.f + kF8Block - 1) / kF8Block;
-    p.tiles_f = p.kb_f;
-    p.tiles_h = (m.h + 2 * kBoxRows - 1) / (2 * kBoxRows);
-    // the line's length is an int and the header has a counter per column tile
-    const long long longest = std::max(static_cast<long long>(p.tiles_f) * p.kb_h, static_cast<long long>(p.tiles_h) * p.kb_f);
-    if (longest * std::min(m.t * m.top, kMaxPairs) > 0x7fffffffll ||
-        p.tiles_h > static_cast<int>(kF8Counters) - kCombine || sm_count() > kCut2 - kCut1)
+    p.max_split = split_limit(m.t * m.top);
+    const size_t es = m.type == kTypeF32 ? 4 : 2, rs = m.router_type == kTypeF32 ? 4 : 2;
+    p.wide = reinterpret_cast<uintptr_t>(m.x) % 16 == 0 && m.ldx * es % 16 == 0 &&
+             (!m.router || (reinterpret_cast<uintptr_t>(m.router) % 16 == 0 && m.ld_router * rs % 16 == 0));
+    // lines are ints and the header has a counter per 32 columns
+    if (sm_count() > kMaxParts || static_cast<long long>(m.f / kBoxRows + 1) * kMaxPairs > 0x7fffffffll ||
+        static_cast<long long>(m.h / 32 + 1) * kMaxPairs * 8 > 0x7fffffffll ||
+        (m.h + 31) / 32 > static_cast<int>(kF8Counters) - kCombine)
         return cudaErrorInvalidValue;
     uint8_t* base = static_cast<uint8_t*>(m.scratch);
     p.ctrl = m.counters;
     p.logits = reinterpret_cast<float*>(base + sc.logits);
     p.xq = base + sc.xq;
     p.hq = base + sc.hq;
-    p.part = reinterpret_cast<float*>(base + sc.part);
     p.pair_out = reinterpret_cast<float*>(base + sc.pair_out);
     p.err = err;
     const bool lo = m.type == kTypeF32;
