@@ -35,13 +35,12 @@
 // (exact but for bits 2^-39 below the block's largest value).
 //
 // The down product may also cut k (a part's groups then divide more evenly);
-// the parts of a sum and the slots of a token are added in a fixed order by
-// the CTA that finishes a group of columns last, so results do not depend on
-// who that is.
+// its sums go to memory per slot and cut, and are added in a fixed order at
+// the end, so results do not depend on who finishes when.
 //
 // Phases: (0) router products and the activations' layout; (1) every CTA
-// picks the experts for itself, gate / up products, SiLU; (2) down products,
-// weighted sum.  A CTA takes a part by ticket and does that part of every
+// picks the experts for itself, gate / up products, SiLU; (2) down products;
+// (3) weighted sums of the slots.  A CTA takes a part by ticket and does that part of every
 // phase.  One that waits long for the others in phase 0 takes further parts,
 // until all are held by CTAs that run, so the launch needs no co-residency (a
 // cooperative launch cost 16 us more per call).  The weight copies of phase 2
@@ -59,11 +58,9 @@
 namespace rk {
 namespace {
 
-constexpr int kConsumers = 8;                // warps
-constexpr int kConsThreads = kConsumers * 32;
-constexpr int kProducers = 4;                // warps
-constexpr int kThreads = kConsThreads + kProducers * 32;
-constexpr int kWarps = kThreads / 32;
+constexpr int kProducers = 4;    // warps that issue copies
+constexpr int kPassGroups = 8;   // groups of a pass, at most
+constexpr int kRouterWarps = 8;  // warps that share a router task
 constexpr int kBoxRows = 16;                 // rows of one TMA box, one MMA tile
 constexpr int kBoxBytes = kBoxRows * kF8Block;
 constexpr int kGroupBytes = 2 * kBoxBytes;   // gate and up, or two boxes of down rows
@@ -73,10 +70,10 @@ constexpr int kMaxParts = 512;               // CTAs of a launch
 constexpr uint64_t kHelpNs = 20000;          // wait for the others before taking a further part
 
 // Words of the zeroed header.
-constexpr int kTicket = 0, kBarrier = 32, kExit = 64, kCombine = 1024;
+constexpr int kTicket = 0, kExit = 32, kDone = 64;  // kDone + 32 i: parts of phase i done
 
 struct MoeParams {
-    CUtensorMap tm_gate, tm_up, tm_down;  // (k, rows, expert), box 128 B x 16 rows
+    CUtensorMap tm_gate, tm_up, tm_down;  // (k, rows, expert), boxes of 128 B x 16, 16 and 32 rows
     const float *gate_s, *up_s, *down_s;
     long long gate_ss, up_ss, down_ss;  // scales of one expert
     const void* x;
@@ -91,36 +88,38 @@ struct MoeParams {
     int wide;  // x and router rows can be read 16 bytes at a time
     unsigned* ctrl;
     float* logits;    // [t][e]
-    uint8_t* xq;      // [t][kb_h] activation blocks
-    uint8_t* hq;      // [pair][kb_f] activation blocks
+    uint8_t* xq;      // [kb_h][t] activation blocks
+    uint8_t* hq;      // [kb_f][pair] activation blocks, pairs in sorted order
     float* pair_out;  // [pair][max_split][h]
     int* err;
 };
 
 // An activation block of 128 values: f16 values (and remainders) in the
 // order of the MMA operands, then eight f32 powers of two, one per 16 values
-// (x: all the first one's).
+// (x: all the first one's).  Its size is an odd multiple of 64 bytes, so that
+// two rows' 64-byte reads fall into different banks of shared memory.
 template <bool LO>
 struct ActBlock {
     static constexpr int kScaleAt = LO ? 512 : 256;
-    static constexpr int kBytes = kScaleAt + 32;
-    // distance of two rows in shared memory: an odd multiple of 64 bytes, so
-    // that two rows' 64-byte reads fall into different banks
-    static constexpr int kPitch = LO ? 576 : 320;
+    static constexpr int kBytes = LO ? 576 : 320;
 };
-
-// Sums that warps exchange: 8 per thread.
-constexpr int kRedBytes = kConsThreads * 8 * 4;
 
 template <int NG, bool LO>
 struct MoeCfg {
     using Act = ActBlock<LO>;
-    static constexpr int kAct = (NG * 8 * Act::kPitch + 1023) / 1024 * 1024;
-    static constexpr int kStage = kConsumers * kGroupBytes + kAct;
-    static constexpr int kStages = (200 * 1024) / kStage;
+    static constexpr int kConsumers = 8;  // a group of a pass each; 16 with fewer registers were slower
+    static constexpr int kConsThreads = kConsumers * 32;
+    static constexpr int kWarps = kConsumers + kProducers;
+    static constexpr int kThreads = kWarps * 32;
+    // registers after the split: 256 x 224 + 128 x 56 of 384 x 168
+    static constexpr int kConsRegs = 224, kProdRegs = 56;
+    static constexpr int kAct = (NG * 8 * Act::kBytes + 1023) / 1024 * 1024;
+    static constexpr int kStage = kPassGroups * kGroupBytes + kAct;
+    static constexpr int kRedBytes = kConsThreads * 8 * 4;  // sums that warps exchange
+    static constexpr int kTableBytes = kRedBytes + kMaxPairs * (4 + 4 + 2 + 2) + kMoeMaxExperts * 4 + 16 + kMaxParts * 2;
+    static constexpr int kStages = (230000 - 2048 - kTableBytes) / kStage;
     static constexpr int kBarOffset = kStages * kStage;
     static constexpr int kTables = kBarOffset + (2 * kStages * 8 + 32 + 15) / 16 * 16;
-    static constexpr int kTableBytes = kMaxPairs * (4 + 4 + 2 + 2) + kMoeMaxExperts * 4 + 16 + kRedBytes + kMaxParts * 2;
     static constexpr int kBytes = kTables + kTableBytes + 1024;  // + alignment slack
     static_assert(kBytes <= 232448, "shared memory");
 };
@@ -133,7 +132,7 @@ struct Tables {
     int* entry;          // [entries] expert << 16 | first position in order
     int* count;          // [expert] pairs
     int* info;           // [0] entries, [1] positions
-    float* red;          // kRedBytes
+    float* red;          // MoeCfg::kRedBytes
 };
 
 __device__ __forceinline__ void fail(int* err, volatile uint32_t* abort, int code) {
@@ -171,9 +170,13 @@ __device__ __forceinline__ bool grid_wait_some(const unsigned* bar, unsigned nee
     return true;
 }
 
-__device__ __forceinline__ void cons_bar() { asm volatile("bar.sync 2, %0;" ::"n"(kConsThreads) : "memory"); }
+// Barrier of the N consumer threads; cons_any: whether any passed true.
+template <int N>
+__device__ __forceinline__ void cons_bar() {
+    asm volatile("bar.sync 2, %0;" ::"n"(N) : "memory");
+}
 
-// The same barrier; whether any consumer thread passed true.
+template <int N>
 __device__ __forceinline__ bool cons_any(bool v) {
     uint32_t r;
     asm volatile(
@@ -184,7 +187,7 @@ __device__ __forceinline__ bool cons_any(bool v) {
         " selp.u32 %0, 1, 0, q;\n"
         "}\n"
         : "=r"(r)
-        : "r"(v ? 1u : 0u), "n"(kConsThreads)
+        : "r"(v ? 1u : 0u), "n"(N)
         : "memory");
     return r != 0;
 }
@@ -257,7 +260,7 @@ __device__ __forceinline__ void layout_x(const MoeParams& p, int half, int halve
     // the two halves of a warp take the same steps
     for (int task = half; task - (lane >> 4) < p.t * p.kb_h; task += halves) {
         const bool live = task < p.t * p.kb_h;
-        const int tok = task / p.kb_h, k = (task - tok * p.kb_h) * kF8Block + l * 8;
+        const int tok = task / p.kb_h, kb = task - tok * p.kb_h, k = kb * kF8Block + l * 8;
         float v[8];
         if (live && p.wide && k < p.h) {  // h is a multiple of 16
             load_dense8(p.x, p.type, tok * p.ldx + k, v);
@@ -274,7 +277,7 @@ __device__ __forceinline__ void layout_x(const MoeParams& p, int half, int halve
         float inv;
         const float s = act_scale(__uint_as_float(m), inv);
         if (live) {
-            uint8_t* blk = p.xq + static_cast<long long>(task) * ActBlock<LO>::kBytes;
+            uint8_t* blk = p.xq + (static_cast<long long>(kb) * p.t + tok) * ActBlock<LO>::kBytes;
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) split_half2<LO>(v[2 * i] * inv, v[2 * i + 1] * inv, hi[i], lo[i]);
@@ -320,16 +323,16 @@ __device__ __forceinline__ void router_dot(const MoeParams& p, int ex, int tok0,
         for (int o = 16; o > 0; o >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
 }
 
-// Part `part` of the router products.  Few tasks: a CTA's consumer warps share
-// a task's k range; many: a warp each.
-__device__ __forceinline__ void router_products(const MoeParams& p, const Tables& tb, int part, int warp, int lane) {
+// Part `part` of the router products.  Few tasks: warps of a CTA share a
+// task's k range; many: a warp each.
+__device__ __forceinline__ void router_products(const MoeParams& p, const Tables& tb, int part, int warp, int warps, int lane) {
     const int groups = (p.t + kRouterTokens - 1) / kRouterTokens, tasks = p.e * groups;
     float s[kRouterTokens];
     if (tasks <= 2 * static_cast<int>(gridDim.x)) {
-        const int per = (p.h / 8 + kConsumers - 1) / kConsumers * 8;
+        const int per = (p.h / 8 + kRouterWarps - 1) / kRouterWarps * 8;
         for (int task = part; task < tasks; task += gridDim.x) {
             const int ex = task / groups, tok0 = (task - ex * groups) * kRouterTokens;
-            if (warp < kConsumers) {
+            if (warp < kRouterWarps) {
                 router_dot(p, ex, tok0, warp * per, min(p.h, (warp + 1) * per), lane, s);
                 if (lane == 0)
 #pragma unroll
@@ -339,13 +342,13 @@ __device__ __forceinline__ void router_products(const MoeParams& p, const Tables
             if (threadIdx.x < kRouterTokens && tok0 + static_cast<int>(threadIdx.x) < p.t) {
                 float sum = 0.0f;
 #pragma unroll
-                for (int w = 0; w < kConsumers; ++w) sum += tb.red[w * kRouterTokens + threadIdx.x];
+                for (int w = 0; w < kRouterWarps; ++w) sum += tb.red[w * kRouterTokens + threadIdx.x];
                 __stcg(p.logits + (tok0 + threadIdx.x) * p.e + ex, sum);
             }
             __syncthreads();
         }
     } else {
-        for (int task = part * kWarps + warp; task < tasks; task += gridDim.x * kWarps) {
+        for (int task = part * warps + warp; task < tasks; task += gridDim.x * warps) {
             const int ex = task / groups, tok0 = (task - ex * groups) * kRouterTokens;
             router_dot(p, ex, tok0, 0, p.h, lane, s);
             if (lane == 0)
@@ -431,11 +434,11 @@ __device__ __forceinline__ void choose(const MoeParams& p, const Tables& tb, int
 
 // Pairs sorted by expert (then token); experts with pairs become entries of
 // at most `cap` pairs each.
-__device__ __forceinline__ void build_tables(const MoeParams& p, const Tables& tb, int cap) {
+__device__ __forceinline__ void build_tables(const MoeParams& p, const Tables& tb, int cap, int threads) {
     // eight pairs per read; those behind the last are empty
     const int eights = (p.t * p.top + 7) / 8;
     const uint4* all = reinterpret_cast<const uint4*>(tb.pair_e);
-    for (int ex = threadIdx.x; ex < p.e; ex += kThreads) {
+    for (int ex = threadIdx.x; ex < p.e; ex += threads) {
         int n = 0;
 #pragma unroll 4
         for (int i = 0; i < eights; ++i) {
@@ -466,7 +469,7 @@ __device__ __forceinline__ void build_tables(const MoeParams& p, const Tables& t
         if (lane == 0) tb.info[0] = ents, tb.info[1] = pos;
     }
     __syncthreads();
-    for (int ex = threadIdx.x; ex < p.e; ex += kThreads) {
+    for (int ex = threadIdx.x; ex < p.e; ex += threads) {
         int at = tb.count[ex];
         if (at < 0) continue;
         for (int i = 0; i < eights; ++i) {
@@ -518,24 +521,40 @@ __device__ __forceinline__ int choose_splits(const MoeParams& p, int entries, in
     return best;
 }
 
-// Up to 8 groups of one entry and split.
+// Up to 8 consecutive groups of the line.  They share the blocks of k, and the
+// activation rows of all their entries (consecutive positions) fit a stage:
+// groups of several entries go together where k is not cut.
 struct Pass {
-    int entry, split, g0, n, k0, k1;
+    int u0, n, split, k0, k1;  // first group in the line
+    int pos0, npos;            // positions of its entries
 };
 
 struct Walk {
     int cur, end;
     __device__ __forceinline__ Walk(const Line& l, int part) : cur(l.start(part)), end(l.start(part + 1)) {}
-    __device__ __forceinline__ bool next(const Line& l, Pass& s) {
+    __device__ __forceinline__ bool next(const Line& l, const Tables& tb, int cap, Pass& s) {
         if (cur >= end) return false;
-        const int es = cur / l.groups;
-        s.g0 = cur - es * l.groups;
-        s.entry = es / l.splits;
-        s.split = es - s.entry * l.splits;
-        const int avail = min(l.groups - s.g0, end - cur), passes = (avail + kConsumers - 1) / kConsumers;
-        s.n = (avail + passes - 1) / passes;  // passes of about one size
+        const int es = cur / l.groups, entry = es / l.splits;
+        s.u0 = cur;
+        s.split = es - entry * l.splits;
         s.k0 = static_cast<int>(static_cast<long long>(s.split) * l.nkb / l.splits);
         s.k1 = static_cast<int>(static_cast<long long>(s.split + 1) * l.nkb / l.splits);
+        int n;
+        entry_pairs(tb, entry, cap, s.pos0, n);
+        s.npos = n;
+        int avail = min((es + 1) * l.groups, end) - cur;
+        if (l.splits == 1) {
+            // on into the next entries, up to 8 groups
+            for (int e = entry + 1; avail < kPassGroups && cur + avail < end; ++e) {
+                int first;
+                entry_pairs(tb, e, cap, first, n);
+                if (s.npos + n > cap) break;
+                s.npos += n;
+                avail = min((e + 1) * l.groups, end) - cur;
+            }
+        }
+        const int passes = (avail + kPassGroups - 1) / kPassGroups;
+        s.n = (avail + passes - 1) / passes;  // passes of about one size
         cur += s.n;
         return true;
     }
@@ -583,9 +602,9 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t v, __half2 s) {
 
 template <int NG, bool LO>
 struct Consumer {
+    using C = MoeCfg<NG, LO>;
     using Act = ActBlock<LO>;
-    static constexpr int kChains = LO ? 4 : 2;
-    // gate / up (or the two boxes of down rows) x token groups x fragment
+    // gate / up (or the two halves of 32 down rows) x token groups x fragment
     float acc[2][NG][4];
 
     __device__ __forceinline__ void clear() {
@@ -597,83 +616,76 @@ struct Consumer {
                 for (int i = 0; i < 4; ++i) acc[b][n][i] = 0.0f;
     }
 
-    // One block of 128: a group's 16 rows of both boxes times ng token groups.
-    // GROUPED: a scale per 16 values (thread t's two 16s are its own).
+    // One block of 128, 64 values (thread t's chunk c of 16) at a time: a
+    // group's 16 rows of both boxes times ng token groups.  at: byte of this
+    // lane's token's row behind act, per token group.
+    // GROUPED: a scale per 16 values (thread t's two chunks have their own).
     // PACKED (LO, at most 4 tokens): column 2c is token c's f16 values and
     // column 2c + 1 their remainders, in one MMA; unpack() adds them.
     template <bool GROUPED, bool PACKED>
-    __device__ __forceinline__ void block(const uint8_t* rows, const uint8_t* act, int lane, int ng, float s0, float s1) {
+    __device__ __forceinline__ void block(const uint8_t* rows, const uint8_t* act, const int (&at)[NG], int lane, int ng,
+                                          float s0, float s1) {
         const int g = lane >> 2, t = lane & 3;
-        uint32_t a[2][8][4];  // box, k step, fragment
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const uint8_t* row = rows + b * kBoxBytes + g * kF8Block;
+        for (int c = 0; c < 2; ++c) {
+            uint32_t a[2][4][4];  // box, k step, fragment
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int at = ((2 * t + c) ^ g) * 16;
-                const uint4 lo = *reinterpret_cast<const uint4*>(row + at);
-                const uint4 hi = *reinterpret_cast<const uint4*>(row + 8 * kF8Block + at);
+            for (int b = 0; b < 2; ++b) {
+                const uint8_t* row = rows + b * kBoxBytes + g * kF8Block + ((2 * t + c) ^ g) * 16;
+                const uint4 lo = *reinterpret_cast<const uint4*>(row);
+                const uint4 hi = *reinterpret_cast<const uint4*>(row + 8 * kF8Block);
                 const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    a[b][4 * c + i][0] = e4m3_to_half2(wl[i] & 0xFFFFu);
-                    a[b][4 * c + i][1] = e4m3_to_half2(wh[i] & 0xFFFFu);
-                    a[b][4 * c + i][2] = e4m3_to_half2(wl[i] >> 16);
-                    a[b][4 * c + i][3] = e4m3_to_half2(wh[i] >> 16);
+                    a[b][i][0] = e4m3_to_half2(wl[i] & 0xFFFFu);
+                    a[b][i][1] = e4m3_to_half2(wh[i] & 0xFFFFu);
+                    a[b][i][2] = e4m3_to_half2(wl[i] >> 16);
+                    a[b][i][3] = e4m3_to_half2(wh[i] >> 16);
                 }
             }
-        }
 #pragma unroll
-        for (int n = 0; n < NG; ++n) {
-            if (n >= (PACKED ? 1 : ng)) break;
-            const uint8_t* row = act + (PACKED ? g >> 1 : n * 8 + g) * Act::kPitch;
-            float xs;  // the block's power of two for column g
-            __half2 f[2];
-            if constexpr (GROUPED) {
-                const float2 s = *reinterpret_cast<const float2*>(row + Act::kScaleAt + t * 8);
-                xs = fmaxf(s.x, s.y);
-                xs = fmaxf(xs, __shfl_xor_sync(0xffffffffu, xs, 1));
-                xs = fmaxf(xs, __shfl_xor_sync(0xffffffffu, xs, 2));
-                const float inv = __uint_as_float((254u << 23) - __float_as_uint(xs));  // powers of two up to 2^114
-                f[0] = __float2half2_rn(s.x * inv);
-                f[1] = __float2half2_rn(s.y * inv);
-            } else {
-                xs = *reinterpret_cast<const float*>(row + Act::kScaleAt);
-            }
-            // independent accumulators: eight MMAs one behind the other would
-            // take longer than the block's copy
-            float d[2][kChains][4] = {};
+            for (int n = 0; n < NG; ++n) {
+                if (n >= (PACKED ? 1 : ng)) break;
+                const uint8_t* row = act + at[n];
+                float xs;  // the block's power of two for column g
+                __half2 f;
+                if constexpr (GROUPED) {
+                    const float2 s = *reinterpret_cast<const float2*>(row + Act::kScaleAt + t * 8);
+                    xs = fmaxf(s.x, s.y);
+                    xs = fmaxf(xs, __shfl_xor_sync(0xffffffffu, xs, 1));
+                    xs = fmaxf(xs, __shfl_xor_sync(0xffffffffu, xs, 2));
+                    // powers of two, at most 2^114
+                    f = __float2half2_rn((c ? s.y : s.x) * __uint_as_float((254u << 23) - __float_as_uint(xs)));
+                } else {
+                    xs = *reinterpret_cast<const float*>(row + Act::kScaleAt);
+                }
+                // two accumulators each: eight MMAs one behind the other would
+                // take longer than the block's copy
+                float d[2][2][4] = {};
 #pragma unroll
-            for (int part = 0; part < (LO && !PACKED ? 2 : 1); ++part)
+                for (int part = 0; part < (LO && !PACKED ? 2 : 1); ++part)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint4 v = *reinterpret_cast<const uint4*>(row + (PACKED ? g & 1 : part) * 256 + j * 64 + t * 16);
-                    if constexpr (GROUPED) {
-                        v.x = mul_half2(v.x, f[j >> 1]);
-                        v.y = mul_half2(v.y, f[j >> 1]);
-                        v.z = mul_half2(v.z, f[j >> 1]);
-                        v.w = mul_half2(v.w, f[j >> 1]);
+                    for (int j = 0; j < 2; ++j) {
+                        uint4 v = *reinterpret_cast<const uint4*>(row + (PACKED ? g & 1 : part) * 256 + (2 * c + j) * 64 + t * 16);
+                        if constexpr (GROUPED) {
+                            v.x = mul_half2(v.x, f);
+                            v.y = mul_half2(v.y, f);
+                            v.z = mul_half2(v.z, f);
+                            v.w = mul_half2(v.w, f);
+                        }
+                        mma_f16(d[0][0], a[0][2 * j], v.x, v.y);
+                        mma_f16(d[1][0], a[1][2 * j], v.x, v.y);
+                        mma_f16(d[0][1], a[0][2 * j + 1], v.z, v.w);
+                        mma_f16(d[1][1], a[1][2 * j + 1], v.z, v.w);
                     }
-                    const int c0 = (PACKED ? 2 * (j & 1) : 2 * part) % kChains, c1 = (c0 + 1) % kChains;
-                    mma_f16(d[0][c0], a[0][2 * j], v.x, v.y);
-                    mma_f16(d[1][c0], a[1][2 * j], v.x, v.y);
-                    mma_f16(d[0][c1], a[0][2 * j + 1], v.z, v.w);
-                    mma_f16(d[1][c1], a[1][2 * j + 1], v.z, v.w);
-                }
-#pragma unroll
-            for (int c = 1; c < kChains; ++c)
+                // columns 2t and 2t + 1
+                const float x0 = __shfl_sync(0xffffffffu, xs, 8 * t), x1 = __shfl_sync(0xffffffffu, xs, 8 * t + 4);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    d[0][0][i] += d[0][c][i];
-                    d[1][0][i] += d[1][c][i];
+                    const float x = (i & 1) ? x1 : x0;
+                    acc[0][n][i] = fmaf(d[0][0][i] + d[0][1][i], s0 * x, acc[0][n][i]);
+                    acc[1][n][i] = fmaf(d[1][0][i] + d[1][1][i], s1 * x, acc[1][n][i]);
                 }
-            // columns 2t and 2t + 1
-            const float x0 = __shfl_sync(0xffffffffu, xs, 8 * t), x1 = __shfl_sync(0xffffffffu, xs, 8 * t + 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = (i & 1) ? x1 : x0;
-                acc[0][n][i] = fmaf(d[0][0][i], s0 * x, acc[0][n][i]);
-                acc[1][n][i] = fmaf(d[1][0][i], s1 * x, acc[1][n][i]);
             }
         }
     }
@@ -702,14 +714,14 @@ struct Consumer {
                 mine[0] = make_float4(acc[0][n][0], acc[0][n][1], acc[0][n][2], acc[0][n][3]);
                 mine[32] = make_float4(acc[1][n][0], acc[1][n][1], acc[1][n][2], acc[1][n][3]);
             }
-            cons_bar();
+            cons_bar<C::kConsThreads>();
             if (warp < n2)
                 for (int w = 1; w < ways; ++w) {
                     const float4 u = mine[w * n2 * 64], v = mine[w * n2 * 64 + 32];
                     acc[0][n][0] += u.x, acc[0][n][1] += u.y, acc[0][n][2] += u.z, acc[0][n][3] += u.w;
                     acc[1][n][0] += v.x, acc[1][n][1] += v.y, acc[1][n][2] += v.z, acc[1][n][3] += v.w;
                 }
-            cons_bar();
+            cons_bar<C::kConsThreads>();
         }
     }
 
@@ -733,7 +745,7 @@ struct Consumer {
                 const float sc = act_scale(m, inv);
                 const int col = i * 8 + 2 * t + j;
                 if (col < n) {
-                    uint8_t* blk = p.hq + (static_cast<long long>(first + col) * p.kb_f + (group >> 3)) * Act::kBytes;
+                    uint8_t* blk = p.hq + (static_cast<long long>(group >> 3) * p.t * p.top + first + col) * Act::kBytes;
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         const float v = h[r] * inv;
@@ -784,57 +796,48 @@ struct Consumer {
     }
 };
 
-// The weighted sums of the columns of the groups in `mask` (bit i: group
-// g0 + i), a warp per group and token; slots and splits in order.
-__device__ __forceinline__ void combine(const MoeParams& p, const Tables& tb, int g0, uint32_t mask, int splits, int warp,
-                                        int lane) {
-    const int items = __popc(mask) * p.t;
-    for (int item = warp; item < items; item += kConsumers) {
-        const int nth = item / p.t, tok = item - nth * p.t;
-        const int row = (g0 + static_cast<int>(__fns(mask, 0, nth + 1))) * 32 + lane;
-        if (row >= p.h) continue;
-        float y = 0.0f;
-        if (splits == 1) {
+// The weighted sums of the slots, a warp per token and 128 columns; slots and
+// cuts of k in order.
+__device__ __forceinline__ void combine(const MoeParams& p, const Tables& tb, int splits, int warp, int warps, int lane) {
+    const int chunks = (p.h + 127) / 128, items = chunks * p.t;
+    for (int item = warp; item < items; item += warps) {
+        const int tok = item / chunks, col = (item - tok * chunks) * 128 + lane * 4;
+        if (col >= p.h) continue;  // h is a multiple of 16
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-            for (int k = 0; k < p.top; ++k) {
-                const int pair = tok * p.top + k;
-                const float w = tb.pair_e[pair] < 0 ? 0.0f : tb.pair_w[pair];
-                const float d = tb.pair_e[pair] < 0 ? 0.0f : __ldcg(p.pair_out + static_cast<long long>(pair) * p.h + row);
-                y = fmaf(w, d, y);
-            }
-        } else {
-            for (int k = 0; k < p.top; ++k) {
-                const int pair = tok * p.top + k;
-                if (tb.pair_e[pair] < 0) continue;
-                const float* from = p.pair_out + static_cast<long long>(pair) * splits * p.h + row;
-                float d[8];
-#pragma unroll
-                for (int s = 0; s < 8; ++s) d[s] = s < splits ? __ldcg(from + static_cast<long long>(s) * p.h) : 0.0f;
-                float sum = 0.0f;
-#pragma unroll
-                for (int s = 0; s < 8; ++s) sum += d[s];
-                y = fmaf(tb.pair_w[pair], sum, y);
-            }
+        for (int i = 0; i < p.top * splits; ++i) {
+            const int k = i / splits, pair = tok * p.top + k;
+            if (tb.pair_e[pair] < 0) continue;
+            const float w = tb.pair_w[pair];
+            const float4 d = __ldcg(reinterpret_cast<const float4*>(p.pair_out + (static_cast<long long>(pair) * splits + (i - k * splits)) * p.h + col));
+            y.x = fmaf(w, d.x, y.x);
+            y.y = fmaf(w, d.y, y.y);
+            y.z = fmaf(w, d.z, y.z);
+            y.w = fmaf(w, d.w, y.w);
         }
-        store_dense(p.out, p.type, tok * p.ldo + row, y);
+        const long long o = tok * p.ldo + col;
+        store_dense(p.out, p.type, o, y.x);
+        store_dense(p.out, p.type, o + 1, y.y);
+        store_dense(p.out, p.type, o + 2, y.z);
+        store_dense(p.out, p.type, o + 3, y.w);
     }
 }
 
 template <int NG, bool LO>
-__global__ void __launch_bounds__(kThreads, 1) moe_f8_kernel(const __grid_constant__ MoeParams p) {
+__global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(const __grid_constant__ MoeParams p) {
     using C = MoeCfg<NG, LO>;
     using Act = ActBlock<LO>;
     constexpr int S = C::kStages, kCap = NG * 8;
+    constexpr int kConsumers = C::kConsumers, kConsThreads = C::kConsThreads, kThreads = C::kThreads, kWarps = C::kWarps;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOffset);
     uint64_t* empty = full + S;
     volatile uint32_t* abort = reinterpret_cast<uint32_t*>(empty + S);
-    volatile uint32_t* last_mask = abort + 1;
     volatile int* ticket = reinterpret_cast<int*>(empty + S) + 2;
     Tables tb;
     tb.red = reinterpret_cast<float*>(smem + C::kTables);
-    tb.pair_w = tb.red + kRedBytes / 4;
+    tb.pair_w = tb.red + C::kRedBytes / 4;
     tb.entry = reinterpret_cast<int*>(tb.pair_w + kMaxPairs);
     tb.count = tb.entry + kMaxPairs;
     tb.info = tb.count + kMoeMaxExperts;
@@ -865,7 +868,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_f8_kernel(const __grid_consta
         const int part = *ticket;
         if (part < parts) {
             layout_x<LO>(p, (part * kWarps + warp) * 2 + (lane >> 4), parts * kWarps * 2, lane);
-            if (p.router) router_products(p, tb, part, warp, lane);
+            if (p.router) router_products(p, tb, part, warp, kWarps, lane);
             asm volatile("fence.proxy.async.global;" ::: "memory");
             if (threadIdx.x == 0) held[nheld] = static_cast<short>(part);
             ++nheld;
@@ -874,13 +877,13 @@ __global__ void __launch_bounds__(kThreads, 1) moe_f8_kernel(const __grid_consta
         bool here = false;
         if (threadIdx.x == 0) {
             if (part < parts) {
-                grid_arrive(p.ctrl + kBarrier);
-                here = grid_wait_some(p.ctrl + kBarrier, parts, kHelpNs);
+                grid_arrive(p.ctrl + kDone);
+                here = grid_wait_some(p.ctrl + kDone, parts, kHelpNs);
                 if (!here) *ticket = static_cast<int>(atomicAdd(p.ctrl + kTicket, 1u));
             } else {
                 // every part is held by a CTA that runs
                 here = true;
-                if (!grid_wait(p.ctrl + kBarrier, parts, abort)) fail(p.err, abort, kErrTimeoutGrid);
+                if (!grid_wait(p.ctrl + kDone, parts, abort)) fail(p.err, abort, kErrTimeoutGrid);
             }
         }
         ready = __syncthreads_or(here);
@@ -910,7 +913,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_f8_kernel(const __grid_consta
         // pairs are read eight at a time
         for (int i = p.t * p.top + threadIdx.x; i < (p.t * p.top + 7) / 8 * 8; i += kThreads) tb.pair_e[i] = -1;
         __syncthreads();
-        build_tables(p, tb, kCap);
+        build_tables(p, tb, kCap, kThreads);
         const int entries = tb.info[0];
         const int groups1 = p.f / kBoxRows, groups2 = (p.h + 31) / 32;
         const int splits = choose_splits(p, entries, groups2);
@@ -918,86 +921,108 @@ __global__ void __launch_bounds__(kThreads, 1) moe_f8_kernel(const __grid_consta
         const Line line2{groups2, splits, p.kb_f, entries * groups2 * splits};
 
         if (warp >= kConsumers) {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-            // ---- producers: three threads for the weights, each every third box of
-            // a stage, and a warp for the activations (an issued copy costs its
-            // thread about 150 cycles; one thread for all took longer over a stage
-            // than the copies themselves) ----
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kProdRegs));
+            // ---- producers.  Phase 1: each of four warps issues every fourth box (one
+            // thread) and every fourth token row (a lane each) of a stage; an issued
+            // copy costs its thread 100 to 150 cycles, and one thread for all took
+            // longer over a stage than the copies.  Phase 2: three issue the weights,
+            // up to S stages ahead of the wait for phase 1, the fourth the hidden
+            // values, one copy per stage. ----
             const int pw = warp - kConsumers;
             asm volatile("fence.proxy.async.global;" ::: "memory");
             int g = 0;  // stages issued
             bool ok = true;
+            // lane 0 waits for the next stage; all learn
             auto stage_free = [&] {
-                if (g >= S && !wait_or_abort(&empty[g % S], ((g / S) & 1) ^ 1, abort)) {
+                if (lane == 0 && g >= S && !wait_or_abort(&empty[g % S], ((g / S) & 1) ^ 1, abort)) {
                     if (!*abort) fail(p.err, abort, kErrTimeoutEmpty);
                     ok = false;
                 }
+                ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
                 return ok;
             };
-            if (pw < kProducers - 1) {
-                if (lane == 0) {
-                    for (int step = 0; ok && step < 2 * nheld; ++step) {
-                        const int phase = step < nheld ? 1 : 2;
-                        const Line& line = phase == 1 ? line1 : line2;
-                        Walk walk(line, held[phase == 1 ? step : step - nheld]);
-                        Pass s;
-                        while (ok && walk.next(line, s)) {
-                            const int ex = tb.entry[s.entry] >> 16, boxes = 2 * s.n;
-                            const uint32_t bytes = (boxes - pw + kProducers - 2) / (kProducers - 1) * kBoxBytes;
-                            for (int kb = s.k0; kb < s.k1 && stage_free(); ++kb, ++g) {
-                                uint64_t* bar = &full[g % S];
-                                uint8_t* dst = smem + g % S * C::kStage;
-                                mbar_arrive_expect_tx(bar, bytes);
-                                for (int i = pw; i < boxes; i += kProducers - 1) {
-                                    const int grp = s.g0 + (i >> 1), box = i & 1;
-                                    if (phase == 1)
-                                        tma_load_3d(dst + i * kBoxBytes, box ? &p.tm_up : &p.tm_gate, bar,
-                                                    kb * kF8Block, grp * kBoxRows, ex);
-                                    else
-                                        tma_load_3d(dst + i * kBoxBytes, &p.tm_down, bar, kb * kF8Block,
-                                                    grp * 32 + box * kBoxRows, ex);
-                                }
+            Pass s;
+            for (int i = 0; ok && i < nheld; ++i) {
+                Walk walk(line1, held[i]);
+                while (ok && walk.next(line1, tb, kCap, s)) {
+                    // few tokens: all of them, in one copy
+                    const bool all = p.t <= 8;
+                    const int rows = all ? (pw == 0 ? p.t : 0) : max(0, s.npos - pw + kProducers - 1) / kProducers;
+                    const uint32_t bytes = (2 * s.n - pw + kProducers - 1) / kProducers * kBoxBytes + rows * Act::kBytes;
+                    const CUtensorMap* map = pw & 1 ? &p.tm_up : &p.tm_gate;  // box i: group i / 2, gate or up
+                    int ex[2 * kPassGroups / kProducers], row[2 * kPassGroups / kProducers];
+#pragma unroll
+                    for (int j = 0; j < 2 * kPassGroups / kProducers; ++j) {
+                        const int u = min(s.u0 + (pw + j * kProducers) / 2, line1.total - 1), entry = u / line1.groups;
+                        ex[j] = tb.entry[entry] >> 16;
+                        row[j] = (u - entry * line1.groups) * kBoxRows;
+                    }
+                    // this lane's token rows
+                    constexpr int kRows = (kCap + 127) / 128;
+                    int from[kRows];
+#pragma unroll
+                    for (int r = 0; r < kRows; ++r)
+                        from[r] = tb.order[s.pos0 + min(pw + kProducers * (lane + 32 * r), s.npos - 1)] / p.top * Act::kBytes;
+                    for (int kb = s.k0; kb < s.k1 && stage_free(); ++kb, ++g) {
+                        uint64_t* bar = &full[g % S];
+                        uint8_t* dst = smem + g % S * C::kStage;
+                        uint8_t* act = dst + kPassGroups * kGroupBytes;
+                        const uint8_t* src = p.xq + static_cast<long long>(kb) * p.t * Act::kBytes;
+                        if (lane == 0) {
+                            mbar_arrive_expect_tx(bar, bytes);
+#pragma unroll
+                            for (int j = 0; j < 2 * kPassGroups / kProducers; ++j)
+                                if (pw + j * kProducers < 2 * s.n)
+                                    tma_load_3d(dst + (pw + j * kProducers) * kBoxBytes, map, bar, kb * kF8Block, row[j], ex[j]);
+                            if (all && pw == 0) bulk_load(act, src, p.t * Act::kBytes, bar);
+                        }
+                        __syncwarp();
+                        if (!all) {
+#pragma unroll
+                            for (int r = 0; r < kRows; ++r) {
+                                const int i = pw + kProducers * (lane + 32 * r);
+                                if (i < s.npos) bulk_load(act + i * Act::kBytes, src + from[r], Act::kBytes, bar);
                             }
                         }
                     }
                 }
-            } else {
-                for (int step = 0; ok && step < 2 * nheld; ++step) {
-                    const int phase = step < nheld ? 1 : 2;
-                    const Line& line = phase == 1 ? line1 : line2;
-                    Walk walk(line, held[phase == 1 ? step : step - nheld]);
-                    if (step == nheld) {
-                        // the hidden values of all CTAs; the other producers' weights
-                        // are on their way meanwhile
-                        if (!grid_wait(p.ctrl + kBarrier, 2 * parts, abort)) {
-                            if (lane == 0 && !*abort) fail(p.err, abort, kErrTimeoutGrid);
-                            ok = false;
-                        }
-                        asm volatile("fence.proxy.async.global;" ::: "memory");
-                        ok = __all_sync(0xffffffffu, ok);
+            }
+            if (ok && pw == kProducers - 1) {
+                if (!grid_wait(p.ctrl + kDone + 32, parts, abort)) {
+                    if (lane == 0 && !*abort) fail(p.err, abort, kErrTimeoutGrid);
+                    ok = false;
+                }
+                asm volatile("fence.proxy.async.global;" ::: "memory");
+                ok = __all_sync(0xffffffffu, ok);
+            }
+            for (int i = 0; ok && i < nheld; ++i) {
+                Walk walk(line2, held[i]);
+                while (ok && walk.next(line2, tb, kCap, s)) {
+                    constexpr int kEach = (kPassGroups + kProducers - 2) / (kProducers - 1);
+                    const uint32_t bytes = max(0, s.n - pw + kProducers - 2) / (kProducers - 1) * kGroupBytes;
+                    int ex[kEach], row[kEach];
+#pragma unroll
+                    for (int j = 0; j < kEach; ++j) {
+                        const int u = min(s.u0 + pw + j * (kProducers - 1), line2.total - 1), es = u / line2.groups;
+                        ex[j] = tb.entry[es / line2.splits] >> 16;
+                        row[j] = (u - es * line2.groups) * 32;
                     }
-                    Pass s;
-                    while (ok && walk.next(line, s)) {
-                        int first, n;
-                        entry_pairs(tb, s.entry, kCap, first, n);
-                        // this lane's rows (the second with more than 32 tokens)
-                        const uint8_t* src[2];
+                    for (int kb = s.k0; kb < s.k1 && stage_free(); ++kb, ++g) {
+                        uint64_t* bar = &full[g % S];
+                        uint8_t* dst = smem + g % S * C::kStage;
+                        if (lane != 0) continue;
+                        if (pw == kProducers - 1) {
+                            mbar_arrive_expect_tx(bar, s.npos * Act::kBytes);
+                            bulk_load(dst + kPassGroups * kGroupBytes,
+                                      p.hq + (static_cast<long long>(kb) * p.t * p.top + s.pos0) * Act::kBytes,
+                                      s.npos * Act::kBytes, bar);
+                        } else {
+                            mbar_arrive_expect_tx(bar, bytes);
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            const int i = min(lane + 32 * r, n - 1);
-                            src[r] = phase == 1 ? p.xq + static_cast<long long>(tb.order[first + i] / p.top) * p.kb_h * Act::kBytes
-                                                : p.hq + static_cast<long long>(first + i) * p.kb_f * Act::kBytes;
-                        }
-                        for (int kb = s.k0; kb < s.k1; ++kb, ++g) {
-                            if (lane == 0 && stage_free()) mbar_arrive_expect_tx(&full[g % S], n * Act::kBytes);
-                            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-                            if (!ok) break;
-                            uint8_t* dst = smem + g % S * C::kStage + kConsumers * kGroupBytes;
-#pragma unroll
-                            for (int r = 0; r < 2; ++r)
-                                if (lane + 32 * r < n)
-                                    bulk_load(dst + (lane + 32 * r) * Act::kPitch, src[r] + kb * Act::kBytes, Act::kBytes,
-                                              &full[g % S]);
+                            for (int j = 0; j < kEach; ++j)
+                                if (pw + j * (kProducers - 1) < s.n)
+                                    tma_load_3d(dst + (pw + j * (kProducers - 1)) * kGroupBytes, &p.tm_down, bar,
+                                                kb * kF8Block, row[j], ex[j]);
                         }
                     }
                 }
@@ -1012,7 +1037,7 @@ __global__ void __launch_bounds__(kThreads, 1) moe_f8_kernel(const __grid_consta
                     }
             __syncwarp();
         } else {
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kConsRegs));
             // ---- consumer warps ----
             Consumer<NG, LO> c;
             int stage = 0;
@@ -1020,29 +1045,33 @@ __global__ void __launch_bounds__(kThreads, 1) moe_f8_kernel(const __grid_consta
             for (int step = 0; ok && step < 2 * nheld; ++step) {
                 const int phase = step < nheld ? 1 : 2, part = held[step < nheld ? step : step - nheld];
                 const Line& line = phase == 1 ? line1 : line2;
-                if (entries == 0 && phase == 2) {
-                    // no slot names an expert: the sums are empty
-                    for (long long i = part * kConsThreads + threadIdx.x; i < static_cast<long long>(p.t) * p.h;
-                         i += parts * kConsThreads)
-                        store_dense(p.out, p.type, i / p.h * p.ldo + i % p.h, 0.0f);
-                }
                 Walk walk(line, part);
                 Pass s;
-                while (ok && walk.next(line, s)) {
-                    int first, n;
-                    entry_pairs(tb, s.entry, kCap, first, n);
-                    const int ng = (n + 7) / 8, ex = tb.entry[s.entry] >> 16;
+                while (ok && walk.next(line, tb, kCap, s)) {
                     // n2 warps with a group each, `ways` of them sharing its blocks
                     const int n2 = s.n > 4 ? 8 : s.n > 2 ? 4 : s.n, ways = kConsumers / n2;
                     const int gi = warp & (n2 - 1), way = warp / n2;
-                    const bool mine = gi < s.n, packed = n <= 4;
-                    const int group = s.g0 + (mine ? gi : 0);
+                    const bool mine = gi < s.n;
+                    const int es = (s.u0 + (mine ? gi : 0)) / line.groups, entry = es / line.splits;
+                    const int group = s.u0 + (mine ? gi : 0) - es * line.groups;
+                    int first, n;
+                    entry_pairs(tb, entry, kCap, first, n);
+                    const int ng = (n + 7) / 8, ex = tb.entry[entry] >> 16;
+                    const bool packed = n <= 4;
                     const float *s0, *s1;
                     if (phase == 1) {
                         s0 = p.gate_s + ex * p.gate_ss + static_cast<long long>(group >> 3) * p.kb_h;
                         s1 = p.up_s + ex * p.up_ss + static_cast<long long>(group >> 3) * p.kb_h;
                     } else {
                         s0 = s1 = p.down_s + ex * p.down_ss + static_cast<long long>(group >> 2) * p.kb_f;
+                    }
+                    // this lane's token's row: its own place, or the token's among all
+                    int row_at[NG];
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) {
+                        // columns behind the last token repeat it; nothing of them is kept
+                        const int col = min(LO && NG == 1 && packed ? lane >> 3 : i * 8 + (lane >> 2), n - 1);
+                        row_at[i] = (phase == 1 && p.t <= 8 ? tb.order[first + col] / p.top : first - s.pos0 + col) * Act::kBytes;
                     }
                     c.clear();
                     float w0 = __ldg(s0 + min(s.k0 + way, s.k1 - 1)), w1 = __ldg(s1 + min(s.k0 + way, s.k1 - 1));
@@ -1058,16 +1087,16 @@ __global__ void __launch_bounds__(kThreads, 1) moe_f8_kernel(const __grid_consta
                             const int nk = min(kb + ways, s.k1 - 1);
                             const float n0 = __ldg(s0 + nk), n1 = __ldg(s1 + nk);
                             const uint8_t* at = smem + st * C::kStage;
-                            const uint8_t *rows = at + gi * kGroupBytes, *act = at + kConsumers * kGroupBytes;
+                            const uint8_t *rows = at + gi * kGroupBytes, *act = at + kPassGroups * kGroupBytes;
                             if (LO && NG == 1 && packed) {
                                 if (phase == 1)
-                                    c.template block<false, true>(rows, act, lane, ng, w0, w1);
+                                    c.template block<false, true>(rows, act, row_at, lane, ng, w0, w1);
                                 else
-                                    c.template block<true, true>(rows, act, lane, ng, w0, w1);
+                                    c.template block<true, true>(rows, act, row_at, lane, ng, w0, w1);
                             } else if (phase == 1) {
-                                c.template block<false, false>(rows, act, lane, ng, w0, w1);
+                                c.template block<false, false>(rows, act, row_at, lane, ng, w0, w1);
                             } else {
-                                c.template block<true, false>(rows, act, lane, ng, w0, w1);
+                                c.template block<true, false>(rows, act, row_at, lane, ng, w0, w1);
                             }
                             w0 = n0;
                             w1 = n1;
@@ -1076,45 +1105,32 @@ __global__ void __launch_bounds__(kThreads, 1) moe_f8_kernel(const __grid_consta
                         if (lane == 0) mbar_arrive(&empty[st]);
                     }
                     // one decision for all consumer warps
-                    if (cons_any(!ok)) {
+                    if (cons_any<kConsThreads>(!ok)) {
                         ok = false;
                         break;
                     }
                     if (LO && NG == 1 && packed) c.unpack(lane);
-                    if (ways > 1) c.reduce(tb.red, warp, lane, ng, n2, ways);
+                    if (ways > 1) c.reduce(tb.red, warp, lane, (min(s.npos, kCap) + 7) / 8, n2, ways);
                     const bool owner = mine && way == 0;
                     if (phase == 1) {
                         if (owner) c.hidden(p, group, first, n, ng, lane);
                     } else {
                         if (owner) c.slot_rows(p, tb, group, s.split, splits, first, n, ng, lane);
-                        // the last to add to 32 columns sums them
-                        __threadfence();
-                        cons_bar();
-                        if (warp == 0) {
-                            bool last = false;
-                            if (lane < s.n) {
-                                unsigned* cnt = p.ctrl + kCombine + s.g0 + lane;
-                                last = atomicAdd(cnt, 1u) == static_cast<unsigned>(entries * splits - 1);
-                                if (last) *cnt = 0u;
-                            }
-                            const uint32_t mask = __ballot_sync(0xffffffffu, last);
-                            if (lane == 0) *last_mask = mask;
-                        }
-                        cons_bar();
-                        const uint32_t mask = *last_mask;
-                        if (mask) {
-                            __threadfence();
-                            combine(p, tb, s.g0, mask, splits, warp, lane);
-                        }
-                        cons_bar();  // last_mask is free again
                     }
                 }
-                if (ok && phase == 1) {
+                if (ok) {
                     asm volatile("fence.proxy.async.global;" ::: "memory");
-                    cons_bar();
-                    if (threadIdx.x == 0) grid_arrive(p.ctrl + kBarrier);
+                    cons_bar<kConsThreads>();
+                    if (threadIdx.x == 0) grid_arrive(p.ctrl + kDone + 32 * phase);
                 }
             }
+            // ---- phase 3 ----
+            if (threadIdx.x == 0 && ok && !grid_wait(p.ctrl + kDone + 64, parts, abort)) {
+                if (!*abort) fail(p.err, abort, kErrTimeoutGrid);
+                ok = false;
+            }
+            if (!cons_any<kConsThreads>(!ok))
+                for (int i = 0; i < nheld; ++i) combine(p, tb, splits, held[i] * kConsumers + warp, parts * kConsumers, lane);
         }
     }
     __syncthreads();
@@ -1123,14 +1139,14 @@ __global__ void __launch_bounds__(kThreads, 1) moe_f8_kernel(const __grid_consta
         __threadfence();
         if (atomicAdd(p.ctrl + kExit, 1u) == static_cast<unsigned>(parts) - 1) {
             p.ctrl[kTicket] = 0u;
-            p.ctrl[kBarrier] = 0u;
             p.ctrl[kExit] = 0u;
+            for (int i = 0; i < 3; ++i) p.ctrl[kDone + 32 * i] = 0u;
         }
     }
 }
 
-// (k, rows, experts) map of an expert stack: box 128 bytes x 16 rows x 1.
-bool make_expert_map(CUtensorMap* map, const MoeWeight& w, int k, int rows, int experts) {
+// (k, rows, experts) map of an expert stack: box 128 bytes x box_rows x 1.
+bool make_expert_map(CUtensorMap* map, const MoeWeight& w, int k, int rows, int experts, unsigned box_rows) {
     static PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
         cudaDriverEntryPointQueryResult q;
         void* fn = nullptr;
@@ -1142,14 +1158,19 @@ bool make_expert_map(CUtensorMap* map, const MoeWeight& w, int k, int rows, int 
     if (!encode) return false;
     cuuint64_t dims[3] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(experts)};
     cuuint64_t strides[2] = {static_cast<cuuint64_t>(w.ld), static_cast<cuuint64_t>(w.stride)};
-    cuuint32_t box[3] = {kF8Block, kBoxRows, 1};
+    cuuint32_t box[3] = {kF8Block, box_rows, 1};
     cuuint32_t estr[3] = {1, 1, 1};
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(w.w), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int token_groups(int t) { return t <= 8 ? 1 : t <= 16 ? 2 : t <= 32 ? 4 : 8; }
+// Token groups of 8 per expert and entry: twice the mean number of tokens per
+// expert, at most all.  An expert with more is read twice.
+int token_groups(int t, int e, int top) {
+    const int cap = std::min(t, 2 * ((t * top + e - 1) / e));
+    return cap <= 8 ? 1 : cap <= 16 ? 2 : cap <= 32 ? 4 : 8;
+}
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -1182,7 +1203,7 @@ int launch_cfg(const MoeParams& p, cudaStream_t s) {
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) attr_done[dev] = true;
     }
-    kern<<<sm_count(), kThreads, C::kBytes, s>>>(p);
+    kern<<<sm_count(), C::kThreads, C::kBytes, s>>>(p);
     return cudaGetLastError();
 }
 
@@ -1196,8 +1217,9 @@ int launch_moe_f8(const MoeF8& m, int* err, cudaStream_t s) {
     MoeParams p{};
     const MoeScratch sc(m.t, m.h, m.f, m.e, m.top, m.type);
     if (m.scratch_bytes < sc.total) return cudaErrorInvalidValue;
-    if (!make_expert_map(&p.tm_gate, m.gate, m.h, m.f, m.e) || !make_expert_map(&p.tm_up, m.up, m.h, m.f, m.e) ||
-        !make_expert_map(&p.tm_down, m.down, m.f, m.h, m.e))
+    if (!make_expert_map(&p.tm_gate, m.gate, m.h, m.f, m.e, kBoxRows) ||
+        !make_expert_map(&p.tm_up, m.up, m.h, m.f, m.e, kBoxRows) ||
+        !make_expert_map(&p.tm_down, m.down, m.f, m.h, m.e, 2 * kBoxRows))
         return cudaErrorInvalidValue;
     p.gate_s = m.gate.scales;
     p.up_s = m.up.scales;
@@ -1227,10 +1249,9 @@ int launch_moe_f8(const MoeF8& m, int* err, cudaStream_t s) {
     const size_t es = m.type == kTypeF32 ? 4 : 2, rs = m.router_type == kTypeF32 ? 4 : 2;
     p.wide = reinterpret_cast<uintptr_t>(m.x) % 16 == 0 && m.ldx * es % 16 == 0 &&
              (!m.router || (reinterpret_cast<uintptr_t>(m.router) % 16 == 0 && m.ld_router * rs % 16 == 0));
-    // lines are ints and the header has a counter per 32 columns
+    // lines are ints
     if (sm_count() > kMaxParts || static_cast<long long>(m.f / kBoxRows + 1) * kMaxPairs > 0x7fffffffll ||
-        static_cast<long long>(m.h / 32 + 1) * kMaxPairs * 8 > 0x7fffffffll ||
-        (m.h + 31) / 32 > static_cast<int>(kF8Counters) - kCombine)
+        static_cast<long long>(m.h / 32 + 1) * kMaxPairs * 8 > 0x7fffffffll)
         return cudaErrorInvalidValue;
     uint8_t* base = static_cast<uint8_t*>(m.scratch);
     p.ctrl = m.counters;
@@ -1240,7 +1261,7 @@ int launch_moe_f8(const MoeF8& m, int* err, cudaStream_t s) {
     p.pair_out = reinterpret_cast<float*>(base + sc.pair_out);
     p.err = err;
     const bool lo = m.type == kTypeF32;
-    switch (token_groups(m.t)) {
+    switch (token_groups(m.t, m.e, m.top)) {
         case 1: return lo ? launch_cfg<1, true>(p, s) : launch_cfg<1, false>(p, s);
         case 2: return lo ? launch_cfg<2, true>(p, s) : launch_cfg<2, false>(p, s);
         case 4: return lo ? launch_cfg<4, true>(p, s) : launch_cfg<4, false>(p, s);
