@@ -103,6 +103,11 @@ bool dense_ok(uint32_t type, const void* p) {
     return size && p && reinterpret_cast<uintptr_t>(p) % size == 0;
 }
 
+// Quantised activations in a workspace: the rows, then their scales.
+size_t quantized_bytes(size_t m, size_t k) {
+    return round_up(m * round_up(k, 16), 256) + m * f8_blocks(k) * sizeof(float);
+}
+
 int launch_status(int e) {
     return e == cudaSuccess ? kOk : (e == cudaErrorInvalidValue ? kInvalid : kExecError);
 }
@@ -1851,20 +1856,19 @@ int rocknpu_b200_gemm_f8(const uint8_t* a_f8, size_t ld_a, const float* a_scales
 
 size_t rocknpu_b200_matmul_f8_workspace_bytes(size_t m, size_t n, size_t k) {
     if (!dim_ok(m) || !dim_ok(n) || !dim_ok(k)) return 0;
-    return round_up(rocknpu_b200_gemm_f8_workspace_bytes(m, n, k), 256) + round_up(m * round_up(k, 16), 256) +
-           m * f8_blocks(k) * sizeof(float);
+    return round_up(rocknpu_b200_gemm_f8_workspace_bytes(m, n, k), 256) + quantized_bytes(m, k);
 }
 
 int rocknpu_b200_matmul_f8(const void* a, uint32_t type, size_t lda, const uint8_t* w_f8, size_t ld_w,
                            const float* w_scales, void* out, uint32_t out_type, size_t ldo, size_t m, size_t k,
                            size_t n, void* workspace, size_t workspace_bytes, int* status, rocknpu_stream stream) {
     if (!dense_ok(type, a) || !workspace || !status || !dim_ok(m) || !dim_ok(k) || !dim_ok(n) || lda < k ||
-        reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
-        workspace_bytes < rocknpu_b200_matmul_f8_workspace_bytes(m, n, k))
+        reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
         return kInvalid;
     rk::GemmF8 g;
     if (!gemm_f8_args(&g, w_f8, ld_w, w_scales, out, out_type, ldo, m, k, n)) return kInvalid;
     const size_t head = round_up(rocknpu_b200_gemm_f8_workspace_bytes(m, n, k), 256), ld8 = round_up(k, 16);
+    if (workspace_bytes < head + quantized_bytes(m, k)) return kInvalid;
     uint8_t* a8 = static_cast<uint8_t*>(workspace) + head;
     float* as = reinterpret_cast<float*>(a8 + round_up(m * ld8, 256));
     g.a = a8;

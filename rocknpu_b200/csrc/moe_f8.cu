@@ -140,33 +140,34 @@ __device__ __forceinline__ void fail(int* err, volatile uint32_t* abort, int cod
     *abort = 1u;
 }
 
-__device__ __forceinline__ unsigned ld_acquire(const unsigned* p) {
+__device__ __forceinline__ unsigned ld_relaxed(const unsigned* p) {
     unsigned v;
-    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
     return v;
 }
 
 // All threads' earlier writes (ordered before by a CTA barrier) are visible
-// to whoever sees the count.
+// to whoever sees the count: the release is cumulative.
 __device__ __forceinline__ void grid_arrive(unsigned* bar) {
-    __threadfence();
     asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(bar) : "memory");
+}
+
+// Waits, for at most ns, until *bar >= need.
+__device__ __forceinline__ bool grid_wait_some(const unsigned* bar, unsigned need, uint64_t ns) {
+    const uint64_t t0 = globaltimer_ns();
+    while (ld_relaxed(bar) < need)
+        if (globaltimer_ns() - t0 > ns) return false;
+    asm volatile("fence.acq_rel.gpu;" ::: "memory");
+    return true;
 }
 
 __device__ __forceinline__ bool grid_wait(const unsigned* bar, unsigned need, volatile uint32_t* abort) {
     const uint64_t t0 = globaltimer_ns();
-    while (ld_acquire(bar) < need) {
+    while (ld_relaxed(bar) < need) {
         if (*abort) return false;
         if (globaltimer_ns() - t0 > kWaitLimitNs) return false;
     }
-    return true;
-}
-
-// As grid_wait, but for at most ns.
-__device__ __forceinline__ bool grid_wait_some(const unsigned* bar, unsigned need, uint64_t ns) {
-    const uint64_t t0 = globaltimer_ns();
-    while (ld_acquire(bar) < need)
-        if (globaltimer_ns() - t0 > ns) return false;
+    asm volatile("fence.acq_rel.gpu;" ::: "memory");
     return true;
 }
 
@@ -371,15 +372,20 @@ __device__ __forceinline__ uint32_t sort_key(float v) {
 // One token: its `top` largest logits, ties to the lower expert.  PER: experts
 // per lane.
 template <int PER>
-__device__ __forceinline__ void choose(const MoeParams& p, const Tables& tb, int tok, int lane) {
-    float v[PER];
+__device__ __forceinline__ void load_logits(const MoeParams& p, int tok, int lane, float (&v)[PER]) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+        v[j] = tok < p.t && lane + 32 * j < p.e ? __ldcg(p.logits + tok * p.e + lane + 32 * j) : -INFINITY;
+}
+
+template <int PER>
+__device__ __forceinline__ void choose(const MoeParams& p, const Tables& tb, int tok, int lane, const float (&v)[PER]) {
     uint32_t key[PER];
     float vmax = -INFINITY;
     bool finite = true;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const int ex = lane + 32 * j;
-        v[j] = ex < p.e ? __ldcg(p.logits + tok * p.e + ex) : -INFINITY;
         finite &= ex >= p.e || isfinite(v[j]);
         key[j] = ex < p.e ? sort_key(v[j]) : 0u;
         vmax = fmaxf(vmax, v[j]);
@@ -432,54 +438,59 @@ __device__ __forceinline__ void choose(const MoeParams& p, const Tables& tb, int
     }
 }
 
+// A warp's tokens, the next one's logits on their way meanwhile.
+template <int PER>
+__device__ __forceinline__ void choose_all(const MoeParams& p, const Tables& tb, int warp, int warps, int lane) {
+    float v[PER], next[PER];
+    load_logits<PER>(p, warp, lane, v);
+    for (int tok = warp; tok < p.t; tok += warps) {
+        load_logits<PER>(p, tok + warps, lane, next);
+        choose<PER>(p, tb, tok, lane, v);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) v[j] = next[j];
+    }
+}
+
 // Pairs sorted by expert (then token); experts with pairs become entries of
 // at most `cap` pairs each.
-__device__ __forceinline__ void build_tables(const MoeParams& p, const Tables& tb, int cap, int threads) {
-    // eight pairs per read; those behind the last are empty
-    const int eights = (p.t * p.top + 7) / 8;
-    const uint4* all = reinterpret_cast<const uint4*>(tb.pair_e);
-    for (int ex = threadIdx.x; ex < p.e; ex += threads) {
+__device__ __forceinline__ void build_tables(const MoeParams& p, const Tables& tb, int cap, int warp, int warps, int lane) {
+    // a warp per expert, 32 pairs at a time
+    const int pairs = p.t * p.top;
+    for (int ex = warp; ex < p.e; ex += warps) {
         int n = 0;
-#pragma unroll 4
-        for (int i = 0; i < eights; ++i) {
-            const uint4 v = all[i];
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) n += (static_cast<int>(w[j] & 0xFFFFu) == ex) + (static_cast<int>(w[j] >> 16) == ex);
-        }
-        tb.count[ex] = n;
+        for (int i = lane; i - lane < pairs; i += 32)
+            n += __popc(__ballot_sync(0xffffffffu, i < pairs && tb.pair_e[i] == ex));
+        if (lane == 0) tb.count[ex] = n;
     }
     __syncthreads();
-    if (threadIdx.x < 32) {
-        const int lane = threadIdx.x;
+    if (warp == 0) {
         int pos = 0, ents = 0;
         for (int e0 = 0; e0 < p.e; e0 += 32) {
             const int ex = e0 + lane, n = ex < p.e ? tb.count[ex] : 0, ne = (n + cap - 1) / cap;
-            int sp = n, se = ne;
+            int both = n | (ne << 16);  // pairs and entries before and with this expert
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int a = __shfl_up_sync(0xffffffffu, sp, o), b = __shfl_up_sync(0xffffffffu, se, o);
-                if (lane >= o) sp += a, se += b;
+                const int up = __shfl_up_sync(0xffffffffu, both, o);
+                if (lane >= o) both += up;
             }
-            for (int i = 0; i < ne; ++i) tb.entry[ents + se - ne + i] = (ex << 16) | (pos + sp - n + i * cap);
-            if (ex < p.e) tb.count[ex] = n ? pos + sp - n : -1;  // now the expert's first position
-            pos += __shfl_sync(0xffffffffu, sp, 31);
-            ents += __shfl_sync(0xffffffffu, se, 31);
+            const int first = pos + (both & 0xFFFF) - n, entry0 = ents + (both >> 16) - ne;
+            for (int i = 0; i < ne; ++i) tb.entry[entry0 + i] = (ex << 16) | (first + i * cap);
+            if (ex < p.e) tb.count[ex] = n ? first : -1;  // now the expert's first position
+            const int all = __shfl_sync(0xffffffffu, both, 31);
+            pos += all & 0xFFFF;
+            ents += all >> 16;
         }
         if (lane == 0) tb.info[0] = ents, tb.info[1] = pos;
     }
     __syncthreads();
-    for (int ex = threadIdx.x; ex < p.e; ex += threads) {
+    for (int ex = warp; ex < p.e; ex += warps) {
         int at = tb.count[ex];
         if (at < 0) continue;
-        for (int i = 0; i < eights; ++i) {
-            const uint4 v = all[i];
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (static_cast<int>(w[j] & 0xFFFFu) == ex) tb.order[at++] = static_cast<short>(8 * i + 2 * j);
-                if (static_cast<int>(w[j] >> 16) == ex) tb.order[at++] = static_cast<short>(8 * i + 2 * j + 1);
-            }
+        for (int i = lane; i - lane < pairs; i += 32) {
+            const bool hit = i < pairs && tb.pair_e[i] == ex;
+            const uint32_t hits = __ballot_sync(0xffffffffu, hit);
+            if (hit) tb.order[at + __popc(hits & ((1u << lane) - 1u))] = static_cast<short>(i);
+            at += __popc(hits);
         }
     }
     __syncthreads();
@@ -498,9 +509,13 @@ __device__ __forceinline__ void entry_pairs(const Tables& tb, int i, int cap, in
 
 struct Line {
     int groups, splits, nkb, total;  // groups per (entry, split), splits of k, blocks of k, groups in all
-    __device__ __forceinline__ int start(int part) const {
-        return static_cast<int>(static_cast<long long>(part) * total / static_cast<int>(gridDim.x));
+    int each, more;                  // groups per part, and those left over, spread over the parts
+    __device__ __forceinline__ Line(int entries, int groups_, int splits_, int nkb_)
+        : groups(groups_), splits(splits_), nkb(nkb_), total(entries * groups_ * splits_) {
+        each = static_cast<int>(static_cast<unsigned>(total) / gridDim.x);
+        more = total - each * static_cast<int>(gridDim.x);
     }
+    __device__ __forceinline__ int start(int part) const { return part * each + static_cast<int>(static_cast<unsigned>(part * more) / gridDim.x); }
 };
 
 // Splits of k for the down product: a part takes q = ceil(groups / parts)
@@ -509,10 +524,10 @@ struct Line {
 // five stages in flight have to cover the latency of memory.
 __device__ __forceinline__ int choose_splits(const MoeParams& p, int entries, int groups) {
     int best = 1;
-    long long least = 0x7fffffffffffffffll;
+    unsigned least = 0xffffffffu;
     for (int s = 1; s <= p.max_split && s <= p.kb_f; s *= 2) {
-        const long long q = (static_cast<long long>(entries) * groups * s + gridDim.x - 1) / gridDim.x;
-        const long long cost = max(q, 3ll) * ((p.kb_f + s - 1) / s);
+        const unsigned q = (static_cast<unsigned>(entries * groups * s) + gridDim.x - 1) / gridDim.x;
+        const unsigned cost = max(q, 3u) * (static_cast<unsigned>(p.kb_f + s - 1) / static_cast<unsigned>(s));
         if (cost < least) {
             least = cost;
             best = s;
@@ -537,8 +552,8 @@ struct Walk {
         const int es = cur / l.groups, entry = es / l.splits;
         s.u0 = cur;
         s.split = es - entry * l.splits;
-        s.k0 = static_cast<int>(static_cast<long long>(s.split) * l.nkb / l.splits);
-        s.k1 = static_cast<int>(static_cast<long long>(s.split + 1) * l.nkb / l.splits);
+        s.k0 = s.split * l.nkb / l.splits;
+        s.k1 = (s.split + 1) * l.nkb / l.splits;
         int n;
         entry_pairs(tb, entry, cap, s.pos0, n);
         s.npos = n;
@@ -577,7 +592,7 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -626,6 +641,29 @@ struct Consumer {
     __device__ __forceinline__ void block(const uint8_t* rows, const uint8_t* act, const int (&at)[NG], int lane, int ng,
                                           float s0, float s1) {
         const int g = lane >> 2, t = lane & 3;
+        // per token group: the power of two of columns 2t and 2t + 1 (times the
+        // weights' scales below), and what brings this lane's chunks to it
+        float x0[NG], x1[NG];
+        __half2 f[NG][2];
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+            if (n >= (PACKED ? 1 : ng)) break;
+            const uint8_t* row = act + at[n];
+            float xs;
+            if constexpr (GROUPED) {
+                const float2 s = *reinterpret_cast<const float2*>(row + Act::kScaleAt + t * 8);
+                xs = fmaxf(s.x, s.y);
+                xs = fmaxf(xs, __shfl_xor_sync(0xffffffffu, xs, 1));
+                xs = fmaxf(xs, __shfl_xor_sync(0xffffffffu, xs, 2));
+                const float inv = __uint_as_float((254u << 23) - __float_as_uint(xs));  // powers of two, at most 2^114
+                f[n][0] = __float2half2_rn(s.x * inv);
+                f[n][1] = __float2half2_rn(s.y * inv);
+            } else {
+                xs = *reinterpret_cast<const float*>(row + Act::kScaleAt);
+            }
+            x0[n] = __shfl_sync(0xffffffffu, xs, 8 * t);
+            x1[n] = __shfl_sync(0xffffffffu, xs, 8 * t + 4);
+        }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             uint32_t a[2][4][4];  // box, k step, fragment
@@ -647,18 +685,6 @@ struct Consumer {
             for (int n = 0; n < NG; ++n) {
                 if (n >= (PACKED ? 1 : ng)) break;
                 const uint8_t* row = act + at[n];
-                float xs;  // the block's power of two for column g
-                __half2 f;
-                if constexpr (GROUPED) {
-                    const float2 s = *reinterpret_cast<const float2*>(row + Act::kScaleAt + t * 8);
-                    xs = fmaxf(s.x, s.y);
-                    xs = fmaxf(xs, __shfl_xor_sync(0xffffffffu, xs, 1));
-                    xs = fmaxf(xs, __shfl_xor_sync(0xffffffffu, xs, 2));
-                    // powers of two, at most 2^114
-                    f = __float2half2_rn((c ? s.y : s.x) * __uint_as_float((254u << 23) - __float_as_uint(xs)));
-                } else {
-                    xs = *reinterpret_cast<const float*>(row + Act::kScaleAt);
-                }
                 // two accumulators each: eight MMAs one behind the other would
                 // take longer than the block's copy
                 float d[2][2][4] = {};
@@ -668,21 +694,19 @@ struct Consumer {
                     for (int j = 0; j < 2; ++j) {
                         uint4 v = *reinterpret_cast<const uint4*>(row + (PACKED ? g & 1 : part) * 256 + (2 * c + j) * 64 + t * 16);
                         if constexpr (GROUPED) {
-                            v.x = mul_half2(v.x, f);
-                            v.y = mul_half2(v.y, f);
-                            v.z = mul_half2(v.z, f);
-                            v.w = mul_half2(v.w, f);
+                            v.x = mul_half2(v.x, f[n][c]);
+                            v.y = mul_half2(v.y, f[n][c]);
+                            v.z = mul_half2(v.z, f[n][c]);
+                            v.w = mul_half2(v.w, f[n][c]);
                         }
                         mma_f16(d[0][0], a[0][2 * j], v.x, v.y);
                         mma_f16(d[1][0], a[1][2 * j], v.x, v.y);
                         mma_f16(d[0][1], a[0][2 * j + 1], v.z, v.w);
                         mma_f16(d[1][1], a[1][2 * j + 1], v.z, v.w);
                     }
-                // columns 2t and 2t + 1
-                const float x0 = __shfl_sync(0xffffffffu, xs, 8 * t), x1 = __shfl_sync(0xffffffffu, xs, 8 * t + 4);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float x = (i & 1) ? x1 : x0;
+                    const float x = (i & 1) ? x1[n] : x0[n];
                     acc[0][n][i] = fmaf(d[0][0][i] + d[0][1][i], s0 * x, acc[0][n][i]);
                     acc[1][n][i] = fmaf(d[1][0][i] + d[1][1][i], s1 * x, acc[1][n][i]);
                 }
@@ -797,23 +821,34 @@ struct Consumer {
 };
 
 // The weighted sums of the slots, a warp per token and 128 columns; slots and
-// cuts of k in order.
+// cuts of k in order, up to eight reads at a time.
 __device__ __forceinline__ void combine(const MoeParams& p, const Tables& tb, int splits, int warp, int warps, int lane) {
     const int chunks = (p.h + 127) / 128, items = chunks * p.t;
     for (int item = warp; item < items; item += warps) {
         const int tok = item / chunks, col = (item - tok * chunks) * 128 + lane * 4;
         if (col >= p.h) continue;  // h is a multiple of 16
         float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (int i = 0; i < p.top * splits; ++i) {
-            const int k = i / splits, pair = tok * p.top + k;
-            if (tb.pair_e[pair] < 0) continue;
-            const float w = tb.pair_w[pair];
-            const float4 d = __ldcg(reinterpret_cast<const float4*>(p.pair_out + (static_cast<long long>(pair) * splits + (i - k * splits)) * p.h + col));
-            y.x = fmaf(w, d.x, y.x);
-            y.y = fmaf(w, d.y, y.y);
-            y.z = fmaf(w, d.z, y.z);
-            y.w = fmaf(w, d.w, y.w);
+        const int terms = p.top * splits;
+        const float* from = p.pair_out + static_cast<long long>(tok) * terms * p.h + col;
+        for (int i0 = 0; i0 < terms; i0 += 8) {
+            float4 d[8];
+            float w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                // an empty slot's rows are whatever they were
+                const int pair = tok * p.top + min(i0 + i, terms - 1) / splits;
+                const bool live = i0 + i < terms && tb.pair_e[pair] >= 0;
+                w[i] = live ? tb.pair_w[pair] : 0.0f;
+                d[i] = live ? __ldcg(reinterpret_cast<const float4*>(from + static_cast<long long>(i0 + i) * p.h))
+                            : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                y.x = fmaf(w[i], d[i].x, y.x);
+                y.y = fmaf(w[i], d[i].y, y.y);
+                y.z = fmaf(w[i], d[i].z, y.z);
+                y.w = fmaf(w[i], d[i].w, y.w);
+            }
         }
         const long long o = tok * p.ldo + col;
         store_dense(p.out, p.type, o, y.x);
@@ -891,14 +926,10 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
     if (!__syncthreads_or(threadIdx.x == 0 && *abort != 0u)) {
         // ---- routing, by every CTA for itself ----
         if (p.router) {
-            for (int tok = warp; tok < p.t; tok += kWarps) {
-                if (p.e <= 32)
-                    choose<1>(p, tb, tok, lane);
-                else if (p.e <= 64)
-                    choose<2>(p, tb, tok, lane);
-                else
-                    choose<kMoeMaxExperts / 32>(p, tb, tok, lane);
-            }
+            if (p.e <= 64)
+                choose_all<2>(p, tb, warp, kWarps, lane);
+            else
+                choose_all<kMoeMaxExperts / 32>(p, tb, warp, kWarps, lane);
         } else {
             for (int i = threadIdx.x; i < p.t * p.top; i += kThreads) {
                 int ex = p.ids[i];
@@ -910,15 +941,13 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
                 tb.pair_w[i] = p.weights[i];
             }
         }
-        // pairs are read eight at a time
-        for (int i = p.t * p.top + threadIdx.x; i < (p.t * p.top + 7) / 8 * 8; i += kThreads) tb.pair_e[i] = -1;
         __syncthreads();
-        build_tables(p, tb, kCap, kThreads);
+        build_tables(p, tb, kCap, warp, kWarps, lane);
         const int entries = tb.info[0];
         const int groups1 = p.f / kBoxRows, groups2 = (p.h + 31) / 32;
         const int splits = choose_splits(p, entries, groups2);
-        const Line line1{groups1, 1, p.kb_h, entries * groups1};
-        const Line line2{groups2, splits, p.kb_f, entries * groups2 * splits};
+        const Line line1(entries, groups1, 1, p.kb_h);
+        const Line line2(entries, groups2, splits, p.kb_f);
 
         if (warp >= kConsumers) {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kProdRegs));
@@ -988,8 +1017,8 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
                 }
             }
             if (ok && pw == kProducers - 1) {
-                if (!grid_wait(p.ctrl + kDone + 32, parts, abort)) {
-                    if (lane == 0 && !*abort) fail(p.err, abort, kErrTimeoutGrid);
+                if (lane == 0 && !grid_wait(p.ctrl + kDone + 32, parts, abort)) {
+                    if (!*abort) fail(p.err, abort, kErrTimeoutGrid);
                     ok = false;
                 }
                 asm volatile("fence.proxy.async.global;" ::: "memory");

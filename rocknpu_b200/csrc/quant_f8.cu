@@ -18,7 +18,7 @@ namespace {
 constexpr int kRowsThreads = 256;
 constexpr int kRowsUnroll = 2;  // blocks of 128 per half-warp and step
 template <class T>
-constexpr int kRowsCtas = sizeof(T) == 4 ? 4 : 5;  // per SM
+constexpr int kRowsCtas = 4;  // per SM (bf16 16384 x 8192: 4 107 us, 5 110, 6 123)
 
 __device__ __forceinline__ uint32_t half_warp_max(uint32_t v) {
 #pragma unroll
@@ -215,6 +215,60 @@ __global__ void __launch_bounds__(kPrepThreads, sizeof(T) == 4 ? 2 : 4) prep_f8_
 
 constexpr int kKqThreads = 1024;
 
+// The values of four superblocks (rows r0 .. r0 + 3 of one superblock column)
+// that a lane owns, 8 each, in dequant8's order.  The sub-blocks' scales and
+// mins of all four are decoded once per warp, a sub-block per lane (Q4_K,
+// Q5_K: 4 x 8; Q6_K: two of 4 x 16 per lane), and handed out by shuffles;
+// dequant8 decodes them in every lane.  The same values, one rounding each.
+template <int KIND>
+__device__ __forceinline__ void dequant4x8(const uint8_t* const (&blk)[4], const bool (&live)[4], int lane,
+                                           float (&v)[4][8]) {
+    if constexpr (KIND == kQ4K || KIND == kQ5K) {
+        const int g = lane >> 3, i4 = (lane & 7) * 4;
+        uint32_t q[4], h[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            q[p] = live[p] ? ld32(blk[p] + (KIND == kQ4K ? 16 : 48) + 32 * g + i4) : 0u;
+            h[p] = KIND == kQ5K && live[p] ? ld32(blk[p] + 16 + i4) : 0u;
+        }
+        // this lane's sub-block: j of superblock g
+        const uint8_t* b = g < 2 ? (g == 0 ? blk[0] : blk[1]) : (g == 2 ? blk[2] : blk[3]);
+        const bool on = g < 2 ? (g == 0 ? live[0] : live[1]) : (g == 2 ? live[2] : live[3]);
+        float dj = 0.0f, mj = 0.0f;
+        if (on) {
+            const uint32_t dd = ld32(b);
+            const uint32_t s[3] = {ld32(b + 4), ld32(b + 8), ld32(b + 12)};
+            int sc, mn;
+            scale_min_k4(lane & 7, s, sc, mn);
+            dj = __fmul_rn(half_bits_to_float(dd), static_cast<float>(sc));
+            mj = __fmul_rn(half_bits_to_float(dd >> 16), static_cast<float>(mn));
+        }
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const float d = __shfl_sync(0xffffffffu, dj, 8 * p + 2 * g + half);
+                const float m = __shfl_sync(0xffffffffu, mj, 8 * p + 2 * g + half);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t c = (q[p] >> (8 * i + 4 * half)) & 0x0Fu;
+                    if constexpr (KIND == kQ5K) c |= ((h[p] >> (8 * i + 2 * g + half)) & 1u) << 4;
+                    v[p][4 * half + i] = __fsub_rn(__fmul_rn(d, small_uint_to_float(c)), m);
+                }
+            }
+    } else {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            if (live[p]) {
+                dequant8<KIND>(blk[p], lane, [&](int slot, int, float x) { v[p][slot] = x; });
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[p][i] = 0.0f;
+            }
+        }
+    }
+}
+
 // K-quant superblocks: one CTA per 128 rows of one superblock column (two
 // 128 x 128 blocks).  A warp dequantises 4 superblocks, 8 values per lane;
 // lanes 0-15 own the first 128 values of a superblock, lanes 16-31 the rest.
@@ -226,21 +280,19 @@ __global__ void __launch_bounds__(kKqThreads) prep_f8_kq_kernel(const uint8_t* _
     __shared__ uint32_t red[2][kKqThreads / 32];
     const unsigned rb = blockIdx.x / sb, cb = blockIdx.x - rb * sb;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float v[4][8];
-    uint32_t m = 0;
+    const long long r0 = static_cast<long long>(rb) * kF8Block + warp * 4;
+    const uint8_t* blk[4];
+    bool live[4];
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-        const long long r = static_cast<long long>(rb) * kF8Block + warp * 4 + p;
-        if (r < n) {
-            dequant8<KIND>(blocks + (r * sb + cb) * kBytes, lane, [&](int slot, int, float x) {
-                v[p][slot] = x;
-                m = max(m, mag_bits(x));
-            });
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[p][i] = 0.0f;
-        }
+        live[p] = r0 + p < n;
+        blk[p] = blocks + ((r0 + p) * sb + cb) * kBytes;
     }
+    float v[4][8];
+    dequant4x8<KIND>(blk, live, lane, v);
+    uint32_t m = 0;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) m = max(m, mag_max(v[p]));
     m = half_warp_max(m);
     if (!mag_finite(m)) atomicExch(err, kErrNonFinite);
     static_assert(kKqThreads / 32 == 32, "two maxima per lane below");
@@ -252,9 +304,8 @@ __global__ void __launch_bounds__(kKqThreads) prep_f8_kq_kernel(const uint8_t* _
         scales[static_cast<long long>(rb) * 2 * sb + 2 * cb + (lane >> 4)] = s;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-        const long long r = static_cast<long long>(rb) * kF8Block + warp * 4 + p;
-        if (r >= n) continue;
-        uint8_t* dst = out + r * ld8 + cb * 256;
+        if (!live[p]) continue;
+        uint8_t* dst = out + (r0 + p) * ld8 + cb * 256;
         uint32_t code[2];
         f8_codes(v[p], s, code);
         if constexpr (KIND == kQ6K) {

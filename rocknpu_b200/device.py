@@ -188,12 +188,12 @@ def _status_ptr(status: torch.Tensor) -> int:
     return status.data_ptr()
 
 
-def _f8_empty(*shape, device) -> torch.Tensor:
-    """e4m3 tensor whose rows start at multiples of 16 bytes."""
+def _f8_empty(like: torch.Tensor, *shape) -> torch.Tensor:
+    """e4m3 tensor on `like`'s device whose rows start at multiples of 16 bytes."""
     k = shape[-1]
     if k % 16 == 0:
-        return torch.empty(shape, dtype=torch.float8_e4m3fn, device=device)
-    return torch.empty((*shape[:-1], (k + 15) // 16 * 16), dtype=torch.float8_e4m3fn, device=device)[..., :k]
+        return like.new_empty(shape, dtype=torch.float8_e4m3fn)
+    return like.new_empty((*shape[:-1], (k + 15) // 16 * 16), dtype=torch.float8_e4m3fn)[..., :k]
 
 
 def _dense_rows(t: torch.Tensor, what: str):
@@ -234,12 +234,12 @@ def _weight_scales(s: torch.Tensor, shape, what: str) -> None:
         raise ValueError(f"{what} scales are contiguous f32 {tuple(shape)}, one per 128 x 128 block")
 
 
-def _dense_out(out, m: int, n: int, dtype, device):
+def _dense_out(out, m: int, n: int, dtype, like: torch.Tensor):
     """(out, type id, row pitch), made when None."""
     if out is None:
         if dtype not in _TYPES:
             raise ValueError("results are f32, f16 or bf16")
-        return torch.empty((m, n), dtype=dtype, device=device), _TYPES[dtype], n
+        return like.new_empty((m, n), dtype=dtype), _TYPES[dtype], n
     rows, cols, ld, type_ = _dense_rows(out, "out")
     if rows != m or cols != n:
         raise ValueError(f"out has shape {(m, n)}")
@@ -252,9 +252,9 @@ def quantize_rows_f8(a: torch.Tensor, status: torch.Tensor, out: torch.Tensor | 
     dev = _device_of(a, status, out, scales)
     m, k, lda, type_ = _dense_rows(a, "a")
     if out is None:
-        out = _f8_empty(m, k, device=a.device)
+        out = _f8_empty(a, m, k)
     if scales is None:
-        scales = torch.empty((m, _f8_blocks(k)), dtype=torch.float32, device=a.device)
+        scales = a.new_empty((m, _f8_blocks(k)), dtype=torch.float32)
     rows, cols, ld8 = _f8_rows(out, "out")
     if rows != m or cols != k:
         raise ValueError("out has a's shape")
@@ -273,8 +273,8 @@ def prepare_f8(w: torch.Tensor, status: torch.Tensor, stream=None):
     count = w.shape[0] if w.dim() == 3 else 1
     if count > 1 and w.stride(0) != n * ldw:
         raise ValueError("a stack of weights has no gaps between them")
-    out = _f8_empty(*w.shape, device=w.device)
-    scales = torch.empty((*w.shape[:-2], _f8_blocks(n), _f8_blocks(k)), dtype=torch.float32, device=w.device)
+    out = _f8_empty(w, *w.shape)
+    scales = w.new_empty((*w.shape[:-2], _f8_blocks(n), _f8_blocks(k)), dtype=torch.float32)
     _launch("prepare_f8", dev, stream, type_, w.data_ptr(), n, k, ldw, count, out.data_ptr(), (k + 15) // 16 * 16,
             scales.data_ptr(), _status_ptr(status))
     return out, scales
@@ -287,8 +287,8 @@ def prepare_f8_q(kind: int, blocks: torch.Tensor, k: int, n: int, status: torch.
         raise ValueError("blocks are contiguous uint8")
     if kind not in BLOCK_BYTES or k <= 0 or n <= 0 or k % 256 or blocks.numel() < n * (k // 256) * BLOCK_BYTES[kind]:
         raise ValueError("blocks hold n rows of k / 256 superblocks")
-    out = torch.empty((n, k), dtype=torch.float8_e4m3fn, device=blocks.device)
-    scales = torch.empty((_f8_blocks(n), _f8_blocks(k)), dtype=torch.float32, device=blocks.device)
+    out = blocks.new_empty((n, k), dtype=torch.float8_e4m3fn)
+    scales = blocks.new_empty((_f8_blocks(n), _f8_blocks(k)), dtype=torch.float32)
     _launch("prepare_f8_q", dev, stream, kind, blocks.data_ptr(), k, n, out.data_ptr(), k, scales.data_ptr(),
             _status_ptr(status))
     return out, scales
@@ -313,7 +313,7 @@ def gemm_f8(a8: torch.Tensor, a_scales: torch.Tensor, w8: torch.Tensor, w_scales
     if kw != k:
         raise ValueError("w8 is [n, k]")
     _weight_scales(w_scales, (_f8_blocks(n), _f8_blocks(k)), "w8")
-    out, out_type, ldo = _dense_out(out, m, n, out_dtype, a8.device)
+    out, out_type, ldo = _dense_out(out, m, n, out_dtype, a8)
     _launch("gemm_f8", dev, stream, a8.data_ptr(), lda, a_scales.data_ptr(), _row_scales(a_scales, m, k, "a_scales"),
             w8.data_ptr(), ldw, w_scales.data_ptr(), out.data_ptr(), out_type, ldo, m, k, n,
             None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.nbytes,
@@ -333,7 +333,7 @@ def matmul_f8(a: torch.Tensor, w8: torch.Tensor, w_scales: torch.Tensor, status:
     if kw != k:
         raise ValueError("w8 is [n, k]")
     _weight_scales(w_scales, (_f8_blocks(n), _f8_blocks(k)), "w8")
-    out, out_type, ldo = _dense_out(out, m, n, out_dtype or a.dtype, a.device)
+    out, out_type, ldo = _dense_out(out, m, n, out_dtype or a.dtype, a)
     _launch("matmul_f8", dev, stream, a.data_ptr(), type_, lda, w8.data_ptr(), ldw, w_scales.data_ptr(),
             out.data_ptr(), out_type, ldo, m, k, n, workspace.data_ptr(), workspace.nbytes, _status_ptr(status))
     return out
@@ -386,8 +386,8 @@ def moe_f8(x: torch.Tensor, gate, up, down, status: torch.Tensor, workspace: tor
         rows, cols, ld_router, router_type = _dense_rows(router, "router")
         if rows != e or cols != h:
             raise ValueError("router is [experts, hidden]")
-        ids = torch.empty((t, top_k), dtype=torch.int32, device=x.device)
-        weights = torch.empty((t, top_k), dtype=torch.float32, device=x.device)
+        ids = x.new_empty((t, top_k), dtype=torch.int32)
+        weights = x.new_empty((t, top_k), dtype=torch.float32)
     else:
         ld_router = router_type = 0
         if ids is None or weights is None or ids.dim() != 2 or ids.shape[0] != t or ids.shape != weights.shape or \
@@ -397,7 +397,7 @@ def moe_f8(x: torch.Tensor, gate, up, down, status: torch.Tensor, workspace: tor
         if top_k is not None and top_k != ids.shape[1]:
             raise ValueError("ids and weights are [tokens, top_k]")
         top_k = ids.shape[1]
-    out, out_type, ldo = _dense_out(out, t, h, x.dtype, x.device)
+    out, out_type, ldo = _dense_out(out, t, h, x.dtype, x)
     if out_type != type_:
         raise ValueError("out has x's type")
     args = _MOE_ARGS.pack(t, h, f, e, top_k, type_, x.data_ptr(), out.data_ptr(), ldx, ldo,

@@ -311,3 +311,68 @@ def test_one_workspace_serves_many_shapes():
         a8, a_s = dev.quantize_rows_f8(a, status)
         check_product(out, a8, a_s, w8, w_s)
     assert status.item() == 0
+
+
+def test_more_than_2_32_values():
+    from rocknpu_b200 import device as dev
+    m, k = 40000, 110000
+    a = torch.empty((m, k), dtype=torch.bfloat16, device="cuda")
+    rows = [0, 19999, 39000, m - 1]
+    a.zero_()
+    for i in rows:
+        a[i] = torch.randn(k, generator=torch.Generator().manual_seed(i)).bfloat16()
+    status = dev.new_status()
+    q, s = dev.quantize_rows_f8(a, status)
+    for i in rows:
+        rq, rs = ref_rows(a[i:i + 1].cpu())
+        assert torch.equal(bits(q[i:i + 1]).cpu(), bits(rq)) and torch.equal(s[i:i + 1].cpu(), rs)
+    assert status.item() == 0
+
+
+def test_output_past_2_31_values():
+    from rocknpu_b200 import device as dev
+    m, n, k = 66000, 33000, 48
+    w8, w_s = weight(n, k, 1)
+    a = torch.randn((m, k), device="cuda")
+    status = dev.new_status()
+    ws = dev.new_workspace(dev.matmul_f8_workspace_bytes(m, n, k))
+    out = dev.matmul_f8(a, w8, w_s, status, ws)
+    a8, a_s = dev.quantize_rows_f8(a, status)
+    for i in (0, 32768, 65077, m - 100):
+        check_product(out[i:i + 100], a8[i:i + 100], a_s[i:i + 100], w8, w_s)
+    assert status.item() == 0
+
+
+def test_refusals():
+    """Shapes, types and devices that the wrappers turn away."""
+    from rocknpu_b200 import device as dev
+    w8, w_s = weight(200, 320, 1)
+    a = torch.randn((4, 320), device="cuda")
+    status = dev.new_status()
+    ws = dev.new_workspace(dev.matmul_f8_workspace_bytes(4, 200, 320))
+    a8, a_s = dev.quantize_rows_f8(a, status)
+    bad = [lambda: dev.quantize_rows_f8(a.double(), status), lambda: dev.quantize_rows_f8(a[0], status),
+           lambda: dev.quantize_rows_f8(a.t(), status), lambda: dev.quantize_rows_f8(a[:0], status),
+           lambda: dev.quantize_rows_f8(a, status.float()), lambda: dev.quantize_rows_f8(a, status.cpu()),
+           lambda: dev.quantize_rows_f8(a, status, out=a8[:, :319]),
+           lambda: dev.quantize_rows_f8(a, status, scales=a_s[:, :2]),
+           lambda: dev.prepare_f8(a.long(), status), lambda: dev.prepare_f8(a[None, None], status),
+           lambda: dev.prepare_f8(torch.randn((4, 9, 320), device="cuda")[::2], status),
+           lambda: dev.prepare_f8_q(4, torch.zeros(100, dtype=torch.uint8, device="cuda"), 256, 1, status),
+           lambda: dev.prepare_f8_q(9, torch.zeros(1000, dtype=torch.uint8, device="cuda"), 256, 1, status),
+           lambda: dev.matmul_f8(a[:, :319], w8, w_s, status, ws), lambda: dev.matmul_f8(a, w8.float(), w_s, status, ws),
+           lambda: dev.matmul_f8(a, w8, w_s[:1], status, ws), lambda: dev.matmul_f8(a, w8, w_s.double(), status, ws),
+           lambda: dev.matmul_f8(a, w8, w_s, status, ws, out=torch.empty((4, 199), device="cuda")),
+           lambda: dev.matmul_f8(a, w8, w_s, status, ws, out_dtype=torch.float64),
+           lambda: dev.gemm_f8(a8, a_s[:, :2], w8, w_s, status), lambda: dev.gemm_f8(a8.float(), a_s, w8, w_s, status),
+           lambda: dev.gemm_f8(a8, a_s, w8[:, :304], w_s, status)]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was accepted")
+    odd = torch.zeros((200, 330), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)[:, 1:321]
+    for call in (lambda: dev.matmul_f8(a, odd, w_s, status, ws),  # rows not at 16-byte boundaries
+                 lambda: dev.matmul_f8(a, w8, w_s, status, ws[:100])):
+        with pytest.raises(RuntimeError):
+            call()
+    assert status.item() == 0

@@ -327,3 +327,71 @@ def test_experts_prepared_from_kquants_and_dense():
     q, s = dev.quantize_rows_f8(y, status)
     ref = (q.float().double() * s.double().repeat_interleave(128, 1)) @ values(*head).t()
     assert ((logits.double() - ref).abs() <= 1e-5 * ref.abs().max()).all()
+
+
+@pytest.mark.parametrize("type_", list(TYPES))
+def test_zero_and_tiny_tokens(type_):
+    """A token of zeros, one near the bottom of f16, hidden values of widely
+    different sizes in one block (gate rows scaled group by group)."""
+    from rocknpu_b200 import device as dev
+    t, h, f, e, top = 4, 384, 272, 3, 2
+    x, gate, up, down, router = layer(t, h, f, e, top, type_, seed=21)
+    x[1] = 0
+    x[2] *= 1e-4
+    up[0].view(torch.uint8)[:, 16:32] = 0                       # a group of zero hidden values
+    up[0].view(torch.uint8)[:, 32:48] &= 0x87                   # a group of small ones
+    status, ws = dev.new_status(), workspace(t, h, f, e, top, x.dtype)
+    out, ids, weights = dev.moe_f8(x, gate, up, down, status, ws, router=router, top_k=top)
+    assert status.item() == 0 and (out[1] == 0).all()
+    check(out, ids, weights, x, gate, up, down)
+
+
+def test_beside_other_work():
+    """Layers on one stream while products keep the SMs busy on another."""
+    from rocknpu_b200 import device as dev
+    t, h, f, e, top = 9, 512, 512, 8, 2
+    x, gate, up, down, router = layer(t, h, f, e, top, "f32", seed=4)
+    status, ws = dev.new_status(), workspace(t, h, f, e, top, x.dtype)
+    big = torch.randn((4096, 4096), device="cuda", dtype=torch.bfloat16)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        with torch.cuda.stream(side):
+            big @ big
+        got.append(dev.moe_f8(x, gate, up, down, status, ws, router=router, top_k=top))
+    torch.cuda.synchronize()
+    assert status.item() == 0
+    for out, ids, weights in got:
+        assert torch.equal(out, got[0][0])
+    check(*got[0], x, gate, up, down)
+
+
+def test_refusals():
+    from rocknpu_b200 import device as dev
+    t, h, f, e, top = 4, 256, 128, 4, 2
+    x, gate, up, down, router = layer(t, h, f, e, top, "f32")
+    status, ws = dev.new_status(), workspace(t, h, f, e, top, x.dtype)
+    ids = torch.zeros((t, top), dtype=torch.int32, device="cuda")
+    weights = torch.ones((t, top), device="cuda")
+
+    def call(x=x, gate=gate, up=up, down=down, ws=ws, **kw):
+        return dev.moe_f8(x, gate, up, down, status, ws, **kw)
+
+    for kw in (dict(), dict(router=router), dict(router=router, top_k=0), dict(router=router, top_k=2, ids=ids),
+               dict(router=router[:3], top_k=2), dict(router=router.double(), top_k=2), dict(ids=ids),
+               dict(ids=ids.long(), weights=weights), dict(ids=ids, weights=weights[:, :1]),
+               dict(ids=ids, weights=weights, top_k=1), dict(ids=ids[:3], weights=weights[:3]),
+               dict(ids=ids, weights=weights, x=x.double()), dict(ids=ids, weights=weights, gate=(gate[0][0], gate[1])),
+               dict(ids=ids, weights=weights, up=down), dict(ids=ids, weights=weights, down=(down[0], down[1][:3])),
+               dict(ids=ids, weights=weights, out=torch.empty((t, h), device="cuda", dtype=torch.float16)),
+               dict(ids=ids.cpu(), weights=weights)):
+        with pytest.raises(ValueError):
+            call(**kw)
+            pytest.fail(f"{list(kw)} was accepted")
+    for kw in (dict(router=router, top_k=5), dict(ids=ids, weights=weights, ws=ws[:1000]),
+               dict(ids=torch.zeros((65, 2), dtype=torch.int32, device="cuda"), weights=torch.ones((65, 2), device="cuda"),
+                    x=torch.randn((65, h), device="cuda"))):
+        with pytest.raises(RuntimeError):
+            call(**kw)
+    assert status.item() == 0
