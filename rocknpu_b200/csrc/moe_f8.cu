@@ -508,10 +508,10 @@ __device__ __forceinline__ void entry_pairs(const Tables& tb, int i, int cap, in
 // ---- the line of groups ----------------------------------------------------
 
 struct Line {
-    int groups, splits, nkb, total;  // groups per (entry, split), splits of k, blocks of k, groups in all
-    int each, more;                  // groups per part, and those left over, spread over the parts
-    __device__ __forceinline__ Line(int entries, int groups_, int splits_, int nkb_)
-        : groups(groups_), splits(splits_), nkb(nkb_), total(entries * groups_ * splits_) {
+    int groups, log_splits, nkb, total;  // groups per (entry, split), splits of k, blocks of k, groups in all
+    int each, more;                      // groups per part, and those left over, spread over the parts
+    __device__ __forceinline__ Line(int entries, int groups_, int log_splits_, int nkb_)
+        : groups(groups_), log_splits(log_splits_), nkb(nkb_), total((entries * groups_) << log_splits_) {
         each = static_cast<int>(static_cast<unsigned>(total) / gridDim.x);
         more = total - each * static_cast<int>(gridDim.x);
     }
@@ -522,15 +522,16 @@ struct Line {
 // groups of ceil(kb / splits) blocks.  A stage of q groups takes q blocks'
 // time, but at least about three: it holds one block of k of each group, and
 // five stages in flight have to cover the latency of memory.
+// Returns the logarithm.
 __device__ __forceinline__ int choose_splits(const MoeParams& p, int entries, int groups) {
-    int best = 1;
+    int best = 0;
     unsigned least = 0xffffffffu;
-    for (int s = 1; s <= p.max_split && s <= p.kb_f; s *= 2) {
+    for (int log = 0, s = 1; s <= p.max_split && s <= p.kb_f; ++log, s *= 2) {
         const unsigned q = (static_cast<unsigned>(entries * groups * s) + gridDim.x - 1) / gridDim.x;
-        const unsigned cost = max(q, 3u) * (static_cast<unsigned>(p.kb_f + s - 1) / static_cast<unsigned>(s));
+        const unsigned cost = max(q, 3u) * (static_cast<unsigned>(p.kb_f + s - 1) >> log);
         if (cost < least) {
             least = cost;
-            best = s;
+            best = log;
         }
     }
     return best;
@@ -549,16 +550,16 @@ struct Walk {
     __device__ __forceinline__ Walk(const Line& l, int part) : cur(l.start(part)), end(l.start(part + 1)) {}
     __device__ __forceinline__ bool next(const Line& l, const Tables& tb, int cap, Pass& s) {
         if (cur >= end) return false;
-        const int es = cur / l.groups, entry = es / l.splits;
+        const int es = cur / l.groups, entry = es >> l.log_splits;
         s.u0 = cur;
-        s.split = es - entry * l.splits;
-        s.k0 = s.split * l.nkb / l.splits;
-        s.k1 = (s.split + 1) * l.nkb / l.splits;
+        s.split = es - (entry << l.log_splits);
+        s.k0 = (s.split * l.nkb) >> l.log_splits;
+        s.k1 = ((s.split + 1) * l.nkb) >> l.log_splits;
         int n;
         entry_pairs(tb, entry, cap, s.pos0, n);
         s.npos = n;
         int avail = min((es + 1) * l.groups, end) - cur;
-        if (l.splits == 1) {
+        if (l.log_splits == 0) {
             // on into the next entries, up to 8 groups
             for (int e = entry + 1; avail < kPassGroups && cur + avail < end; ++e) {
                 int first;
@@ -568,8 +569,8 @@ struct Walk {
                 avail = min((e + 1) * l.groups, end) - cur;
             }
         }
-        const int passes = (avail + kPassGroups - 1) / kPassGroups;
-        s.n = (avail + passes - 1) / passes;  // passes of about one size
+        // full passes first: the rest then shares its blocks among more warps
+        s.n = min(avail, kPassGroups);
         cur += s.n;
         return true;
     }
@@ -822,13 +823,13 @@ struct Consumer {
 
 // The weighted sums of the slots, a warp per token and 128 columns; slots and
 // cuts of k in order, up to eight reads at a time.
-__device__ __forceinline__ void combine(const MoeParams& p, const Tables& tb, int splits, int warp, int warps, int lane) {
+__device__ __forceinline__ void combine(const MoeParams& p, const Tables& tb, int log_splits, int warp, int warps, int lane) {
     const int chunks = (p.h + 127) / 128, items = chunks * p.t;
     for (int item = warp; item < items; item += warps) {
         const int tok = item / chunks, col = (item - tok * chunks) * 128 + lane * 4;
         if (col >= p.h) continue;  // h is a multiple of 16
         float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const int terms = p.top * splits;
+        const int terms = p.top << log_splits;
         const float* from = p.pair_out + static_cast<long long>(tok) * terms * p.h + col;
         for (int i0 = 0; i0 < terms; i0 += 8) {
             float4 d[8];
@@ -836,7 +837,7 @@ __device__ __forceinline__ void combine(const MoeParams& p, const Tables& tb, in
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 // an empty slot's rows are whatever they were
-                const int pair = tok * p.top + min(i0 + i, terms - 1) / splits;
+                const int pair = tok * p.top + (min(i0 + i, terms - 1) >> log_splits);
                 const bool live = i0 + i < terms && tb.pair_e[pair] >= 0;
                 w[i] = live ? tb.pair_w[pair] : 0.0f;
                 d[i] = live ? __ldcg(reinterpret_cast<const float4*>(from + static_cast<long long>(i0 + i) * p.h))
@@ -945,9 +946,7 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
         build_tables(p, tb, kCap, warp, kWarps, lane);
         const int entries = tb.info[0];
         const int groups1 = p.f / kBoxRows, groups2 = (p.h + 31) / 32;
-        const int splits = choose_splits(p, entries, groups2);
-        const Line line1(entries, groups1, 1, p.kb_h);
-        const Line line2(entries, groups2, splits, p.kb_f);
+        const Line line1(entries, groups1, 0, p.kb_h);
 
         if (warp >= kConsumers) {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kProdRegs));
@@ -1016,6 +1015,7 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
                     }
                 }
             }
+            const Line line2(entries, groups2, choose_splits(p, entries, groups2), p.kb_f);
             if (ok && pw == kProducers - 1) {
                 if (lane == 0 && !grid_wait(p.ctrl + kDone + 32, parts, abort)) {
                     if (!*abort) fail(p.err, abort, kErrTimeoutGrid);
@@ -1033,7 +1033,7 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
 #pragma unroll
                     for (int j = 0; j < kEach; ++j) {
                         const int u = min(s.u0 + pw + j * (kProducers - 1), line2.total - 1), es = u / line2.groups;
-                        ex[j] = tb.entry[es / line2.splits] >> 16;
+                        ex[j] = tb.entry[es >> line2.log_splits] >> 16;
                         row[j] = (u - es * line2.groups) * 32;
                     }
                     for (int kb = s.k0; kb < s.k1 && stage_free(); ++kb, ++g) {
@@ -1071,9 +1071,10 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
             Consumer<NG, LO> c;
             int stage = 0;
             bool ok = true;
+            Line line = line1;
             for (int step = 0; ok && step < 2 * nheld; ++step) {
                 const int phase = step < nheld ? 1 : 2, part = held[step < nheld ? step : step - nheld];
-                const Line& line = phase == 1 ? line1 : line2;
+                if (step == nheld) line = Line(entries, groups2, choose_splits(p, entries, groups2), p.kb_f);
                 Walk walk(line, part);
                 Pass s;
                 while (ok && walk.next(line, tb, kCap, s)) {
@@ -1081,7 +1082,7 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
                     const int n2 = s.n > 4 ? 8 : s.n > 2 ? 4 : s.n, ways = kConsumers / n2;
                     const int gi = warp & (n2 - 1), way = warp / n2;
                     const bool mine = gi < s.n;
-                    const int es = (s.u0 + (mine ? gi : 0)) / line.groups, entry = es / line.splits;
+                    const int es = (s.u0 + (mine ? gi : 0)) / line.groups, entry = es >> line.log_splits;
                     const int group = s.u0 + (mine ? gi : 0) - es * line.groups;
                     int first, n;
                     entry_pairs(tb, entry, kCap, first, n);
@@ -1144,7 +1145,7 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
                     if (phase == 1) {
                         if (owner) c.hidden(p, group, first, n, ng, lane);
                     } else {
-                        if (owner) c.slot_rows(p, tb, group, s.split, splits, first, n, ng, lane);
+                        if (owner) c.slot_rows(p, tb, group, s.split, 1 << line.log_splits, first, n, ng, lane);
                     }
                 }
                 if (ok) {
@@ -1159,7 +1160,7 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
                 ok = false;
             }
             if (!cons_any<kConsThreads>(!ok))
-                for (int i = 0; i < nheld; ++i) combine(p, tb, splits, held[i] * kConsumers + warp, parts * kConsumers, lane);
+                for (int i = 0; i < nheld; ++i) combine(p, tb, line.log_splits, held[i] * kConsumers + warp, parts * kConsumers, lane);
         }
     }
     __syncthreads();
