@@ -328,9 +328,11 @@ int rocknpu_b200_gemv_kq(uint32_t kind, const uint8_t *layout, size_t k, size_t 
  * per 128 x 128 block, scales[ceil(n / 128)][ceil(k / 128)] (the last block
  * of a row or column may be shorter).  A block's scale is amax times
  * 1 / 448 (both f32), at least 2^-126, or 1 for a block of zeros; a value is
- * fl(x / scale) rounded to the nearest e4m3 (ties to even).  Products of two scales must be finite.
+ * fl(x / scale) rounded to the nearest e4m3 (ties to even).  Products of two
+ * scales must be finite, and lose precision below 2^-126.
  * `type` / `out_type` are ggml ids: ROCKNPU_GGML_F32, _F16 or _BF16; dense
- * pointers are aligned to their elements (16-byte aligned rows are faster).
+ * pointers are aligned to their elements (16-byte aligned rows are faster),
+ * scales and status words to 4 bytes.
  * A non-finite input sets *status to 1 and leaves the outputs unspecified. */
 
 /* Activation rows a[m][lda] -> a_f8[m][ld_f8] + scales[m][ld_scales]; columns
@@ -358,7 +360,7 @@ size_t rocknpu_b200_gemm_f8_workspace_bytes(size_t m, size_t n, size_t k);
  * `workspace` (optional, device memory, 16-byte aligned) lets shapes with few
  * tiles split K; NULL or fewer than rocknpu_b200_gemm_f8_workspace_bytes runs
  * without.  The first 64 KiB must be zero before the first use of a
- * workspace; every launch that ends with status 0 or 1 leaves them zero, so
+ * workspace; every launch that ends with status 0, 1 or 9 leaves them zero, so
  * one workspace serves calls of any shape, in turn.  Calls that share a
  * workspace must not overlap on the GPU (two streams, two captured graphs
  * replayed at once).  Results do not depend on the order in which CTAs
@@ -397,8 +399,9 @@ typedef struct rocknpu_b200_f8_experts {
  * With a router, ids and weights [tokens][top_k] are outputs (slots in order
  * of falling logits).  Without (NULL) they are inputs: a negative id is an
  * empty slot, whatever its weight; a token with only empty slots gets a row
- * of zeros; an id may occur twice; an id >= experts sets *status to 9
- * (INVALID_ARGUMENT by rocknpu_b200_status_code) and counts as empty.
+ * of zeros, whatever its row of x; an id may occur twice; an id >= experts sets *status to 9
+ * (INVALID_ARGUMENT by rocknpu_b200_status_code) and counts as empty.  out may
+ * be x.
  * Activations are not quantised: f32 ones (and the hidden values) enter the
  * products with 22 bits relative to the largest of their block of 128 (hidden
  * values: of 16), f16 and bf16 ones exactly, with hidden values of 11 bits;

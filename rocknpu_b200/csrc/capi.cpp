@@ -103,6 +103,9 @@ bool dense_ok(uint32_t type, const void* p) {
     return size && p && reinterpret_cast<uintptr_t>(p) % size == 0;
 }
 
+// A pointer to f32 (or 32-bit integer) values.
+bool word_ok(const void* p) { return p && reinterpret_cast<uintptr_t>(p) % 4 == 0; }
+
 // Quantised activations in a workspace: the rows, then their scales.
 size_t quantized_bytes(size_t m, size_t k) {
     return round_up(m * round_up(k, 16), 256) + m * f8_blocks(k) * sizeof(float);
@@ -114,7 +117,7 @@ int launch_status(int e) {
 
 bool gemm_f8_args(rk::GemmF8* g, const uint8_t* w_f8, size_t ld_w, const float* w_scales, void* out, uint32_t out_type,
                   size_t ldo, size_t m, size_t k, size_t n) {
-    if (!w_f8 || !w_scales || !dense_ok(out_type, out) || ld_w < k || ld_w % 16 != 0 || ldo < n ||
+    if (!w_f8 || !word_ok(w_scales) || !dense_ok(out_type, out) || ld_w < k || ld_w % 16 != 0 || ldo < n ||
         reinterpret_cast<uintptr_t>(w_f8) % 16 != 0)
         return false;
     g->w = w_f8;
@@ -138,7 +141,7 @@ bool moe_shape_ok(const rocknpu_b200_moe_f8_args& a) {
 }
 
 bool moe_weight(rk::MoeWeight* o, const rocknpu_b200_f8_experts& w, size_t rows, size_t k, size_t experts) {
-    if (!w.w_f8 || !w.scales || reinterpret_cast<uintptr_t>(w.w_f8) % 16 != 0 || w.ld < k || w.ld % 16 != 0 ||
+    if (!w.w_f8 || !word_ok(w.scales) || reinterpret_cast<uintptr_t>(w.w_f8) % 16 != 0 || w.ld < k || w.ld % 16 != 0 ||
         (experts > 1 && (w.stride < (rows - 1) * w.ld + k || w.stride % 16 != 0 ||
                          w.scale_stride < f8_blocks(rows) * f8_blocks(k))))
         return false;
@@ -1796,7 +1799,7 @@ int rocknpu_b200_gemv_kq(uint32_t kind, const uint8_t* layout, size_t k, size_t 
 
 int rocknpu_b200_quantize_rows_f8(uint32_t type, const void* a, size_t m, size_t k, size_t lda, uint8_t* a_f8,
                                   size_t ld_f8, float* scales, size_t ld_scales, int* status, rocknpu_stream stream) {
-    if (!dense_ok(type, a) || !a_f8 || !scales || !status || !dim_ok(m) || !dim_ok(k) || lda < k || ld_f8 < k ||
+    if (!dense_ok(type, a) || !a_f8 || !word_ok(scales) || !word_ok(status) || !dim_ok(m) || !dim_ok(k) || lda < k || ld_f8 < k ||
         ld_scales < f8_blocks(k))
         return kInvalid;
     return launch_status(rk::launch_quant_rows_f8(static_cast<int>(type), a, static_cast<int>(m), static_cast<int>(k),
@@ -1807,7 +1810,7 @@ int rocknpu_b200_quantize_rows_f8(uint32_t type, const void* a, size_t m, size_t
 
 int rocknpu_b200_prepare_f8(uint32_t type, const void* w, size_t n, size_t k, size_t ldw, size_t count, uint8_t* w_f8,
                             size_t ld_f8, float* scales, int* status, rocknpu_stream stream) {
-    if (!dense_ok(type, w) || !w_f8 || !scales || !status || !dim_ok(n) || !dim_ok(k) || !dim_ok(count) || ldw < k ||
+    if (!dense_ok(type, w) || !w_f8 || !word_ok(scales) || !word_ok(status) || !dim_ok(n) || !dim_ok(k) || !dim_ok(count) || ldw < k ||
         ld_f8 < k)
         return kInvalid;
     return launch_status(rk::launch_prep_f8(static_cast<int>(type), w, static_cast<int>(n), static_cast<int>(k),
@@ -1818,7 +1821,7 @@ int rocknpu_b200_prepare_f8(uint32_t type, const void* w, size_t n, size_t k, si
 
 int rocknpu_b200_prepare_f8_q(uint32_t kind, const uint8_t* blocks, size_t k, size_t n, uint8_t* w_f8, size_t ld_f8,
                               float* scales, int* status, rocknpu_stream stream) {
-    if ((kind != 4 && kind != 5 && kind != 6) || !blocks || !w_f8 || !scales || !status || !dim_ok(n) || !dim_ok(k) ||
+    if ((kind != 4 && kind != 5 && kind != 6) || !blocks || !w_f8 || !word_ok(scales) || !word_ok(status) || !dim_ok(n) || !dim_ok(k) ||
         k % 256 != 0 || ld_f8 < k || ld_f8 % 4 != 0 || reinterpret_cast<uintptr_t>(blocks) % 4 != 0 ||
         reinterpret_cast<uintptr_t>(w_f8) % 4 != 0)
         return kInvalid;
@@ -1837,7 +1840,7 @@ int rocknpu_b200_gemm_f8(const uint8_t* a_f8, size_t ld_a, const float* a_scales
                          size_t ld_w, const float* w_scales, void* out, uint32_t out_type, size_t ldo, size_t m,
                          size_t k, size_t n, void* workspace, size_t workspace_bytes, int* status,
                          rocknpu_stream stream) {
-    if (!a_f8 || !a_scales || !status || ld_as < f8_blocks(k) || ld_a < k || !dim_ok(m) || !dim_ok(k) || !dim_ok(n) ||
+    if (!a_f8 || !word_ok(a_scales) || !word_ok(status) || ld_as < f8_blocks(k) || ld_a < k || !dim_ok(m) || !dim_ok(k) || !dim_ok(n) ||
         ld_a % 16 != 0 || reinterpret_cast<uintptr_t>(a_f8) % 16 != 0 || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
         return kInvalid;
     rk::GemmF8 g;
@@ -1862,7 +1865,7 @@ size_t rocknpu_b200_matmul_f8_workspace_bytes(size_t m, size_t n, size_t k) {
 int rocknpu_b200_matmul_f8(const void* a, uint32_t type, size_t lda, const uint8_t* w_f8, size_t ld_w,
                            const float* w_scales, void* out, uint32_t out_type, size_t ldo, size_t m, size_t k,
                            size_t n, void* workspace, size_t workspace_bytes, int* status, rocknpu_stream stream) {
-    if (!dense_ok(type, a) || !workspace || !status || !dim_ok(m) || !dim_ok(k) || !dim_ok(n) || lda < k ||
+    if (!dense_ok(type, a) || !workspace || !word_ok(status) || !dim_ok(m) || !dim_ok(k) || !dim_ok(n) || lda < k ||
         reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
         return kInvalid;
     rk::GemmF8 g;
@@ -1903,11 +1906,11 @@ size_t rocknpu_b200_moe_f8_workspace_bytes(size_t tokens, size_t hidden, size_t 
 
 int rocknpu_b200_moe_f8(const rocknpu_b200_moe_f8_args* args, void* workspace, size_t workspace_bytes, int* status,
                         rocknpu_stream stream) {
-    if (!args || !workspace || !status || !moe_shape_ok(*args)) return kInvalid;
+    if (!args || !workspace || !word_ok(status) || !moe_shape_ok(*args)) return kInvalid;
     const rocknpu_b200_moe_f8_args& a = *args;
     rk::MoeF8 m;
-    if (!dense_ok(a.type, a.x) || !dense_ok(a.type, a.out) || a.ld_x < a.hidden || a.ld_out < a.hidden || !a.ids ||
-        !a.weights || (a.router && (!dense_ok(a.router_type, a.router) || a.ld_router < a.hidden)) ||
+    if (!dense_ok(a.type, a.x) || !dense_ok(a.type, a.out) || a.ld_x < a.hidden || a.ld_out < a.hidden || !word_ok(a.ids) ||
+        !word_ok(a.weights) || (a.router && (!dense_ok(a.router_type, a.router) || a.ld_router < a.hidden)) ||
         !moe_weight(&m.gate, a.gate, a.ffn, a.hidden, a.experts) ||
         !moe_weight(&m.up, a.up, a.ffn, a.hidden, a.experts) ||
         !moe_weight(&m.down, a.down, a.hidden, a.ffn, a.experts) || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||

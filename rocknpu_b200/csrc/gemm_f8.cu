@@ -392,7 +392,8 @@ F8Plan plan_f8(int m, int n, int k) {
     double best = 1e300;
     for (int bt : {16, 32, 64, 128}) {
         if (bt > 16 && bt >= 2 * m) break;
-        const long long tiles = static_cast<long long>((n + kWRows - 1) / kWRows) * ((m + bt - 1) / bt);
+        const long long tiles =  // more are refused at the launch
+            std::min<long long>(static_cast<long long>((n + kWRows - 1) / kWRows) * ((m + bt - 1) / bt), 0x7fffffff);
         const double block = std::max(4.0 * std::max(55.0, bt / 2.0) + 150.0, (kWRows + bt) * 128 / 60.0);
         const double whole = static_cast<double>((tiles + sms - 1) / sms) * kb * block;
         const long long total = tiles * kb;
@@ -404,7 +405,7 @@ F8Plan plan_f8(int m, int n, int k) {
             best = cost;
             pl.bt = bt;
             pl.stream = stream;
-            pl.tiles = static_cast<int>(std::min<long long>(tiles, 0x7fffffff));
+            pl.tiles = static_cast<int>(tiles);
             pl.grid = static_cast<int>(std::min<long long>(stream ? total : tiles, sms));
             pl.scratch = stream ? static_cast<size_t>(pl.grid) * 2 * kWRows * bt * sizeof(float) : 0;
         }

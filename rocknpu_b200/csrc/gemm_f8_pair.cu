@@ -257,9 +257,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             };
             const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * 128);
             auto add = [&](int c, const uint32_t(&r)[32], float s) {
-const float2 ss = make_float2(s, s);
+                const float2 ss = make_float2(s, s);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) acc[c * 16 + j] = __ffma2_rn(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), ss, acc[c * 16 + j]);
+                for (int j = 0; j < 16; ++j)
+                    acc[c * 16 + j] = __ffma2_rn(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), ss,
+                                                 acc[c * 16 + j]);
             };
             // scales two blocks ahead
             const int last = p.num_kb - 1;
@@ -267,7 +269,7 @@ const float2 ss = make_float2(s, s);
             uint32_t r0[32], r1[32];
             ready(g);
             tmem_ld32(lane_base + (g & 1) * kTile, r0);
-// unrolled, so that the carried piece stays in place (1089 -> 1015 us at
+            // unrolled, so that the carried piece stays in place (1089 -> 1015 us at
             // 4096 x 28672 x 8192)
 #pragma unroll 4
             for (int kb = 0; kb < p.num_kb; ++kb, ++g) {

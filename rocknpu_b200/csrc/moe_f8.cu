@@ -262,6 +262,15 @@ __device__ __forceinline__ void layout_x(const MoeParams& p, int half, int halve
     for (int task = half; task - (lane >> 4) < p.t * p.kb_h; task += halves) {
         const bool live = task < p.t * p.kb_h;
         const int tok = task / p.kb_h, kb = task - tok * p.kb_h, k = kb * kF8Block + l * 8;
+        // a token without a slot (a padded row) may hold anything: it counts as
+        // zeros; a lane per slot
+        static_assert(kMoeMaxTop <= 16, "a slot per lane");
+        bool used = p.router != nullptr;
+        if (!used) {
+            const bool slot = live && l < p.top &&
+                              static_cast<unsigned>(__ldg(p.ids + tok * p.top + l)) < static_cast<unsigned>(p.e);
+            used = (__ballot_sync(0xffffffffu, slot) >> (lane & 16) & 0xFFFFu) != 0u;
+        }
         float v[8];
         if (live && p.wide && k < p.h) {  // h is a multiple of 16
             load_dense8(p.x, p.type, tok * p.ldx + k, v);
@@ -271,7 +280,10 @@ __device__ __forceinline__ void layout_x(const MoeParams& p, int half, int halve
         }
         uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, mag_bits(v[i]));
+        for (int i = 0; i < 8; ++i) {
+            v[i] = used ? v[i] : 0.0f;
+            m = max(m, mag_bits(v[i]));
+        }
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
         most = max(most, m);
@@ -362,9 +374,9 @@ __device__ __forceinline__ void router_products(const MoeParams& p, const Tables
 
 // ---- routing ---------------------------------------------------------------
 
-// Order-preserving integer of a logit, above 0; NaN sorts last.
+// Order-preserving integer of a logit, above 0; -0 is 0, NaN sorts last.
 __device__ __forceinline__ uint32_t sort_key(float v) {
-    const uint32_t b = __float_as_uint(v);
+    const uint32_t b = __float_as_uint(v + 0.0f);
     if ((b & 0x7FFFFFFFu) > 0x7F800000u) return 1u;
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }

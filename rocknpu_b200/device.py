@@ -167,12 +167,12 @@ def _device_of(first: torch.Tensor, *others) -> int:
 _ENTRY = {}
 
 
-def _launch(name: str, dev: int, stream, *args) -> None:
-    """Call entry point `name` with device `dev` current; the stream goes last."""
+def _launch(name: str, dev: int, *args) -> None:
+    """Call entry point `name` on device `dev` and its current stream."""
     fn = _ENTRY.get(name)
     if fn is None:
         fn = _ENTRY[name] = getattr(lib(), "rocknpu_b200_" + name)
-    handle = torch._C._cuda_getCurrentRawStream(dev) if stream is None else _stream(stream)
+    handle = torch._C._cuda_getCurrentRawStream(dev)
     if torch._C._cuda_getDevice() == dev:
         st = fn(*args, handle)
     else:
@@ -180,6 +180,17 @@ def _launch(name: str, dev: int, stream, *args) -> None:
             st = fn(*args, handle)
     if st != 0:
         raise RuntimeError(f"{name} failed with status {st}")
+
+
+def _on(stream, dev: int):
+    """The given stream as the current one, so that what a call allocates
+    belongs to it."""
+    if not isinstance(stream, torch.cuda.Stream):
+        handle = int(stream)
+        stream = torch.cuda.ExternalStream(handle, device=dev) if handle else torch.cuda.default_stream(dev)
+    if stream.device.index != dev:
+        raise ValueError("the stream is on another device than the operands")
+    return torch.cuda.stream(stream)
 
 
 def _status_ptr(status: torch.Tensor) -> int:
@@ -250,6 +261,9 @@ def quantize_rows_f8(a: torch.Tensor, status: torch.Tensor, out: torch.Tensor | 
                      scales: torch.Tensor | None = None, stream=None):
     """f32 / f16 / bf16 [m, k] -> (e4m3 [m, k], f32 scales [m, ceil(k / 128)])."""
     dev = _device_of(a, status, out, scales)
+    if stream is not None:
+        with _on(stream, dev):
+            return quantize_rows_f8(a, status, out, scales)
     m, k, lda, type_ = _dense_rows(a, "a")
     if out is None:
         out = _f8_empty(a, m, k)
@@ -258,7 +272,7 @@ def quantize_rows_f8(a: torch.Tensor, status: torch.Tensor, out: torch.Tensor | 
     rows, cols, ld8 = _f8_rows(out, "out")
     if rows != m or cols != k:
         raise ValueError("out has a's shape")
-    _launch("quantize_rows_f8", dev, stream, type_, a.data_ptr(), m, k, lda, out.data_ptr(), ld8, scales.data_ptr(),
+    _launch("quantize_rows_f8", dev, type_, a.data_ptr(), m, k, lda, out.data_ptr(), ld8, scales.data_ptr(),
             _row_scales(scales, m, k, "scales"), _status_ptr(status))
     return out, scales
 
@@ -267,6 +281,9 @@ def prepare_f8(w: torch.Tensor, status: torch.Tensor, stream=None):
     """Dense weight(s) [n, k] or [experts, n, k] -> (e4m3 of the same shape,
     f32 scales [..., ceil(n / 128), ceil(k / 128)])."""
     dev = _device_of(w, status)
+    if stream is not None:
+        with _on(stream, dev):
+            return prepare_f8(w, status)
     if w.dim() not in (2, 3):
         raise ValueError("w is a matrix or a stack of them")
     n, k, ldw, type_ = _dense_rows(w if w.dim() == 2 else w[0] if w.shape[0] else w.flatten(0, 1), "w")
@@ -275,7 +292,7 @@ def prepare_f8(w: torch.Tensor, status: torch.Tensor, stream=None):
         raise ValueError("a stack of weights has no gaps between them")
     out = _f8_empty(w, *w.shape)
     scales = w.new_empty((*w.shape[:-2], _f8_blocks(n), _f8_blocks(k)), dtype=torch.float32)
-    _launch("prepare_f8", dev, stream, type_, w.data_ptr(), n, k, ldw, count, out.data_ptr(), (k + 15) // 16 * 16,
+    _launch("prepare_f8", dev, type_, w.data_ptr(), n, k, ldw, count, out.data_ptr(), (k + 15) // 16 * 16,
             scales.data_ptr(), _status_ptr(status))
     return out, scales
 
@@ -283,13 +300,16 @@ def prepare_f8(w: torch.Tensor, status: torch.Tensor, stream=None):
 def prepare_f8_q(kind: int, blocks: torch.Tensor, k: int, n: int, status: torch.Tensor, stream=None):
     """K-quant rows -> (e4m3 [n, k], f32 scales [ceil(n / 128), k / 128])."""
     dev = _device_of(blocks, status)
+    if stream is not None:
+        with _on(stream, dev):
+            return prepare_f8_q(kind, blocks, k, n, status)
     if blocks.dtype is not torch.uint8 or not blocks.is_contiguous():
         raise ValueError("blocks are contiguous uint8")
     if kind not in BLOCK_BYTES or k <= 0 or n <= 0 or k % 256 or blocks.numel() < n * (k // 256) * BLOCK_BYTES[kind]:
         raise ValueError("blocks hold n rows of k / 256 superblocks")
     out = blocks.new_empty((n, k), dtype=torch.float8_e4m3fn)
     scales = blocks.new_empty((_f8_blocks(n), _f8_blocks(k)), dtype=torch.float32)
-    _launch("prepare_f8_q", dev, stream, kind, blocks.data_ptr(), k, n, out.data_ptr(), k, scales.data_ptr(),
+    _launch("prepare_f8_q", dev, kind, blocks.data_ptr(), k, n, out.data_ptr(), k, scales.data_ptr(),
             _status_ptr(status))
     return out, scales
 
@@ -308,13 +328,16 @@ def gemm_f8(a8: torch.Tensor, a_scales: torch.Tensor, w8: torch.Tensor, w_scales
     """Block-scaled e4m3 product a8 [m, k] . w8 [n, k]^T (quantize_rows_f8,
     prepare_f8).  Rows start at multiples of 16 bytes."""
     dev = _device_of(a8, a_scales, w8, w_scales, status, out, workspace)
+    if stream is not None:
+        with _on(stream, dev):
+            return gemm_f8(a8, a_scales, w8, w_scales, status, out, out_dtype, workspace)
     m, k, lda = _f8_rows(a8, "a8")
     n, kw, ldw = _f8_rows(w8, "w8")
     if kw != k:
         raise ValueError("w8 is [n, k]")
     _weight_scales(w_scales, (_f8_blocks(n), _f8_blocks(k)), "w8")
     out, out_type, ldo = _dense_out(out, m, n, out_dtype, a8)
-    _launch("gemm_f8", dev, stream, a8.data_ptr(), lda, a_scales.data_ptr(), _row_scales(a_scales, m, k, "a_scales"),
+    _launch("gemm_f8", dev, a8.data_ptr(), lda, a_scales.data_ptr(), _row_scales(a_scales, m, k, "a_scales"),
             w8.data_ptr(), ldw, w_scales.data_ptr(), out.data_ptr(), out_type, ldo, m, k, n,
             None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.nbytes,
             _status_ptr(status))
@@ -328,13 +351,16 @@ def matmul_f8(a: torch.Tensor, w8: torch.Tensor, w_scales: torch.Tensor, status:
     `workspace` (new_workspace of matmul_f8_workspace_bytes) is kept by the
     caller, one per stream on which calls may be in flight."""
     dev = _device_of(a, w8, w_scales, status, workspace, out)
+    if stream is not None:
+        with _on(stream, dev):
+            return matmul_f8(a, w8, w_scales, status, workspace, out, out_dtype)
     m, k, lda, type_ = _dense_rows(a, "a")
     n, kw, ldw = _f8_rows(w8, "w8")
     if kw != k:
         raise ValueError("w8 is [n, k]")
     _weight_scales(w_scales, (_f8_blocks(n), _f8_blocks(k)), "w8")
     out, out_type, ldo = _dense_out(out, m, n, out_dtype or a.dtype, a)
-    _launch("matmul_f8", dev, stream, a.data_ptr(), type_, lda, w8.data_ptr(), ldw, w_scales.data_ptr(),
+    _launch("matmul_f8", dev, a.data_ptr(), type_, lda, w8.data_ptr(), ldw, w_scales.data_ptr(),
             out.data_ptr(), out_type, ldo, m, k, n, workspace.data_ptr(), workspace.nbytes, _status_ptr(status))
     return out
 
@@ -376,6 +402,10 @@ def moe_f8(x: torch.Tensor, gate, up, down, status: torch.Tensor, workspace: tor
     `workspace`: new_workspace(moe_f8_workspace_bytes(...)), kept by the
     caller, one per stream on which calls may be in flight."""
     dev = _device_of(x, *gate, *up, *down, status, workspace, router, ids, weights, out)
+    if stream is not None:
+        with _on(stream, dev):
+            return moe_f8(x, gate, up, down, status, workspace, router=router, top_k=top_k, renormalize=renormalize,
+                          ids=ids, weights=weights, out=out)
     t, h, ldx, type_ = _dense_rows(x, "x")
     if gate[0].dim() != 3:
         raise ValueError("gate is [experts, ffn, hidden]")
@@ -404,5 +434,5 @@ def moe_f8(x: torch.Tensor, gate, up, down, status: torch.Tensor, workspace: tor
                           *_experts(gate, (e, f, h), "gate"), *_experts(up, (e, f, h), "up"),
                           *_experts(down, (e, h, f), "down"), 0 if router is None else router.data_ptr(), router_type,
                           ld_router, 1 if renormalize else 0, ids.data_ptr(), weights.data_ptr())
-    _launch("moe_f8", dev, stream, args, workspace.data_ptr(), workspace.nbytes, _status_ptr(status))
+    _launch("moe_f8", dev, args, workspace.data_ptr(), workspace.nbytes, _status_ptr(status))
     return out, ids, weights

@@ -137,6 +137,31 @@ def test_moe_argument_bytes():
     assert flat == values[:len(flat)] and struct.calcsize("P") == 8
 
 
+@pytest.mark.parametrize("bad", [P + 1, P + 2, P + 3])
+def test_unaligned_scales_indices_and_status(bad):
+    lib = rk.lib()
+    for name in ("scales", "status"):
+        assert lib.rocknpu_b200_quantize_rows_f8(*changed(QUANTIZE, **{name: bad})) == BAD
+        assert lib.rocknpu_b200_prepare_f8(*changed(PREPARE, **{name: bad})) == BAD
+        assert lib.rocknpu_b200_prepare_f8_q(*changed(PREPARE_Q, **{name: bad})) == BAD
+    for name in ("a_s", "w_s", "status"):
+        assert lib.rocknpu_b200_gemm_f8(*changed(GEMM, **{name: bad})) == BAD
+    for name in ("w_s", "status"):
+        assert lib.rocknpu_b200_matmul_f8(*matmul_args(**{name: bad})) == BAD
+    for name in ("gate__scales", "up__scales", "down__scales", "ids", "weights", "status"):
+        assert moe_call(**{name: bad}) == BAD
+
+
+def test_workspace_sizes_of_the_largest_dimensions():
+    """Sizes nothing can hold are answered without overflow."""
+    lib, most = rk.lib(), 0x7fffff00
+    for m, n, k in [(most, 1, most), (1, most, most), (most, most, most)]:
+        assert 65536 <= lib.rocknpu_b200_gemm_f8_workspace_bytes(m, n, k) < 64 << 20
+        assert lib.rocknpu_b200_matmul_f8_workspace_bytes(m, n, k) >= m * k
+    for m, n, k in [(most + 1, 1, 1), (1, most + 1, 1), (1, 1, most + 1)]:
+        assert lib.rocknpu_b200_gemm_f8_workspace_bytes(m, n, k) == 0
+
+
 def test_host_tensors_are_refused():
     from rocknpu_b200 import device as dev
     a, status = torch.zeros((2, 128)), torch.zeros(1, dtype=torch.int32)

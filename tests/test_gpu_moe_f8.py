@@ -191,6 +191,91 @@ def test_no_slot_used():
     assert status.item() == 0 and (out[:, :h] == 0).all() and (out[:, h:] == 5).all()
 
 
+@pytest.mark.parametrize("type_", list(TYPES))
+def test_padded_rows_may_hold_anything(type_):
+    """Tokens whose slots are all empty: NaN and infinities in their rows of x
+    and in their weights change nothing and set no status."""
+    from rocknpu_b200 import device as dev
+    t, h, f, e, top = 11, 272, 160, 4, 3
+    x, gate, up, down, _ = layer(t, h, f, e, top, type_, seed=3)
+    g = torch.Generator().manual_seed(4)
+    ids = torch.randint(0, e, (t, top), generator=g, dtype=torch.int32)
+    weights = torch.rand((t, top), generator=g)
+    pad = [0, 4, 5, 10]
+    ids[pad] = -1
+    ids[1, 0] = -7
+    ids, weights = ids.cuda(), weights.cuda()
+    status, ws = dev.new_status(), workspace(t, h, f, e, top, x.dtype)
+    plain, _, _ = dev.moe_f8(x, gate, up, down, status, ws, ids=ids, weights=weights)
+    x[0], x[4, 7], x[5], x[10, ::3] = float("nan"), float("inf"), -float("inf"), float("nan")
+    weights[pad], weights[1, 0] = float("nan"), float("inf")
+    out, _, _ = dev.moe_f8(x, gate, up, down, status, ws, ids=ids, weights=weights)
+    assert status.item() == 0
+    assert torch.equal(out, plain) and (out[pad] == 0).all()
+    x[1, 3] = float("nan")
+    dev.moe_f8(x, gate, up, down, status, ws, ids=ids, weights=weights)
+    assert status.item() == 1
+
+
+def test_logits_of_both_zeros_are_equal():
+    """Products that underflow to -0 and to +0 take the lower expert too."""
+    from rocknpu_b200 import device as dev
+    t, h, f, e, top = 2, 256, 256, 6, 3
+    x, gate, up, down, _ = layer(t, h, f, e, top, "f32")
+    x = torch.full_like(x, 1e-30)
+    router = torch.full((e, h), 1e-30, device="cuda")
+    router[::2] *= -1.0
+    status, ws = dev.new_status(), workspace(t, h, f, e, top, x.dtype)
+    _, ids, _ = dev.moe_f8(x, gate, up, down, status, ws, router=router, top_k=top)
+    assert status.item() == 0
+    assert torch.equal(ids.cpu(), torch.arange(top, dtype=torch.int32).expand(t, top))
+
+
+@pytest.mark.parametrize("raw", [False, True])
+def test_given_stream_owns_the_results(raw):
+    """A call with a stream allocates on it: results reuse no block that work
+    on the current stream may still read."""
+    from rocknpu_b200 import device as dev
+    t, h, f, e, top = 3, 512, 256, 4, 2
+    x, gate, up, down, router = layer(t, h, f, e, top, "bf16")
+    status, ws = dev.new_status(), workspace(t, h, f, e, top, x.dtype)
+    want = dev.moe_f8(x, gate, up, down, status, ws, router=router, top_k=top)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    busy = torch.randn((4096, 4096), device="cuda")
+    for _ in range(20):
+        busy = busy @ busy * 1e-2
+    held = torch.empty_like(want[0])
+    address = held.data_ptr()
+    del held  # free for the current stream, whose queue is long
+    out, ids, weights = dev.moe_f8(x, gate, up, down, status, ws, router=router, top_k=top,
+                                   stream=side.cuda_stream if raw else side)
+    side.synchronize()
+    assert out.data_ptr() != address
+    assert torch.equal(out, want[0]) and torch.equal(ids, want[1]) and torch.equal(weights, want[2])
+    a8, a_s = dev.quantize_rows_f8(x, status, stream=side)
+    w8, w_s = dev.prepare_f8(router, status, stream=side)
+    one = dev.gemm_f8(a8, a_s, w8, w_s, status, stream=side)
+    need = dev.matmul_f8_workspace_bytes(t, e, h)
+    with torch.cuda.stream(side):
+        own = dev.new_workspace(need)
+    two = dev.matmul_f8(x, w8, w_s, status, own, out_dtype=torch.float32, stream=0 if raw else side)
+    torch.cuda.synchronize()
+    assert torch.equal(one, two) and status.item() == 0
+
+
+def test_out_in_place_of_x():
+    """x is read before anything is stored: out may be x."""
+    from rocknpu_b200 import device as dev
+    t, h, f, e, top = 19, 384, 256, 4, 2
+    x, gate, up, down, router = layer(t, h, f, e, top, "f32")
+    status, ws = dev.new_status(), workspace(t, h, f, e, top, x.dtype)
+    want = dev.moe_f8(x, gate, up, down, status, ws, router=router, top_k=top)
+    got = dev.moe_f8(x, gate, up, down, status, ws, router=router, top_k=top, out=x)
+    assert got[0].data_ptr() == x.data_ptr()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and status.item() == 0
+
+
 def test_index_out_of_range_sets_status():
     from rocknpu_b200 import device as dev
     from rocknpu_b200 import lib
