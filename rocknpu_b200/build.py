@@ -24,7 +24,7 @@ LIB = os.path.join(HERE, "librocknpu.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O3",
               "--expt-relaxed-constexpr", "-I", INCLUDE]
-SOURCES = ["quant.cu", "quant_f8.cu", "gemm.cu", "gemm_plain.cu", "gemm_fused.cu", "gemm_gather.cu", "gemm_pair.cu", "gemm_f8.cu", "gemm_f8_pair.cu", "moe_f8.cu", "gemv.cu", "gemv_kq.cu", "gemv_q4k.cu", "gemv_q6k.cu", "noalloc.cu", "shard.cu", "capi.cpp", "plugin_rules.cpp", "sidecar.cpp", "synth.cpp", "hostmem.cpp", "plugin_graph.cpp"]
+SOURCES = ["quant.cu", "quant_f8.cu", "gemm.cu", "gemm_plain.cu", "gemm_fused.cu", "gemm_gather.cu", "gemm_pair.cu", "gemm_f8.cu", "gemm_f8_pair.cu", "gemv_f8.cu", "moe_f8.cu", "gemv.cu", "gemv_kq.cu", "gemv_q4k.cu", "gemv_q6k.cu", "noalloc.cu", "shard.cu", "capi.cpp", "plugin_rules.cpp", "sidecar.cpp", "synth.cpp", "hostmem.cpp", "plugin_graph.cpp"]
 HEADERS = ["kernels.h", "ptx.cuh", "quant_math.cuh", "kquant.cuh", "f8.cuh", "gemm_f8.cuh", "gemm_kernel.cuh", "gemv_stage.cuh"]
 
 

@@ -1872,6 +1872,9 @@ int rocknpu_b200_matmul_f8(const void* a, uint32_t type, size_t lda, const uint8
     if (!gemm_f8_args(&g, w_f8, ld_w, w_scales, out, out_type, ldo, m, k, n)) return kInvalid;
     const size_t head = round_up(rocknpu_b200_gemm_f8_workspace_bytes(m, n, k), 256), ld8 = round_up(k, 16);
     if (workspace_bytes < head + quantized_bytes(m, k)) return kInvalid;
+    if (rk::gemv_f8_fits(g) && rk::gemv_f8_quantizes(g))
+        return launch_status(rk::launch_gemv_f8(g, a, static_cast<int>(type), static_cast<long long>(lda), status,
+                                                static_cast<cudaStream_t>(stream)));
     uint8_t* a8 = static_cast<uint8_t*>(workspace) + head;
     float* as = reinterpret_cast<float*>(a8 + round_up(m * ld8, 256));
     g.a = a8;

@@ -456,6 +456,7 @@ int launch_cfg(const F8Params& p, int grid, cudaStream_t s) {
 size_t gemm_f8_scratch_bytes(int m, int n, int k) { return plan_f8(m, n, k).scratch; }
 
 int launch_gemm_f8(const GemmF8& g, int* err, cudaStream_t s) {
+    if (gemv_f8_fits(g)) return launch_gemv_f8(g, nullptr, 0, 0, err, s);
     F8Plan pl = plan_f8(g.m, g.n, g.k);
     if (pl.stream && (!g.counters || !g.scratch || g.scratch_bytes < pl.scratch)) {
         pl.stream = false;

@@ -181,6 +181,12 @@ struct GemmF8 {
     bool early_weights = false;
 };
 int launch_gemm_f8(const GemmF8& g, int* err, cudaStream_t s);
+// The form for a few tokens (gemv_f8.cu): whether it takes the product, and
+// whether it quantises the rows itself ([m][ld] of type at `dense`) better
+// than a launch of its own; dense null: g.a.
+bool gemv_f8_fits(const GemmF8& g);
+bool gemv_f8_quantizes(const GemmF8& g);
+int launch_gemv_f8(const GemmF8& g, const void* dense, int type, long long ld, int* err, cudaStream_t s);
 
 // A mixture-of-experts layer (moe_f8.cu) over stacks of prepared weights.
 constexpr int kMoeMaxTokens = 64, kMoeMaxTop = 16, kMoeMaxExperts = 256;

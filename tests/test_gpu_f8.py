@@ -216,6 +216,37 @@ def test_matmul_types(type_, m, n, k):
     check_product(wide, a8, a_s, w8, w_s)
 
 
+@pytest.mark.parametrize("type_", list(TYPES))
+@pytest.mark.parametrize("m,n,k", [(1, 1, 32), (1, 16, 128), (1, 17, 96), (2, 130, 160), (3, 40, 288), (5, 48, 1600),
+                                   (8, 5632, 2048), (9, 300, 4096), (16, 1000, 1024), (1, 333, 16384), (2, 6000, 8192),
+                                   (8, 2400, 8192), (16, 129, 64), (4, 20000, 512), (1, 40000, 256), (7, 9999, 2080)])
+def test_few_tokens(type_, m, n, k):
+    """Rows that the product may quantise itself and rows that it may not; a
+    weight that starts at a 16-byte boundary only; wider rows around the result."""
+    from rocknpu_b200 import device as dev
+    w8, w_s = weight(n, k, m + k)
+    a = (torch.randn((m, k + 3), device="cuda", generator=torch.Generator("cuda").manual_seed(n)) * 3).to(TYPES[type_])
+    a[:, 40:70] = 0
+    status = dev.new_status()
+    ws = dev.new_workspace(dev.matmul_f8_workspace_bytes(m, n, k))
+    for rows in (a[:, :k], a[:, 3:], a[:, :k].contiguous()):
+        a8, a_s = dev.quantize_rows_f8(rows, status)
+        wide = torch.full((m, n + 9), -5.0, device="cuda")
+        out = dev.matmul_f8(rows, w8, w_s, status, ws, out=wide[:, 4:4 + n])
+        check_product(out, a8, a_s, w8, w_s)
+        assert (wide[:, :4] == -5).all() and (wide[:, 4 + n:] == -5).all()
+        assert torch.equal(out, dev.gemm_f8(a8, a_s, w8, w_s, status, workspace=ws))
+        own = dev.matmul_f8(rows, w8, w_s, status, ws)
+        assert own.dtype == rows.dtype and torch.equal(own, out.to(rows.dtype))
+    odd = torch.zeros(n * k + 16, dtype=torch.uint8, device="cuda")[16:].view(n, k).view(torch.float8_e4m3fn)
+    odd.view(torch.uint8).copy_(w8.view(torch.uint8))
+    check_product(dev.matmul_f8(rows, odd, w_s, status, ws, out_dtype=torch.float32), a8, a_s, w8, w_s)
+    assert status.item() == 0
+    rows[m - 1, k - 1] = float("nan")
+    dev.matmul_f8(rows, w8, w_s, status, ws)
+    assert status.item() == 1
+
+
 def test_matmul_strided_rows_leave_the_rest():
     from rocknpu_b200 import device as dev
     m, n, k = 19, 200, 320
