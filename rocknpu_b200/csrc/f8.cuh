@@ -31,20 +31,31 @@ __device__ __forceinline__ uint32_t f8_pack4(float a, float b, float c, float d)
     return f8_pack2(a, b) | (f8_pack2(c, d) << 16);
 }
 
-// fl(x / s) for the values of a block whose scale is s.  Markstein's method
-// (IBM J. Res. Dev. 34, 1990): with y = RN(1 / s), a quotient q off by less
-// than a unit in the last place and its exact remainder r = x - q s (one
-// fused multiply-add), q + r y rounds to the IEEE quotient.  x y is off by at
-// most 1.5 units, so a first step brings it within one and a second makes it
-// exact: five multiply-adds where the IEEE division takes about thirty
-// instructions.  The remainder of a quotient that matters (2^-11 and more;
-// smaller ones are 0 in e4m3) is exact for s >= 2^-100; below that, and in no
-// real tensor, the division itself.
+// A quotient whose e4m3 rounding is that of fl(x / s): one step of Markstein's
+// method (IBM J. Res. Dev. 34, 1990) from x y, y = RN(1 / s).  x y is off by
+// at most 2^-23 of it, the step's remainder and y by 2^-24 of theirs, so q is
+// the rounding of a number within 2^-46 of x / s, and differs from fl(x / s)
+// only if x / s is that near to the middle of two neighbouring floats.  The
+// e4m3 codes then differ only if one of those floats is the middle of two
+// e4m3 values.  With s = S 2^i and x = X 2^j (24-bit S, X) and the floats'
+// middle C 2^l, C = 2^20 M +- 1 (25 bits, M of 5; 2^21 M - 1 below a power of
+// two), that is X 2^k - S C = N, |N| <= 2^49 2^-46 = 8, k >= 23: S is within 8
+// of a multiple of 2^20.  N = 0 cannot be, C is odd and longer than X.  For
+// such S but the multiples themselves (16 of 2^20) f8_codes() divides.
+// Neither a quotient that matters (2^-11 and more; smaller ones are 0 in
+// e4m3) nor its remainder, a multiple of 2^-34 2^-23 s, underflows for
+// s >= 2^-90; for a smaller s, in no real tensor, f8_codes() divides too.
+// Three operations where the IEEE division takes about thirty; the signs are
+// such that a quotient of -0 stays one.
 __device__ __forceinline__ float f8_quotient(float x, float s, float y) {
-    float q = __fmul_rn(x, y);
-    q = __fmaf_rn(__fmaf_rn(-q, s, x), y, q);
-    q = __fmaf_rn(__fmaf_rn(-q, s, x), y, q);
-    return copysignf(q, x);  // a quotient of -0 came out as 0
+    const float q = __fmul_rn(x, y);
+    return __fmaf_rn(-y, __fmaf_rn(q, s, -x), q);
+}
+
+// Whether f8_quotient serves a block of this scale.
+__device__ __forceinline__ bool f8_quick(float s) {
+    const uint32_t near = (__float_as_uint(s) + 8u) & 0xFFFFFu;
+    return s >= 8.0779357e-28f && (near > 16u || near == 8u);
 }
 
 // e4m3 codes of a thread's values of one block (N a multiple of 4), four per
@@ -52,7 +63,7 @@ __device__ __forceinline__ float f8_quotient(float x, float s, float y) {
 template <int N>
 __device__ __forceinline__ void f8_codes(const float (&v)[N], float s, uint32_t (&code)[N / 4]) {
     float q[N];
-    if (s >= 7.88860905e-31f) {
+    if (f8_quick(s)) {
         const float y = __frcp_rn(s);
 #pragma unroll
         for (int i = 0; i < N; ++i) q[i] = f8_quotient(v[i], s, y);
@@ -132,6 +143,23 @@ struct Raw8 {
                 w[i] = b;
             else
                 w[i / 2] = (i & 1) ? (w[i / 2] | (b << 16)) : b;
+        }
+    }
+    // the largest magnitude, as f32 bits (mag_bits); 16-bit types two at a time
+    __device__ __forceinline__ uint32_t mag_max() const {
+        if constexpr (sizeof(T) == 4) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+            return m;
+        } else {
+            uint32_t m = w[0] & 0x7FFF7FFFu;
+#pragma unroll
+            for (int i = 1; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+            const unsigned short b = static_cast<unsigned short>(max(m & 0xFFFFu, m >> 16));
+            T x;
+            memcpy(&x, &b, 2);
+            return __float_as_uint(to_f32<T>(x));
         }
     }
     __device__ __forceinline__ void values(float (&v)[8]) const {

@@ -109,9 +109,7 @@ __device__ __forceinline__ void fill(const GemvParams& p, uint8_t* act) {
                 raw.load_some(row + col, p.k - col);
             float v[8];
             raw.values(v);
-            uint32_t m = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) m = max(m, mag_bits(v[j]));
+            uint32_t m = raw.mag_max();
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
             most = max(most, m);

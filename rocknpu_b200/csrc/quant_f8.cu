@@ -17,8 +17,7 @@ namespace {
 
 constexpr int kRowsThreads = 256;
 constexpr int kRowsUnroll = 2;  // blocks of 128 per half-warp and step
-template <class T>
-constexpr int kRowsCtas = 4;  // per SM (bf16 16384 x 8192: 4 107 us, 5 110, 6 123)
+constexpr int kRowsCtas = 4;  // per SM (bf16 16384 x 8192: 4 97 us, 5 101, 6 105)
 
 __device__ __forceinline__ uint32_t half_warp_max(uint32_t v) {
 #pragma unroll
@@ -80,7 +79,7 @@ struct At {
 // quantised.  Triggers the dependent product at its start: that reads nothing
 // of this kernel's before its own wait.
 template <class T, bool VEC>
-__global__ void __launch_bounds__(kRowsThreads, kRowsCtas<T>)
+__global__ void __launch_bounds__(kRowsThreads, kRowsCtas)
     rows_f8_kernel(const T* __restrict__ a, int k, long long lda, unsigned kb, unsigned blocks,
                    uint8_t* __restrict__ out, long long ld8, float* __restrict__ scales, long long lds, int* err) {
     constexpr int U = kRowsUnroll;
@@ -113,7 +112,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtas<T>)
         for (int u = 0; u < U; ++u) {
             float v[8];
             cur[u].values(v);
-            const uint32_t m = half_warp_max(mag_max(v));
+            const uint32_t m = half_warp_max(cur[u].mag_max());
             most = max(most, m);
             const float s = f8_scale(__uint_as_float(m));
             if (at.b < blocks) {
@@ -135,12 +134,13 @@ int rows_f8(const T* a, int m, int k, long long lda, uint8_t* out, long long ld8
     const unsigned long long total = static_cast<unsigned long long>(m) * kb;
     if (total > 0xF0000000ull) return cudaErrorInvalidValue;
     const unsigned per = kRowsThreads / 16 * kRowsUnroll;
-    const unsigned grid = static_cast<unsigned>(std::min<unsigned long long>((total + per - 1) / per, sm_count() * kRowsCtas<T>));
+    const unsigned grid = static_cast<unsigned>(std::min<unsigned long long>((total + per - 1) / per, sm_count() * kRowsCtas));
     const bool vec = (reinterpret_cast<uintptr_t>(a) % 16 == 0) && (lda * sizeof(T)) % 16 == 0 &&
                      (reinterpret_cast<uintptr_t>(out) % 8 == 0) && ld8 % 8 == 0;
     auto kern = vec ? rows_f8_kernel<T, true> : rows_f8_kernel<T, false>;
     // the max-shared carveout, so that the dependent product's CTA (about
-    // 200 KB of shared memory) becomes resident beside these
+    // 200 KB of shared memory) becomes resident beside these; a long run is no
+    // slower with it
     static bool carve[64][2] = {};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -193,11 +193,7 @@ __global__ void __launch_bounds__(kPrepThreads, sizeof(T) == 4 ? 2 : 4) prep_f8_
     }
     uint32_t m = 0;
 #pragma unroll
-    for (int p = 0; p < 8; ++p) {
-        float v[8];
-        raw[p].values(v);
-        m = max(m, mag_max(v));
-    }
+    for (int p = 0; p < 8; ++p) m = max(m, raw[p].mag_max());
     m = cta_max<kPrepThreads>(m, red);
     const float s = f8_scale(__uint_as_float(m));
     if (threadIdx.x == 0) {

@@ -116,6 +116,49 @@ def test_quantize_rows_smallest_and_largest_values():
     assert status.item() == 0 and torch.equal(s.cpu(), rs) and torch.equal(bits(q).cpu(), bits(rq))
 
 
+def nearly_half_quotients():
+    """Rows whose quotients lie as near to the middle of two floats as any, next
+    to a middle of two e4m3 values: scales S 2^i with S within 40 of a multiple
+    of 2^20 (and others), x one of the three floats at s C 2^e, C = 2^20 M +- 1."""
+    rng = np.random.default_rng(7)
+    rows = []
+    for a in range(8, 17):
+        for n in list(range(-40, 41)) + [int(v) for v in rng.integers(-2 ** 19, 2 ** 19, 40)]:
+            S = a * 2 ** 20 + n
+            if not 2 ** 23 <= S < 2 ** 24:
+                continue
+            s = np.float32(S) * np.float32(2.0 ** -23)
+            near = np.float32(s * np.float32(448.0)).view(np.uint32).astype(np.int64) + np.arange(-4, 5)
+            amax = near.astype(np.uint32).view(np.float32)
+            amax = amax[amax * np.float32(1.0 / 448.0) == s]
+            if not len(amax):
+                continue
+            M = rng.integers(16, 32, 127).astype(object)
+            C = M * 2 ** 20 + rng.choice([-1, 0, 1], 127).astype(object)
+            e = rng.integers(-10, 8, 127)
+            product = np.array([S * int(c) for c in C], dtype=object)  # up to 49 bits
+            x = np.array([float(v) for v in product]) * 2.0 ** (-23.0 - 24) * 2.0 ** e
+            x = x.astype(np.float32).view(np.int32) + rng.integers(-1, 2, 127).astype(np.int32)
+            x = x.view(np.float32) * rng.choice([-1.0, 1.0], 127).astype(np.float32)
+            x = np.where(np.abs(x) <= amax[0], x, np.float32(0.0))
+            rows.append(np.concatenate([amax[:1], x]).astype(np.float32))
+    return torch.from_numpy(np.stack(rows))
+
+
+@pytest.mark.parametrize("exponent", [0, -60, -83, -84, -100, -110, 100])
+def test_quantize_rows_nearly_half_quotients(exponent):
+    from rocknpu_b200 import device as dev
+    a = nearly_half_quotients() * 2.0 ** exponent
+    assert a.shape[0] > 500
+    status = dev.new_status()
+    q, s = dev.quantize_rows_f8(a.cuda(), status)
+    want_q, want_s = ref_rows(a)
+    assert status.item() == 0 and torch.equal(s.cpu(), want_s)
+    assert torch.equal(bits(q.cpu()), bits(want_q))
+    q, s = dev.prepare_f8(a[:, None, :].cuda(), status)
+    assert torch.equal(bits(q.cpu()[:, 0]), bits(want_q)) and torch.equal(s.cpu()[:, 0], want_s)
+
+
 def test_quantize_rows_strided_in_and_out():
     """A column slice of a wider matrix into a slice of a wider one; what lies
     beside it stays."""
