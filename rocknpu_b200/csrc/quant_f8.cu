@@ -209,33 +209,31 @@ __global__ void __launch_bounds__(kPrepThreads, sizeof(T) == 4 ? 2 : 4) prep_f8_
     }
 }
 
-constexpr int kKqThreads = 1024;
+constexpr int kKqThreads = 512;
 
-// The values of four superblocks (rows r0 .. r0 + 3 of one superblock column)
-// that a lane owns, 8 each, in dequant8's order.  The sub-blocks' scales and
-// mins of all four are decoded once per warp, a sub-block per lane (Q4_K,
-// Q5_K: 4 x 8; Q6_K: two of 4 x 16 per lane), and handed out by shuffles;
+// The values of half a superblock in four rows that a lane owns, 8 each, in
+// dequant8's order; `at` is the lane's place there (0..15 the first 128
+// values, 16..31 the rest).  A half-warp has a row, rows 2 p and 2 p + 1 of the
+// warp's eight are a warp's step p.  The sub-blocks' scales and mins of all eight
+// rows, four each, are decoded once per warp, one per lane, and handed out by shuffles;
 // dequant8 decodes them in every lane.  The same values, one rounding each.
 template <int KIND>
-__device__ __forceinline__ void dequant4x8(const uint8_t* const (&blk)[4], const bool (&live)[4], int lane,
-                                           float (&v)[4][8]) {
+__device__ __forceinline__ void dequant4x8(const uint8_t* const (&blk)[4], const bool (&live)[4], const uint8_t* mine,
+                                           int lane, int at, float (&v)[4][8]) {
     if constexpr (KIND == kQ4K || KIND == kQ5K) {
-        const int g = lane >> 3, i4 = (lane & 7) * 4;
+        const int g = at >> 3, i4 = (at & 7) * 4;
         uint32_t q[4], h[4];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
             q[p] = live[p] ? ld32(blk[p] + (KIND == kQ4K ? 16 : 48) + 32 * g + i4) : 0u;
             h[p] = KIND == kQ5K && live[p] ? ld32(blk[p] + 16 + i4) : 0u;
         }
-        // this lane's sub-block: j of superblock g
-        const uint8_t* b = g < 2 ? (g == 0 ? blk[0] : blk[1]) : (g == 2 ? blk[2] : blk[3]);
-        const bool on = g < 2 ? (g == 0 ? live[0] : live[1]) : (g == 2 ? live[2] : live[3]);
         float dj = 0.0f, mj = 0.0f;
-        if (on) {
-            const uint32_t dd = ld32(b);
-            const uint32_t s[3] = {ld32(b + 4), ld32(b + 8), ld32(b + 12)};
+        if (mine) {
+            const uint32_t dd = ld32(mine);
+            const uint32_t s[3] = {ld32(mine + 4), ld32(mine + 8), ld32(mine + 12)};
             int sc, mn;
-            scale_min_k4(lane & 7, s, sc, mn);
+            scale_min_k4((at & 16) / 4 + (lane & 3), s, sc, mn);
             dj = __fmul_rn(half_bits_to_float(dd), static_cast<float>(sc));
             mj = __fmul_rn(half_bits_to_float(dd >> 16), static_cast<float>(mn));
         }
@@ -243,8 +241,8 @@ __device__ __forceinline__ void dequant4x8(const uint8_t* const (&blk)[4], const
         for (int p = 0; p < 4; ++p)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const float d = __shfl_sync(0xffffffffu, dj, 8 * p + 2 * g + half);
-                const float m = __shfl_sync(0xffffffffu, mj, 8 * p + 2 * g + half);
+                const int from = 4 * (2 * p + (lane >> 4)) + 2 * (g & 1) + half;
+                const float d = __shfl_sync(0xffffffffu, dj, from), m = __shfl_sync(0xffffffffu, mj, from);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint32_t c = (q[p] >> (8 * i + 4 * half)) & 0x0Fu;
@@ -256,7 +254,7 @@ __device__ __forceinline__ void dequant4x8(const uint8_t* const (&blk)[4], const
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
             if (live[p]) {
-                dequant8<KIND>(blk[p], lane, [&](int slot, int, float x) { v[p][slot] = x; });
+                dequant8<KIND>(blk[p], at, [&](int slot, int, float x) { v[p][slot] = x; });
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[p][i] = 0.0f;
@@ -265,54 +263,56 @@ __device__ __forceinline__ void dequant4x8(const uint8_t* const (&blk)[4], const
     }
 }
 
-// K-quant superblocks: one CTA per 128 rows of one superblock column (two
-// 128 x 128 blocks).  A warp dequantises 4 superblocks, 8 values per lane;
-// lanes 0-15 own the first 128 values of a superblock, lanes 16-31 the rest.
+// K-quant superblocks: one CTA per 128 x 128 block, 128 rows of half a
+// superblock column.  Bound by its arithmetic, with HBM waiting (5632 x 2048:
+// Q4_K 11.8 us, Q5_K 14.3, Q6_K 14.9), so several CTAs share an SM and some
+// compute while others load; one of 1024 threads per superblock column was alone there
+// and took 15.4, 17.3 and 18.6.  Three CTAs spill: faster for Q6_K only (two: 16.3).
 template <int KIND>
-__global__ void __launch_bounds__(kKqThreads) prep_f8_kq_kernel(const uint8_t* __restrict__ blocks, int n,
-                                                                unsigned sb, uint8_t* __restrict__ out,
-                                                                long long ld8, float* __restrict__ scales, int* err) {
+__global__ void __launch_bounds__(kKqThreads, KIND == kQ6K ? 3 : 2)
+    prep_f8_kq_kernel(const uint8_t* __restrict__ blocks, int n, unsigned sb, uint8_t* __restrict__ out, long long ld8,
+                      float* __restrict__ scales, int* err) {
     constexpr int kBytes = KIND == kQ4K ? 144 : KIND == kQ5K ? 176 : 210;
-    __shared__ uint32_t red[2][kKqThreads / 32];
-    const unsigned rb = blockIdx.x / sb, cb = blockIdx.x - rb * sb;
+    __shared__ uint32_t red[kKqThreads / 32];
+    const unsigned rb = blockIdx.x / (2 * sb), half_col = blockIdx.x - rb * 2 * sb, cb = half_col >> 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long r0 = static_cast<long long>(rb) * kF8Block + warp * 4;
+    const int at = static_cast<int>(half_col & 1) * 16 + (lane & 15);
+    const long long r0 = static_cast<long long>(rb) * kF8Block + warp * 8;
     const uint8_t* blk[4];
     bool live[4];
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-        live[p] = r0 + p < n;
-        blk[p] = blocks + ((r0 + p) * sb + cb) * kBytes;
+        const long long r = r0 + 2 * p + (lane >> 4);
+        live[p] = r < n;
+        blk[p] = blocks + (r * sb + cb) * kBytes;
     }
+    const long long rs = r0 + (lane >> 2);
     float v[4][8];
-    dequant4x8<KIND>(blk, live, lane, v);
+    dequant4x8<KIND>(blk, live, rs < n ? blocks + (rs * sb + cb) * kBytes : nullptr, lane, at, v);
     uint32_t m = 0;
 #pragma unroll
     for (int p = 0; p < 4; ++p) m = max(m, mag_max(v[p]));
-    m = half_warp_max(m);
-    if (!mag_finite(m)) atomicExch(err, kErrNonFinite);
-    static_assert(kKqThreads / 32 == 32, "two maxima per lane below");
-    if ((lane & 15) == 0) red[lane >> 4][warp] = m;
-    __syncthreads();
-    // two reads of 16 maxima by each half-warp, then a shuffle
-    const float s = f8_scale(__uint_as_float(half_warp_max(max(red[lane >> 4][lane & 15], red[lane >> 4][16 + (lane & 15)]))));
-    if (warp == 0 && (lane & 15) == 0)
-        scales[static_cast<long long>(rb) * 2 * sb + 2 * cb + (lane >> 4)] = s;
+    m = cta_max<kKqThreads>(m, red);
+    const float s = f8_scale(__uint_as_float(m));
+    if (threadIdx.x == 0) {
+        if (!mag_finite(m)) atomicExch(err, kErrNonFinite);
+        scales[blockIdx.x] = s;
+    }
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
         if (!live[p]) continue;
-        uint8_t* dst = out + (r0 + p) * ld8 + cb * 256;
+        uint8_t* dst = out + (r0 + 2 * p + (lane >> 4)) * ld8 + cb * 256;
         uint32_t code[2];
         f8_codes(v[p], s, code);
         if constexpr (KIND == kQ6K) {
             // slots t and 4 + t are neighbours
-            const int base = 128 * (lane >> 4) + (lane & 15) * 2;
+            const int base = 128 * (at >> 4) + (at & 15) * 2;
 #pragma unroll
             for (int t = 0; t < 4; ++t)
                 *reinterpret_cast<uint16_t*>(dst + base + 32 * t) =
                     static_cast<uint16_t>(__byte_perm(code[0], code[1], t | ((4 + t) << 4)));
         } else {
-            const int base = 64 * (lane >> 3) + (lane & 7) * 4;
+            const int base = 64 * (at >> 3) + (at & 7) * 4;
             *reinterpret_cast<uint32_t*>(dst + base) = code[0];
             *reinterpret_cast<uint32_t*>(dst + base + 32) = code[1];
         }
@@ -358,7 +358,7 @@ int launch_prep_f8(int type, const void* w, int n, int k, long long ldw, int cou
 int launch_prep_f8_kq(int kind, const uint8_t* blocks, int n, int k, uint8_t* out, long long ld8, float* scales,
                       int* err, cudaStream_t s) {
     const unsigned sb = static_cast<unsigned>(k / 256), nb = (n + kF8Block - 1) / kF8Block;
-    const unsigned long long grid = static_cast<unsigned long long>(nb) * sb;
+    const unsigned long long grid = static_cast<unsigned long long>(nb) * sb * 2;
     if (grid > 0x7fffffffull) return cudaErrorInvalidValue;
     const unsigned g = static_cast<unsigned>(grid);
     switch (kind) {
