@@ -2,9 +2,11 @@
 // rows (a scale per row and 128 columns) and weights (a scale per 128 x 128
 // block), dense or from ggml K-quant superblocks.
 //
-// All are byte streams bound by HBM: each value is read once, held in
-// registers while its block's largest magnitude is found (warp shuffles, for
-// a 128 x 128 block also shared memory), and its code written once.
+// All are byte streams: each value is read once, held in registers while its
+// block's largest magnitude is found (warp shuffles, for a 128 x 128 block
+// also shared memory), and its code written once.  What bounds them is the
+// arithmetic of a code (an SM issues in about three of four cycles): maximum,
+// quotient, conversion, and for K-quants the decoding.
 #include <algorithm>
 
 #include "f8.cuh"
@@ -17,7 +19,7 @@ namespace {
 
 constexpr int kRowsThreads = 256;
 constexpr int kRowsUnroll = 2;  // blocks of 128 per half-warp and step
-constexpr int kRowsCtas = 4;  // per SM (bf16 16384 x 8192: 4 97 us, 5 101, 6 105)
+constexpr int kRowsCtas = 4;  // per SM (bf16 16384 x 8192: 4 84 us, 5 85)
 
 __device__ __forceinline__ uint32_t half_warp_max(uint32_t v) {
 #pragma unroll
@@ -77,8 +79,11 @@ struct At {
 // A half-warp per kRowsUnroll consecutive blocks, 8 consecutive values per
 // lane and block; a step's loads are issued before the step before it is
 // quantised.  Triggers the dependent product at its start: that reads nothing
-// of this kernel's before its own wait.
-template <class T, bool VEC>
+// of this kernel's before its own wait.  WHOLE (and VEC): k is a multiple of
+// kRowsUnroll blocks, so a step's blocks are whole and neighbours in a row, with one
+// address for all: the kernel is bound by its instructions (bf16 16384 x 8192
+// 84 us, 4.9 TB/s; 97 with an address and bounds for each block).
+template <class T, bool VEC, bool WHOLE>
 __global__ void __launch_bounds__(kRowsThreads, kRowsCtas)
     rows_f8_kernel(const T* __restrict__ a, int k, long long lda, unsigned kb, unsigned blocks,
                    uint8_t* __restrict__ out, long long ld8, float* __restrict__ scales, long long lds, int* err) {
@@ -90,13 +95,24 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtas)
     step.set(gridDim.x * (kRowsThreads / 16) * U, kb);
     at.set((blockIdx.x * (kRowsThreads / 16) + (threadIdx.x >> 4)) * U, kb);
     auto load = [&](At p, Raw8<T>(&v)[U]) {
+        if constexpr (WHOLE) {
+            const T* row = a + p.r * lda + p.c * kF8Block + lane * 8;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (p.b < blocks)
-                row_load8<T, VEC>(a + p.r * lda, static_cast<int>(p.c) * kF8Block + lane * 8, k, v[u]);
-            else
-                v[u].clear();
-            p.on(one, kb);
+            for (int u = 0; u < U; ++u) {
+                if (p.b < blocks)
+                    v[u].load(row + u * kF8Block);
+                else
+                    v[u].clear();
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (p.b < blocks)
+                    row_load8<T, VEC>(a + p.r * lda, static_cast<int>(p.c) * kF8Block + lane * 8, k, v[u]);
+                else
+                    v[u].clear();
+                p.on(one, kb);
+            }
         }
     };
     Raw8<T> cur[U];
@@ -115,11 +131,21 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtas)
             const uint32_t m = half_warp_max(cur[u].mag_max());
             most = max(most, m);
             const float s = f8_scale(__uint_as_float(m));
-            if (at.b < blocks) {
-                row_store8<VEC>(out + at.r * ld8, static_cast<int>(at.c) * kF8Block + lane * 8, k, v, s);
-                if (lane == 0) scales[at.r * lds + at.c] = s;
+            if constexpr (WHOLE) {
+                uint32_t code[2];
+                f8_codes(v, s, code);
+                if (at.b < blocks) {
+                    *reinterpret_cast<uint2*>(out + at.r * ld8 + at.c * kF8Block + lane * 8 + u * kF8Block) =
+                        make_uint2(code[0], code[1]);
+                    if (lane == 0) scales[at.r * lds + at.c + u] = s;
+                }
+            } else {
+                if (at.b < blocks) {
+                    row_store8<VEC>(out + at.r * ld8, static_cast<int>(at.c) * kF8Block + lane * 8, k, v, s);
+                    if (lane == 0) scales[at.r * lds + at.c] = s;
+                }
+                at.on(one, kb);
             }
-            at.on(one, kb);
             cur[u] = next[u];
         }
         at = then;
@@ -137,16 +163,19 @@ int rows_f8(const T* a, int m, int k, long long lda, uint8_t* out, long long ld8
     const unsigned grid = static_cast<unsigned>(std::min<unsigned long long>((total + per - 1) / per, sm_count() * kRowsCtas));
     const bool vec = (reinterpret_cast<uintptr_t>(a) % 16 == 0) && (lda * sizeof(T)) % 16 == 0 &&
                      (reinterpret_cast<uintptr_t>(out) % 8 == 0) && ld8 % 8 == 0;
-    auto kern = vec ? rows_f8_kernel<T, true> : rows_f8_kernel<T, false>;
+    const int kind = !vec ? 0 : k % (kRowsUnroll * kF8Block) == 0 ? 2 : 1;
+    auto kern = kind == 0 ? rows_f8_kernel<T, false, false>
+                : kind == 1 ? rows_f8_kernel<T, true, false>
+                            : rows_f8_kernel<T, true, true>;
     // the max-shared carveout, so that the dependent product's CTA (about
     // 200 KB of shared memory) becomes resident beside these; a long run is no
     // slower with it
-    static bool carve[64][2] = {};
+    static bool carve[64][3] = {};
     int dev = 0;
     cudaGetDevice(&dev);
-    if (dev >= 0 && dev < 64 && !carve[dev][vec]) {
+    if (dev >= 0 && dev < 64 && !carve[dev][kind]) {
         cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-        carve[dev][vec] = true;
+        carve[dev][kind] = true;
     }
     kern<<<grid, kRowsThreads, 0, s>>>(a, k, lda, kb, static_cast<unsigned>(total), out, ld8, scales, lds, err);
     return cudaGetLastError();
@@ -155,6 +184,7 @@ int rows_f8(const T* a, int m, int k, long long lda, uint8_t* out, long long ld8
 // ---- 128 x 128 weight blocks ----------------------------------------------
 
 constexpr int kPrepThreads = 256;
+constexpr int kPrepRows = kPrepThreads / 16, kPrepPasses = kF8Block / kPrepRows;
 
 template <int THREADS>
 __device__ __forceinline__ uint32_t cta_max(uint32_t v, uint32_t* red) {
@@ -167,13 +197,15 @@ __device__ __forceinline__ uint32_t cta_max(uint32_t v, uint32_t* red) {
     return r;
 }
 
-// One CTA per block: 16 lanes of 8 values per row, 16 rows per pass, 8 passes
-// held in registers.
-template <class T, bool VEC>
-__global__ void __launch_bounds__(kPrepThreads, sizeof(T) == 4 ? 2 : 4) prep_f8_dense_kernel(const T* __restrict__ w, int n, int k,
-                                                                     long long ldw, unsigned nb, unsigned kb,
-                                                                     uint8_t* __restrict__ out, long long ld8,
-                                                                     float* __restrict__ scales, int* err) {
+// One CTA per block: 16 lanes of 8 values per row, kPrepRows rows per pass, all
+// passes held in registers.
+// WHOLE (and VEC): every block is, and nothing is asked of bounds (bf16, 8 of
+// 5632 x 2048: 55 us, 5.0 TB/s; 58.6 without).  CTAs per SM as the registers
+// hold the passes: WHOLE with four spills, 69 us; two of 512 threads 63.
+template <class T, bool VEC, bool WHOLE>
+__global__ void __launch_bounds__(kPrepThreads, sizeof(T) == 4 ? 2 : WHOLE ? 3 : 4)
+    prep_f8_dense_kernel(const T* __restrict__ w, int n, int k, long long ldw, unsigned nb, unsigned kb,
+                         uint8_t* __restrict__ out, long long ld8, float* __restrict__ scales, int* err) {
     __shared__ uint32_t red[kPrepThreads / 32];
     const unsigned per = nb * kb;
     const unsigned mat = blockIdx.x / per, b = blockIdx.x - mat * per;
@@ -182,18 +214,20 @@ __global__ void __launch_bounds__(kPrepThreads, sizeof(T) == 4 ? 2 : 4) prep_f8_
     const int row0 = static_cast<int>(rb) * kF8Block + (threadIdx.x >> 4);
     w += static_cast<long long>(mat) * n * ldw;
     out += static_cast<long long>(mat) * n * ld8;
-    Raw8<T> raw[8];
+    Raw8<T> raw[kPrepPasses];
 #pragma unroll
-    for (int p = 0; p < 8; ++p) {
-        const int r = row0 + 16 * p;
-        if (r < n)
+    for (int p = 0; p < kPrepPasses; ++p) {
+        const int r = row0 + kPrepRows * p;
+        if constexpr (WHOLE)
+            raw[p].load(w + r * ldw + col);
+        else if (r < n)
             row_load8<T, VEC>(w + r * ldw, col, k, raw[p]);
         else
             raw[p].clear();
     }
     uint32_t m = 0;
 #pragma unroll
-    for (int p = 0; p < 8; ++p) m = max(m, raw[p].mag_max());
+    for (int p = 0; p < kPrepPasses; ++p) m = max(m, raw[p].mag_max());
     m = cta_max<kPrepThreads>(m, red);
     const float s = f8_scale(__uint_as_float(m));
     if (threadIdx.x == 0) {
@@ -201,11 +235,17 @@ __global__ void __launch_bounds__(kPrepThreads, sizeof(T) == 4 ? 2 : 4) prep_f8_
         scales[blockIdx.x] = s;
     }
 #pragma unroll
-    for (int p = 0; p < 8; ++p) {
-        const int r = row0 + 16 * p;
+    for (int p = 0; p < kPrepPasses; ++p) {
+        const int r = row0 + kPrepRows * p;
         float v[8];
         raw[p].values(v);
-        if (r < n) row_store8<VEC>(out + r * ld8, col, k, v, s);
+        if constexpr (WHOLE) {
+            uint32_t code[2];
+            f8_codes(v, s, code);
+            *reinterpret_cast<uint2*>(out + r * ld8 + col) = make_uint2(code[0], code[1]);
+        } else {
+            if (r < n) row_store8<VEC>(out + r * ld8, col, k, v, s);
+        }
     }
 }
 
@@ -327,7 +367,9 @@ int prep_dense(const T* w, int n, int k, long long ldw, int count, uint8_t* out,
     if (grid > 0x7fffffffull) return cudaErrorInvalidValue;
     const bool vec = (reinterpret_cast<uintptr_t>(w) % 16 == 0) && (ldw * sizeof(T)) % 16 == 0 &&
                      (reinterpret_cast<uintptr_t>(out) % 8 == 0) && ld8 % 8 == 0;
-    auto kern = vec ? prep_f8_dense_kernel<T, true> : prep_f8_dense_kernel<T, false>;
+    auto kern = !vec                              ? prep_f8_dense_kernel<T, false, false>
+                : n % kF8Block || k % kF8Block ? prep_f8_dense_kernel<T, true, false>
+                                               : prep_f8_dense_kernel<T, true, true>;
     kern<<<static_cast<unsigned>(grid), kPrepThreads, 0, s>>>(w, n, k, ldw, nb, kb, out, ld8, scales, err);
     return cudaGetLastError();
 }
