@@ -259,7 +259,7 @@ constexpr int kKqThreads = 512;
 // dequant8 decodes them in every lane.  The same values, one rounding each.
 template <int KIND>
 __device__ __forceinline__ void dequant4x8(const uint8_t* const (&blk)[4], const bool (&live)[4], const uint8_t* mine,
-                                           int lane, int at, float (&v)[4][8]) {
+                                           bool on, int lane, int at, float (&v)[4][8]) {
     if constexpr (KIND == kQ4K || KIND == kQ5K) {
         const int g = at >> 3, i4 = (at & 7) * 4;
         uint32_t q[4], h[4];
@@ -269,7 +269,7 @@ __device__ __forceinline__ void dequant4x8(const uint8_t* const (&blk)[4], const
             h[p] = KIND == kQ5K && live[p] ? ld32(blk[p] + 16 + i4) : 0u;
         }
         float dj = 0.0f, mj = 0.0f;
-        if (mine) {
+        if (on) {
             const uint32_t dd = ld32(mine);
             const uint32_t s[3] = {ld32(mine + 4), ld32(mine + 8), ld32(mine + 12)};
             int sc, mn;
@@ -305,10 +305,12 @@ __device__ __forceinline__ void dequant4x8(const uint8_t* const (&blk)[4], const
 
 // K-quant superblocks: one CTA per 128 x 128 block, 128 rows of half a
 // superblock column.  Bound by its arithmetic, with HBM waiting (5632 x 2048:
-// Q4_K 11.8 us, Q5_K 14.3, Q6_K 14.9), so several CTAs share an SM and some
-// compute while others load; one of 1024 threads per superblock column was alone there
-// and took 15.4, 17.3 and 18.6.  Three CTAs spill: faster for Q6_K only (two: 16.3).
-template <int KIND>
+// Q4_K 10.8 us, Q5_K 13.1, Q6_K 13.3), so several CTAs share an SM and some
+// compute while others load; one of 1024 threads per superblock column was
+// alone there and took 15.4, 17.3 and 18.6.  Three CTAs spill: faster for Q6_K
+// only (n not a multiple of 128: 14.9, two 16.3).
+// WHOLE: n is a multiple of 128.
+template <int KIND, bool WHOLE>
 __global__ void __launch_bounds__(kKqThreads, KIND == kQ6K ? 3 : 2)
     prep_f8_kq_kernel(const uint8_t* __restrict__ blocks, int n, unsigned sb, uint8_t* __restrict__ out, long long ld8,
                       float* __restrict__ scales, int* err) {
@@ -323,12 +325,12 @@ __global__ void __launch_bounds__(kKqThreads, KIND == kQ6K ? 3 : 2)
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
         const long long r = r0 + 2 * p + (lane >> 4);
-        live[p] = r < n;
+        live[p] = WHOLE || r < n;
         blk[p] = blocks + (r * sb + cb) * kBytes;
     }
     const long long rs = r0 + (lane >> 2);
     float v[4][8];
-    dequant4x8<KIND>(blk, live, rs < n ? blocks + (rs * sb + cb) * kBytes : nullptr, lane, at, v);
+    dequant4x8<KIND>(blk, live, blocks + (rs * sb + cb) * kBytes, WHOLE || rs < n, lane, at, v);
     uint32_t m = 0;
 #pragma unroll
     for (int p = 0; p < 4; ++p) m = max(m, mag_max(v[p]));
@@ -374,6 +376,14 @@ int prep_dense(const T* w, int n, int k, long long ldw, int count, uint8_t* out,
     return cudaGetLastError();
 }
 
+template <int KIND>
+int prep_kq(const uint8_t* blocks, int n, unsigned sb, unsigned grid, uint8_t* out, long long ld8, float* scales, int* err,
+            cudaStream_t s) {
+    auto kern = n % kF8Block == 0 ? prep_f8_kq_kernel<KIND, true> : prep_f8_kq_kernel<KIND, false>;
+    kern<<<grid, kKqThreads, 0, s>>>(blocks, n, sb, out, ld8, scales, err);
+    return cudaGetLastError();
+}
+
 }  // namespace
 
 int launch_quant_rows_f8(int type, const void* a, int m, int k, long long lda, uint8_t* out, long long ld8,
@@ -404,12 +414,11 @@ int launch_prep_f8_kq(int kind, const uint8_t* blocks, int n, int k, uint8_t* ou
     if (grid > 0x7fffffffull) return cudaErrorInvalidValue;
     const unsigned g = static_cast<unsigned>(grid);
     switch (kind) {
-        case kQ4K: prep_f8_kq_kernel<kQ4K><<<g, kKqThreads, 0, s>>>(blocks, n, sb, out, ld8, scales, err); break;
-        case kQ5K: prep_f8_kq_kernel<kQ5K><<<g, kKqThreads, 0, s>>>(blocks, n, sb, out, ld8, scales, err); break;
-        case kQ6K: prep_f8_kq_kernel<kQ6K><<<g, kKqThreads, 0, s>>>(blocks, n, sb, out, ld8, scales, err); break;
+        case kQ4K: return prep_kq<kQ4K>(blocks, n, sb, g, out, ld8, scales, err, s);
+        case kQ5K: return prep_kq<kQ5K>(blocks, n, sb, g, out, ld8, scales, err, s);
+        case kQ6K: return prep_kq<kQ6K>(blocks, n, sb, g, out, ld8, scales, err, s);
         default: return cudaErrorInvalidValue;
     }
-    return cudaGetLastError();
 }
 
 }  // namespace rk
