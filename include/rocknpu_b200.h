@@ -375,7 +375,8 @@ int rocknpu_b200_gemm_f8(const uint8_t *a_f8, size_t ld_a, const float *a_scales
  * rocknpu_b200_quantize_rows_f8 followed by rocknpu_b200_gemm_f8 with a
  * workspace.  `workspace` as above but required, with at least
  * rocknpu_b200_matmul_f8_workspace_bytes bytes (it also holds the quantised
- * activations). */
+ * activations).  No element of out is one of a: a short row is read while
+ * others' results are stored. */
 size_t rocknpu_b200_matmul_f8_workspace_bytes(size_t m, size_t n, size_t k);
 int rocknpu_b200_matmul_f8(const void *a, uint32_t type, size_t lda, const uint8_t *w_f8, size_t ld_w,
                            const float *w_scales, void *out, uint32_t out_type, size_t ldo, size_t m, size_t k,

@@ -347,7 +347,8 @@ def gemm_f8(a8: torch.Tensor, a_scales: torch.Tensor, w8: torch.Tensor, w_scales
 def matmul_f8(a: torch.Tensor, w8: torch.Tensor, w_scales: torch.Tensor, status: torch.Tensor,
               workspace: torch.Tensor, out: torch.Tensor | None = None, out_dtype=None, stream=None) -> torch.Tensor:
     """quantize_rows_f8 + gemm_f8: f32 / f16 / bf16 a [m, k] times a prepared
-    weight; the result has a's type unless `out` or `out_dtype` says another.
+    weight; the result has a's type unless `out` or `out_dtype` says another
+    (`out` is apart from `a`).
     `workspace` (new_workspace of matmul_f8_workspace_bytes) is kept by the
     caller, one per stream on which calls may be in flight."""
     dev = _device_of(a, w8, w_scales, status, workspace, out)
