@@ -79,11 +79,12 @@ struct At {
 // A half-warp per kRowsUnroll consecutive blocks, 8 consecutive values per
 // lane and block; a step's loads are issued before the step before it is
 // quantised.  Triggers the dependent product at its start: that reads nothing
-// of this kernel's before its own wait.  WHOLE (and VEC): k is a multiple of
+// of this kernel's before its own wait.  VEC, VOUT: rows can be read
+// 16 bytes, codes written 8 bytes at a time.  WHOLE (and both): k is a multiple of
 // kRowsUnroll blocks, so a step's blocks are whole and neighbours in a row, with one
 // address for all: the kernel is bound by its instructions (bf16 16384 x 8192
 // 84 us, 4.9 TB/s; 97 with an address and bounds for each block).
-template <class T, bool VEC, bool WHOLE>
+template <class T, bool VEC, bool VOUT, bool WHOLE>
 __global__ void __launch_bounds__(kRowsThreads, kRowsCtas)
     rows_f8_kernel(const T* __restrict__ a, int k, long long lda, unsigned kb, unsigned blocks,
                    uint8_t* __restrict__ out, long long ld8, float* __restrict__ scales, long long lds, int* err) {
@@ -141,7 +142,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtas)
                 }
             } else {
                 if (at.b < blocks) {
-                    row_store8<VEC>(out + at.r * ld8, static_cast<int>(at.c) * kF8Block + lane * 8, k, v, s);
+                    row_store8<VOUT>(out + at.r * ld8, static_cast<int>(at.c) * kF8Block + lane * 8, k, v, s);
                     if (lane == 0) scales[at.r * lds + at.c] = s;
                 }
                 at.on(one, kb);
@@ -161,16 +162,18 @@ int rows_f8(const T* a, int m, int k, long long lda, uint8_t* out, long long ld8
     if (total > 0xF0000000ull) return cudaErrorInvalidValue;
     const unsigned per = kRowsThreads / 16 * kRowsUnroll;
     const unsigned grid = static_cast<unsigned>(std::min<unsigned long long>((total + per - 1) / per, sm_count() * kRowsCtas));
-    const bool vec = (reinterpret_cast<uintptr_t>(a) % 16 == 0) && (lda * sizeof(T)) % 16 == 0 &&
-                     (reinterpret_cast<uintptr_t>(out) % 8 == 0) && ld8 % 8 == 0;
-    const int kind = !vec ? 0 : k % (kRowsUnroll * kF8Block) == 0 ? 2 : 1;
-    auto kern = kind == 0 ? rows_f8_kernel<T, false, false>
-                : kind == 1 ? rows_f8_kernel<T, true, false>
-                            : rows_f8_kernel<T, true, true>;
+    // rows of odd lengths still have aligned codes
+    const bool vout = reinterpret_cast<uintptr_t>(out) % 8 == 0 && ld8 % 8 == 0;
+    const bool vec = reinterpret_cast<uintptr_t>(a) % 16 == 0 && (lda * sizeof(T)) % 16 == 0 && vout;
+    const int kind = !vout ? 0 : !vec ? 1 : k % (kRowsUnroll * kF8Block) ? 2 : 3;
+    auto kern = kind == 0   ? rows_f8_kernel<T, false, false, false>
+                : kind == 1 ? rows_f8_kernel<T, false, true, false>
+                : kind == 2 ? rows_f8_kernel<T, true, true, false>
+                            : rows_f8_kernel<T, true, true, true>;
     // the max-shared carveout, so that the dependent product's CTA (about
     // 200 KB of shared memory) becomes resident beside these; a long run is no
     // slower with it
-    static bool carve[64][3] = {};
+    static bool carve[64][4] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 0 && dev < 64 && !carve[dev][kind]) {
@@ -199,10 +202,11 @@ __device__ __forceinline__ uint32_t cta_max(uint32_t v, uint32_t* red) {
 
 // One CTA per block: 16 lanes of 8 values per row, kPrepRows rows per pass, all
 // passes held in registers.
-// WHOLE (and VEC): every block is, and nothing is asked of bounds (bf16, 8 of
+// VEC, VOUT: rows can be read 16 bytes, codes written 8 bytes at a time.
+// WHOLE (and both): every block is, and nothing is asked of bounds (bf16, 8 of
 // 5632 x 2048: 55 us, 5.0 TB/s; 58.6 without).  CTAs per SM as the registers
 // hold the passes: WHOLE with four spills, 69 us; two of 512 threads 63.
-template <class T, bool VEC, bool WHOLE>
+template <class T, bool VEC, bool VOUT, bool WHOLE>
 __global__ void __launch_bounds__(kPrepThreads, sizeof(T) == 4 ? 2 : WHOLE ? 3 : 4)
     prep_f8_dense_kernel(const T* __restrict__ w, int n, int k, long long ldw, unsigned nb, unsigned kb,
                          uint8_t* __restrict__ out, long long ld8, float* __restrict__ scales, int* err) {
@@ -244,7 +248,7 @@ __global__ void __launch_bounds__(kPrepThreads, sizeof(T) == 4 ? 2 : WHOLE ? 3 :
             f8_codes(v, s, code);
             *reinterpret_cast<uint2*>(out + r * ld8 + col) = make_uint2(code[0], code[1]);
         } else {
-            if (r < n) row_store8<VEC>(out + r * ld8, col, k, v, s);
+            if (r < n) row_store8<VOUT>(out + r * ld8, col, k, v, s);
         }
     }
 }
@@ -367,11 +371,12 @@ int prep_dense(const T* w, int n, int k, long long ldw, int count, uint8_t* out,
     const unsigned nb = (n + kF8Block - 1) / kF8Block, kb = (k + kF8Block - 1) / kF8Block;
     const unsigned long long grid = static_cast<unsigned long long>(nb) * kb * count;
     if (grid > 0x7fffffffull) return cudaErrorInvalidValue;
-    const bool vec = (reinterpret_cast<uintptr_t>(w) % 16 == 0) && (ldw * sizeof(T)) % 16 == 0 &&
-                     (reinterpret_cast<uintptr_t>(out) % 8 == 0) && ld8 % 8 == 0;
-    auto kern = !vec                              ? prep_f8_dense_kernel<T, false, false>
-                : n % kF8Block || k % kF8Block ? prep_f8_dense_kernel<T, true, false>
-                                               : prep_f8_dense_kernel<T, true, true>;
+    const bool vout = reinterpret_cast<uintptr_t>(out) % 8 == 0 && ld8 % 8 == 0;
+    const bool vec = reinterpret_cast<uintptr_t>(w) % 16 == 0 && (ldw * sizeof(T)) % 16 == 0 && vout;
+    auto kern = !vout                          ? prep_f8_dense_kernel<T, false, false, false>
+                : !vec                         ? prep_f8_dense_kernel<T, false, true, false>
+                : n % kF8Block || k % kF8Block ? prep_f8_dense_kernel<T, true, true, false>
+                                               : prep_f8_dense_kernel<T, true, true, true>;
     kern<<<static_cast<unsigned>(grid), kPrepThreads, 0, s>>>(w, n, k, ldw, nb, kb, out, ld8, scales, err);
     return cudaGetLastError();
 }
