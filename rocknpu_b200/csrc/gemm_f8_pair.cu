@@ -29,6 +29,8 @@
 // that its sums are in TMEM; the epilogue is never more than the two TMEM
 // buffers behind, less than the stages, so it cannot miss a phase.
 //
+// Measured: 4096 x 8192 x 28672 bf16 1015 us with the quantiser, 1.9 PFLOP/s.
+//
 // Bounded waits as in the int8 pair kernel (gemm_pair.cu).
 #include <algorithm>
 
