@@ -403,10 +403,9 @@ typedef struct rocknpu_b200_f8_experts {
  * of zeros, whatever its row of x; an id may occur twice; an id >= experts sets *status to 9
  * (INVALID_ARGUMENT by rocknpu_b200_status_code) and counts as empty.  out may
  * be x.
- * Activations are not quantised: f32 ones (and the hidden values) enter the
- * products with 22 bits relative to the largest of their block of 128 (hidden
- * values: of 16), f16 and bf16 ones exactly, with hidden values of 11 bits;
- * sums are f32.
+ * Activations are not quantised: f32 ones, and the hidden values of every
+ * type, enter the products with 22 bits relative to the largest of their block
+ * of 128 (hidden values: of 16), f16 and bf16 ones exactly; sums are f32.
  * hidden and ffn are multiples of 16, top_k <= 16, experts <= 256. */
 typedef struct rocknpu_b200_moe_f8_args {
     size_t tokens, hidden, ffn, experts, top_k;

@@ -10,12 +10,13 @@
 // Products.  Weights go from TMA stages (128-byte swizzle) to registers,
 // e4m3 -> f16 (exact), into mma.sync m16n8k16 with tokens as the 8 columns.
 // Activations are not quantised: a block of them is scaled by a power of two
-// so that its largest magnitude is in [2^14, 2^15) and held in f16; for f32
-// calls a second f16 holds the remainder (22 bits in all), for f16 / bf16
-// calls the inputs fit one f16 and the hidden values are rounded to 11 bits,
-// finer than the result's own rounding for bf16, the same for f16.  Sums are
-// f32: 128 products per block in the MMA's accumulator, times the weight
-// scale and the activation's power of two, added to f32 totals.
+// so that its largest magnitude is in [2^14, 2^15) and held in f16.  A second
+// f16 holds the remainder, 22 bits in all, of f32 inputs and of the hidden
+// values of every type: rounded to 11 bits they alone moved a f16 result by
+// as much as its own rounding.  f16 / bf16 inputs fit one f16 (but for what is
+// below 2^-39 of their block's largest).  Sums are f32: 128 products per
+// block in the MMA's accumulator, times the weight scale and the activation's
+// power of two, added to f32 totals.
 //
 // k order.  The sum over k may run in any order, so thread (g, t) of a warp
 // takes 32 consecutive bytes 32 t .. of weight row g (two 16-byte reads that
@@ -72,7 +73,8 @@ constexpr int kBoxBytes = kBoxRows * kF8Block;
 constexpr int kGroupBytes = 2 * kBoxBytes;   // gate and up, or two boxes of down rows
 constexpr int kMaxPairs = kMoeMaxTokens * kMoeMaxTop;
 constexpr int kRouterTokens = 4;             // tokens per router task
-constexpr int kMaxParts = 512;               // CTAs of a launch
+constexpr int kMaxParts = 256;               // CTAs of a launch
+constexpr int kMaxEntries = kMoeMaxExperts + kMaxPairs / 8;  // an expert's last entry may be short, the others hold 8 or more
 constexpr uint64_t kHelpNs = 20000;          // wait for the others before taking a further part
 
 // Words of the zeroed header.
@@ -112,18 +114,20 @@ struct ActBlock {
 
 template <int NG, bool LO>
 struct MoeCfg {
-    using Act = ActBlock<LO>;
+    using Act = ActBlock<LO>;    // of x
+    using Hid = ActBlock<true>;  // of hidden values
     static constexpr int kConsumers = 8;  // a group of a pass each; 16 with fewer registers were slower
     static constexpr int kConsThreads = kConsumers * 32;
     static constexpr int kWarps = kConsumers + kProducers;
     static constexpr int kThreads = kWarps * 32;
     // registers after the split: 256 x 224 + 128 x 56 of 384 x 168
     static constexpr int kConsRegs = 224, kProdRegs = 56;
-    static constexpr int kAct = (NG * 8 * Act::kBytes + 1023) / 1024 * 1024;
+    static constexpr int kAct = (NG * 8 * Hid::kBytes + 1023) / 1024 * 1024;  // the larger of the two
     static constexpr int kStage = kPassGroups * kGroupBytes + kAct;
     static constexpr int kRedBytes = kConsThreads * 8 * 4;  // sums that warps exchange
-    static constexpr int kTableBytes = kRedBytes + kMaxPairs * (4 + 4 + 2 + 2) + kMoeMaxExperts * 4 + 16 + kMaxParts * 2;
-    static constexpr int kStages = (230000 - 2048 - kTableBytes) / kStage;
+    static constexpr int kTableBytes =
+        kRedBytes + kMaxPairs * (4 + 2 + 2) + (kMaxEntries + kMoeMaxExperts) * 4 + 16 + kMaxParts * 2;
+    static constexpr int kStages = (232448 - 1024 - 256 - kTableBytes) / kStage;  // 256: barriers
     static constexpr int kBarOffset = kStages * kStage;
     static constexpr int kTables = kBarOffset + (2 * kStages * 8 + 32 + 15) / 16 * 16;
     static constexpr int kBytes = kTables + kTableBytes + 1024;  // + alignment slack
@@ -637,7 +641,7 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t v, __half2 s) {
 template <int NG, bool LO>
 struct Consumer {
     using C = MoeCfg<NG, LO>;
-    using Act = ActBlock<LO>;
+    using Hid = typename C::Hid;
     // gate / up (or the two halves of 32 down rows) x token groups x fragment
     float acc[2][NG][4];
 
@@ -653,12 +657,15 @@ struct Consumer {
     // One block of 128, 64 values (thread t's chunk c of 16) at a time: a
     // group's 16 rows of both boxes times ng token groups.  at: byte of this
     // lane's token's row behind act, per token group.
-    // GROUPED: a scale per 16 values (thread t's two chunks have their own).
-    // PACKED (LO, at most 4 tokens): column 2c is token c's f16 values and
-    // column 2c + 1 their remainders, in one MMA; unpack() adds them.
+    // GROUPED: hidden values, a scale per 16 (thread t's two chunks have their
+    // own) and remainders.
+    // PACKED (remainders, at most 4 tokens): column 2c is token c's f16 values
+    // and column 2c + 1 their remainders, in one MMA; unpack() adds them.
     template <bool GROUPED, bool PACKED>
     __device__ __forceinline__ void block(const uint8_t* rows, const uint8_t* act, const int (&at)[NG], int lane, int ng,
                                           float s0, float s1) {
+        using Act = ActBlock<LO || GROUPED>;
+        constexpr int kTerms = (LO || GROUPED) && !PACKED ? 2 : 1;
         const int g = lane >> 2, t = lane & 3;
         // per token group: the power of two of columns 2t and 2t + 1 (times the
         // weights' scales below), and what brings this lane's chunks to it
@@ -708,7 +715,7 @@ struct Consumer {
                 // take longer than the block's copy
                 float d[2][2][4] = {};
 #pragma unroll
-                for (int part = 0; part < (LO && !PACKED ? 2 : 1); ++part)
+                for (int part = 0; part < kTerms; ++part)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         uint4 v = *reinterpret_cast<const uint4*>(row + (PACKED ? g & 1 : part) * 256 + (2 * c + j) * 64 + t * 16);
@@ -788,16 +795,16 @@ struct Consumer {
                 const float sc = act_scale(m, inv);
                 const int col = i * 8 + 2 * t + j;
                 if (col < n) {
-                    uint8_t* blk = p.hq + (static_cast<long long>(group >> 3) * p.t * p.top + first + col) * Act::kBytes;
+                    uint8_t* blk = p.hq + (static_cast<long long>(group >> 3) * p.t * p.top + first + col) * Hid::kBytes;
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         const float v = h[r] * inv;
                         const __half hi = __float2half_rn(v);
                         const int at = act_at((group & 7) * 16 + g + 8 * r);
                         *reinterpret_cast<__half*>(blk + at) = hi;
-                        if constexpr (LO) *reinterpret_cast<__half*>(blk + 256 + at) = __float2half_rn(v - __half2float(hi));
+                        *reinterpret_cast<__half*>(blk + 256 + at) = __float2half_rn(v - __half2float(hi));
                     }
-                    if (g == 0) reinterpret_cast<float*>(blk + Act::kScaleAt)[group & 7] = sc;
+                    if (g == 0) reinterpret_cast<float*>(blk + Hid::kScaleAt)[group & 7] = sc;
                     // the rest of the last block: zeros
                     if ((group + 1) * kBoxRows == p.f)
                         for (int rest = (group & 7) + 1; rest < 8; ++rest) {
@@ -805,9 +812,9 @@ struct Consumer {
                             for (int r = 0; r < 2; ++r) {
                                 const int at = act_at(rest * 16 + g + 8 * r);
                                 *reinterpret_cast<__half*>(blk + at) = __half(0.0f);
-                                if constexpr (LO) *reinterpret_cast<__half*>(blk + 256 + at) = __half(0.0f);
+                                *reinterpret_cast<__half*>(blk + 256 + at) = __half(0.0f);
                             }
-                            if (g == 0) reinterpret_cast<float*>(blk + Act::kScaleAt)[rest] = 1.17549435e-38f;
+                            if (g == 0) reinterpret_cast<float*>(blk + Hid::kScaleAt)[rest] = 1.17549435e-38f;
                         }
                 }
             }
@@ -880,7 +887,8 @@ __device__ __forceinline__ void combine(const MoeParams& p, const Tables& tb, in
 template <int NG, bool LO>
 __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(const __grid_constant__ MoeParams p) {
     using C = MoeCfg<NG, LO>;
-    using Act = ActBlock<LO>;
+    using Act = typename C::Act;
+    using Hid = typename C::Hid;
     constexpr int S = C::kStages, kCap = NG * 8;
     constexpr int kConsumers = C::kConsumers, kConsThreads = C::kConsThreads, kThreads = C::kThreads, kWarps = C::kWarps;
     extern __shared__ uint8_t smem_raw[];
@@ -893,7 +901,7 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
     tb.red = reinterpret_cast<float*>(smem + C::kTables);
     tb.pair_w = tb.red + C::kRedBytes / 4;
     tb.entry = reinterpret_cast<int*>(tb.pair_w + kMaxPairs);
-    tb.count = tb.entry + kMaxPairs;
+    tb.count = tb.entry + kMaxEntries;
     tb.info = tb.count + kMoeMaxExperts;
     tb.pair_e = reinterpret_cast<short*>(tb.info + 4);
     tb.order = tb.pair_e + kMaxPairs;
@@ -1059,10 +1067,10 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
                         uint8_t* dst = smem + g % S * C::kStage;
                         if (lane != 0) continue;
                         if (pw == kProducers - 1) {
-                            mbar_arrive_expect_tx(bar, s.npos * Act::kBytes);
+                            mbar_arrive_expect_tx(bar, s.npos * Hid::kBytes);
                             bulk_load(dst + kPassGroups * kGroupBytes,
-                                      p.hq + (static_cast<long long>(kb) * p.t * p.top + s.pos0) * Act::kBytes,
-                                      s.npos * Act::kBytes, bar);
+                                      p.hq + (static_cast<long long>(kb) * p.t * p.top + s.pos0) * Hid::kBytes,
+                                      s.npos * Hid::kBytes, bar);
                         } else {
                             mbar_arrive_expect_tx(bar, bytes);
 #pragma unroll
@@ -1105,7 +1113,7 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
                     int first, n;
                     entry_pairs(tb, entry, kCap, first, n);
                     const int ng = (n + 7) / 8, ex = tb.entry[entry] >> 16;
-                    const bool packed = n <= 4;
+                    const bool packed = NG == 1 && n <= 4 && (LO || phase == 2);
                     const float *s0, *s1;
                     if (phase == 1) {
                         s0 = p.gate_s + ex * p.gate_ss + static_cast<long long>(group >> 3) * p.kb_h;
@@ -1118,8 +1126,9 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
 #pragma unroll
                     for (int i = 0; i < NG; ++i) {
                         // columns behind the last token repeat it; nothing of them is kept
-                        const int col = min(LO && NG == 1 && packed ? lane >> 3 : i * 8 + (lane >> 2), n - 1);
-                        row_at[i] = (phase == 1 && p.t <= 8 ? tb.order[first + col] / p.top : first - s.pos0 + col) * Act::kBytes;
+                        const int col = min(packed ? lane >> 3 : i * 8 + (lane >> 2), n - 1);
+                        row_at[i] = (phase == 1 && p.t <= 8 ? tb.order[first + col] / p.top : first - s.pos0 + col) *
+                                    (phase == 1 ? Act::kBytes : Hid::kBytes);
                     }
                     c.clear();
                     float w0 = __ldg(s0 + min(s.k0 + way, s.k1 - 1)), w1 = __ldg(s1 + min(s.k0 + way, s.k1 - 1));
@@ -1136,15 +1145,16 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
                             const float n0 = __ldg(s0 + nk), n1 = __ldg(s1 + nk);
                             const uint8_t* at = smem + st * C::kStage;
                             const uint8_t *rows = at + gi * kGroupBytes, *act = at + kPassGroups * kGroupBytes;
-                            if (LO && NG == 1 && packed) {
-                                if (phase == 1)
-                                    c.template block<false, true>(rows, act, row_at, lane, ng, w0, w1);
+                            if (phase == 1) {
+                                if (LO && NG == 1 && packed)
+                                    c.template block<false, LO && NG == 1>(rows, act, row_at, lane, ng, w0, w1);
                                 else
-                                    c.template block<true, true>(rows, act, row_at, lane, ng, w0, w1);
-                            } else if (phase == 1) {
-                                c.template block<false, false>(rows, act, row_at, lane, ng, w0, w1);
+                                    c.template block<false, false>(rows, act, row_at, lane, ng, w0, w1);
                             } else {
-                                c.template block<true, false>(rows, act, row_at, lane, ng, w0, w1);
+                                if (NG == 1 && packed)
+                                    c.template block<true, NG == 1>(rows, act, row_at, lane, ng, w0, w1);
+                                else
+                                    c.template block<true, false>(rows, act, row_at, lane, ng, w0, w1);
                             }
                             w0 = n0;
                             w1 = n1;
@@ -1157,7 +1167,7 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
                         ok = false;
                         break;
                     }
-                    if (LO && NG == 1 && packed) c.unpack(lane);
+                    if (packed) c.unpack(lane);
                     if (ways > 1) c.reduce(tb.red, warp, lane, (min(s.npos, kCap) + 7) / 8, n2, ways);
                     const bool owner = mine && way == 0;
                     if (phase == 1) {
@@ -1229,12 +1239,12 @@ int split_limit(int pairs) { return std::max(1, std::min(8, 256 / pairs)); }
 struct MoeScratch {
     size_t logits, xq, hq, pair_out, total;
     MoeScratch(int t, int h, int f, int e, int top, int type) {
-        const size_t blk = type == kTypeF32 ? ActBlock<true>::kBytes : ActBlock<false>::kBytes;
+        const size_t blk = type == kTypeF32 ? ActBlock<true>::kBytes : ActBlock<false>::kBytes, hid = ActBlock<true>::kBytes;
         const size_t kb_h = (h + 127) / 128, kb_f = (f + 127) / 128, pairs = static_cast<size_t>(t) * top;
         logits = 0;
         xq = logits + up256(static_cast<size_t>(t) * e * 4);
         hq = xq + up256(t * kb_h * blk);
-        pair_out = hq + up256(pairs * kb_f * blk);
+        pair_out = hq + up256(pairs * kb_f * hid);
         total = pair_out + pairs * split_limit(static_cast<int>(pairs)) * h * 4;
     }
 };
