@@ -32,8 +32,10 @@
 // a 10 us layer).  A part runs in passes of up to 8 groups, one per warp;
 // with fewer, warps share a group's blocks and add through shared memory.
 // Hidden values are scaled per group of 16; the down product brings the
-// eight groups of a block to the block's largest scale as it reads them
-// (exact but for bits 2^-39 below the block's largest value).
+// eight groups of a block to the block's largest scale as it reads them.  A
+// group whose scale is less than 2^-14 of that would lose its last bits in
+// f16, or all of them; the block's products are then run again for such
+// groups alone, brought to the largest scale among them.
 //
 // The down product may also cut k (a part's groups then divide more evenly);
 // its sums go to memory per slot and cut, and are added in a fixed order at
@@ -75,6 +77,7 @@ constexpr int kMaxPairs = kMoeMaxTokens * kMoeMaxTop;
 constexpr int kRouterTokens = 4;             // tokens per router task
 constexpr int kMaxParts = 256;               // CTAs of a launch
 constexpr int kMaxEntries = kMoeMaxExperts + kMaxPairs / 8;  // an expert's last entry may be short, the others hold 8 or more
+constexpr float kNear = 1.0f / 16384.0f;     // hidden groups of a pass: from the largest scale down to this part of it
 constexpr uint64_t kHelpNs = 20000;          // wait for the others before taking a further part
 
 // Words of the zeroed header.
@@ -235,9 +238,8 @@ __device__ __forceinline__ void store_dense(void* p, int type, long long i, floa
         static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
-// Power of two s with amax / s in [2^14, 2^15), at least 2^-126 (zeros too:
-// next to other groups of a block theirs must not be the largest scale), and
-// its exact reciprocal.
+// Power of two s with amax / s in [2^14, 2^15), at least 2^-126 (zeros too),
+// and its exact reciprocal.
 __device__ __forceinline__ float act_scale(float amax, float& inv) {
     const uint32_t ex = (__float_as_uint(amax) >> 23) & 0xFFu;
     const uint32_t se = ex > 15u ? ex - 14u : 1u;
@@ -661,9 +663,12 @@ struct Consumer {
     // own) and remainders.
     // PACKED (remainders, at most 4 tokens): column 2c is token c's f16 values
     // and column 2c + 1 their remainders, in one MMA; unpack() adds them.
+    // A pass takes the groups of at least 2^-14 of the largest scale among those
+    // whose bit of `left` is set (two per token group), and clears their bits;
+    // returns whether any lane has groups left.
     template <bool GROUPED, bool PACKED>
-    __device__ __forceinline__ void block(const uint8_t* rows, const uint8_t* act, const int (&at)[NG], int lane, int ng,
-                                          float s0, float s1) {
+    __device__ __forceinline__ bool block(const uint8_t* rows, const uint8_t* act, const int (&at)[NG], int lane, int ng,
+                                          float s0, float s1, uint32_t& left) {
         using Act = ActBlock<LO || GROUPED>;
         constexpr int kTerms = (LO || GROUPED) && !PACKED ? 2 : 1;
         const int g = lane >> 2, t = lane & 3;
@@ -678,18 +683,25 @@ struct Consumer {
             float xs;
             if constexpr (GROUPED) {
                 const float2 s = *reinterpret_cast<const float2*>(row + Act::kScaleAt + t * 8);
-                xs = fmaxf(s.x, s.y);
+                const float u = left >> (2 * n) & 1 ? s.x : 0.0f, v = left >> (2 * n) & 2 ? s.y : 0.0f;
+                xs = fmaxf(u, v);
                 xs = fmaxf(xs, __shfl_xor_sync(0xffffffffu, xs, 1));
                 xs = fmaxf(xs, __shfl_xor_sync(0xffffffffu, xs, 2));
-                const float inv = __uint_as_float((254u << 23) - __float_as_uint(xs));  // powers of two, at most 2^114
-                f[n][0] = __float2half2_rn(s.x * inv);
-                f[n][1] = __float2half2_rn(s.y * inv);
+                const float least = xs * kNear;
+                const float inv = __uint_as_float((254u << 23) - __float_as_uint(xs));  // powers of two, scales at most 2^114
+                // a group of zeros, of scale 0, counts as taken
+                const bool far0 = u > 0.0f && u < least, far1 = v > 0.0f && v < least;
+                f[n][0] = __float2half2_rn(far0 ? 0.0f : u * inv);
+                f[n][1] = __float2half2_rn(far1 ? 0.0f : v * inv);
+                if (!far0) left &= ~(1u << (2 * n));
+                if (!far1) left &= ~(2u << (2 * n));
             } else {
                 xs = *reinterpret_cast<const float*>(row + Act::kScaleAt);
             }
             x0[n] = __shfl_sync(0xffffffffu, xs, 8 * t);
             x1[n] = __shfl_sync(0xffffffffu, xs, 8 * t + 4);
         }
+        const bool more = GROUPED && __any_sync(0xffffffffu, left != 0u);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             uint32_t a[2][4][4];  // box, k step, fragment
@@ -738,6 +750,7 @@ struct Consumer {
                 }
             }
         }
+        return more;
     }
 
     // PACKED sums to the plain layout: token c = 2t + j in thread t's column j.
@@ -792,7 +805,8 @@ struct Consumer {
                 float m = fmaxf(fabsf(h[0]), fabsf(h[1])), inv;
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                const float sc = act_scale(m, inv);
+                float sc = act_scale(m, inv);
+                if (m == 0.0f) sc = 0.0f;  // zeros ask for no further pass
                 const int col = i * 8 + 2 * t + j;
                 if (col < n) {
                     uint8_t* blk = p.hq + (static_cast<long long>(group >> 3) * p.t * p.top + first + col) * Hid::kBytes;
@@ -814,7 +828,7 @@ struct Consumer {
                                 *reinterpret_cast<__half*>(blk + at) = __half(0.0f);
                                 *reinterpret_cast<__half*>(blk + 256 + at) = __half(0.0f);
                             }
-                            if (g == 0) reinterpret_cast<float*>(blk + Hid::kScaleAt)[rest] = 1.17549435e-38f;
+                            if (g == 0) reinterpret_cast<float*>(blk + Hid::kScaleAt)[rest] = 0.0f;
                         }
                 }
             }
@@ -1145,16 +1159,16 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
                             const float n0 = __ldg(s0 + nk), n1 = __ldg(s1 + nk);
                             const uint8_t* at = smem + st * C::kStage;
                             const uint8_t *rows = at + gi * kGroupBytes, *act = at + kPassGroups * kGroupBytes;
+                            uint32_t left = (1u << 2 * ng) - 1u;  // hidden groups still to be added
                             if (phase == 1) {
                                 if (LO && NG == 1 && packed)
-                                    c.template block<false, LO && NG == 1>(rows, act, row_at, lane, ng, w0, w1);
+                                    c.template block<false, LO && NG == 1>(rows, act, row_at, lane, ng, w0, w1, left);
                                 else
-                                    c.template block<false, false>(rows, act, row_at, lane, ng, w0, w1);
+                                    c.template block<false, false>(rows, act, row_at, lane, ng, w0, w1, left);
+                            } else if (NG == 1 && packed) {
+                                while (c.template block<true, NG == 1>(rows, act, row_at, lane, ng, w0, w1, left)) {}
                             } else {
-                                if (NG == 1 && packed)
-                                    c.template block<true, NG == 1>(rows, act, row_at, lane, ng, w0, w1);
-                                else
-                                    c.template block<true, false>(rows, act, row_at, lane, ng, w0, w1);
+                                while (c.template block<true, false>(rows, act, row_at, lane, ng, w0, w1, left)) {}
                             }
                             w0 = n0;
                             w1 = n1;

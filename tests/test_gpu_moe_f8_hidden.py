@@ -10,8 +10,10 @@ sum over magnitudes), with the rounding of a hidden value relative to its own
 - silu has a slope below 1.1, |silu(g)| <= |g|, and 8u for its evaluation;
 - a hidden value is two f16 terms of its group's power of two, which puts the
   group's largest in [2^14, 2^15): the remainder is at most 2^3 and rounded to
-  2^-9, 2^-23 of 2^14.  The power of two that brings a group to its block of
-  128's largest moves neither here (the groups are of one size): q = 2^-23.
+  2^-9, 2^-23 of 2^14.  Where the block of 128 has a larger group, both terms
+  are multiplied by a power of two of 2^-14 or more, and rounded again where
+  that gives less than 2^-14: 2^-25 each, against 2^14 2^-14: 2^-24 together.
+  q = 2^-23 + 2^-24.
 """
 import pytest
 
@@ -21,7 +23,7 @@ torch = pytest.importorskip("torch")
 
 TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 U = 2.0 ** -24
-Q = 2.0 ** -23
+Q = 2.0 ** -23 + 2.0 ** -24
 
 
 def blocks_of(n):
@@ -114,6 +116,32 @@ def test_nearly_equal_hidden_values(type_, t, e, top):
         for i in range(h):
             a, b = torch.randperm(f, generator=g)[:2].tolist()
             down[ex, i, a], down[ex, i, b] = 1.0, -1.0
+    ids, weights = routing(t, e, top, g)
+    x = x.to(TYPES[type_]).cuda()
+    w = codes(gate), codes(up), codes(down)
+    check(run(x, *w, ids, weights), x, *w, ids, weights)
+
+
+@pytest.mark.parametrize("type_", list(TYPES))
+@pytest.mark.parametrize("t,e,top", [(1, 1, 1), (3, 2, 1), (8, 1, 1), (13, 2, 2), (30, 2, 1), (64, 2, 2)])
+def test_groups_far_below_their_neighbours(type_, t, e, top):
+    """Groups of 16 hidden values down to 2^-70 of the others in their block of
+    128 (f16: 2^-24), and groups of zeros; each down row looks at one group only."""
+    g = torch.Generator().manual_seed(100 + t)
+    far = [0, 3, 13, 14, 15, 20, 24, None] if type_ == "f16" else [0, 13, 14, 16, 27, 45, 70, None]
+    h, f = 8 * 128, 272
+    x = torch.zeros((t, h))
+    for tok in range(t):
+        for i in range(8):
+            d = far[(i + tok) % 8]  # another order per token
+            x[tok, 128 * i + 1] = 0.0 if d is None else 2.0 ** -d
+    x[:, 0] = 1.0
+    group = torch.arange(f) // 16 % 8
+    gate, up = torch.zeros((e, f, h)), torch.zeros((e, f, h))
+    gate[:, :, 0] = torch.randint(1, 5, (e, f), generator=g).float()
+    up[:, torch.arange(f), 128 * group + 1] = torch.randint(1, 17, (e, f), generator=g).float()
+    down = torch.randint(-16, 17, (e, h, f), generator=g).float()
+    down *= group[None, None, :] == (torch.arange(h) % 8)[None, :, None]
     ids, weights = routing(t, e, top, g)
     x = x.to(TYPES[type_]).cuda()
     w = codes(gate), codes(up), codes(down)
