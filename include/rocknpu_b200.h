@@ -14,6 +14,8 @@
  *     waiting.  Kernels report errors in the device word `status`
  *     (0 = ok, 1 = non-finite input, 9 = an index out of range, any other:
  *     a device-side wait ran out).
+ *     The first error stays in the word, but a wait that ran out replaces 1
+ *     and 9 and is replaced by neither.
  *     Whenever that word is non-zero after the work has run, the call's
  *     outputs are unspecified (later kernels of the call may have run on
  *     scratch the failed step never wrote); only a zero status vouches for
@@ -361,7 +363,8 @@ size_t rocknpu_b200_gemm_f8_workspace_bytes(size_t m, size_t n, size_t k);
  * tiles split K; NULL or fewer than rocknpu_b200_gemm_f8_workspace_bytes runs
  * without.  The first 64 KiB must be zero before the first use of a
  * workspace; every launch that ends with status 0, 1 or 9 leaves them zero, so
- * one workspace serves calls of any shape, in turn.  Calls that share a
+ * one workspace serves calls of any shape, in turn (after any other status,
+ * zero them again).  Calls that share a
  * workspace must not overlap on the GPU (two streams, two captured graphs
  * replayed at once).  Results do not depend on the order in which CTAs
  * finish. */

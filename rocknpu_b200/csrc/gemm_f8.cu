@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_f8_kernel(const __grid_const
             // copies in flight must land before the CTA exits
             for (int i = max(0, g - S); i < g; ++i) {
                 if (!mbar_wait(&full[i % S], (i / S) & 1)) {
-                    atomicCAS(p.err, 0, kErrTimeoutDrain);
+                    report(p.err, kErrTimeoutDrain);
                     break;
                 }
             }
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_f8_kernel(const __grid_const
             }
             // our MMAs must finish before TMEM is released
             tc_commit(drain);
-            if (!mbar_wait(drain, 0)) atomicCAS(p.err, 0, kErrTimeoutDrain);
+            if (!mbar_wait(drain, 0)) report(p.err, kErrTimeoutDrain);
         }
         __syncwarp();
     } else {

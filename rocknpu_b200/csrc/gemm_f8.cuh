@@ -34,7 +34,7 @@ int pair_slots();
 int launch_pair(const F8Params& p, int npairs, cudaStream_t s);
 
 __device__ __forceinline__ void fail(int* err, volatile uint32_t* abort, int code) {
-    atomicCAS(err, 0, code);
+    report(err, code);
     *abort = 1u;
 }
 

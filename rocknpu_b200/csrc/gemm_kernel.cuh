@@ -94,7 +94,7 @@ struct Shared {
 };
 
 __device__ __forceinline__ void fail(const GemmParams& p, const Shared& sh, int code) {
-    atomicCAS(p.err, 0, code);
+    report(p.err, code);
     *sh.abort = 1u;
 }
 
@@ -169,7 +169,7 @@ __device__ __forceinline__ void fused_quant(const GemmParams& p, const Shared& s
             for (int w = 0; w < wpr; ++w) rmax = fmaxf(rmax, sh.red[row_in * wpr + w]);
             const float scale = row_scale(rmax);
             const float inv = row_inv(scale);
-            if (bad && lane == 0) atomicExch(p.err, kErrNonFinite);
+            if (bad && lane == 0) report(p.err, kErrNonFinite);
             int8_t* dst = p.q_a8 + static_cast<long long>(r) * p.q_ld8;
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
             // producer's arrival is part of the phase)
             for (int i = max(0, g - STAGES); i < g; ++i) {
                 if (!mbar_wait(&sh.full[i % STAGES], (i / STAGES) & 1)) {
-                    atomicCAS(p.err, 0, kErrTimeoutDrain);
+                    report(p.err, kErrTimeoutDrain);
                     break;
                 }
             }
@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_tc_kernel(const __grid_const
             }
             // our MMAs must finish before TMEM is released
             tc_commit(sh.drain);
-            if (!mbar_wait(sh.drain, 0)) atomicCAS(p.err, 0, kErrTimeoutDrain);
+            if (!mbar_wait(sh.drain, 0)) report(p.err, kErrTimeoutDrain);
         }
         __syncwarp();
     } else {

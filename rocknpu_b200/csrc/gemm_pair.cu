@@ -136,7 +136,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             // has landed) before the CTA leaves
             for (int i = max(0, g - S); i < g; ++i) {
                 if (!mbar_wait(&empty[i % S], (i / S) & 1)) {
-                    atomicCAS(p.err, 0, kErrTimeoutDrain);
+                    report(p.err, kErrTimeoutDrain);
                     break;
                 }
             }
@@ -177,10 +177,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
             // the pair's MMAs must finish before either CTA releases TMEM
             tc_commit_pair(drain, 0x3);
-            if (!mbar_wait(drain, 0)) atomicCAS(p.err, 0, kErrTimeoutDrain);
+            if (!mbar_wait(drain, 0)) report(p.err, kErrTimeoutDrain);
         } else if (lane == 0) {
             // odd CTA: the leader's MMAs write this CTA's TMEM too
-            if (!mbar_wait(drain, 0)) atomicCAS(p.err, 0, kErrTimeoutDrain);
+            if (!mbar_wait(drain, 0)) report(p.err, kErrTimeoutDrain);
         }
         __syncwarp();
     } else {

@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kGemvThreads) gemv_w8a8_x_kernel(const int8_t*
             if constexpr (HostOut)
                 *reinterpret_cast<volatile int*>(err) = kErrNonFinite;
             else
-                atomicExch(err, kErrNonFinite);
+                report(err, kErrNonFinite);
         }
         return;
     }

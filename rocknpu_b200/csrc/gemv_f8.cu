@@ -124,7 +124,7 @@ __device__ __forceinline__ void fill(const GemvParams& p, uint8_t* act) {
             if (l == 0) *reinterpret_cast<float*>(row + 256) = s;
         }
     }
-    if (!mag_finite(most) && blockIdx.x == 0) atomicExch(p.err, kErrNonFinite);
+    if (!mag_finite(most) && blockIdx.x == 0) report(p.err, kErrNonFinite);
 }
 
 template <class T>

@@ -60,7 +60,7 @@ struct StageParams {
     int err_plain;  // err (and y) are mapped host memory: errors by plain store
 };
 
-// Record an error code: in device memory the first error wins (atomic); a
+// Record an error code: in device memory by report(); a
 // status word in mapped host memory takes a plain store (atomics to host
 // memory need PCIe atomic operations), so there a later error code may
 // replace an earlier one -- either way the word is non-zero.
@@ -68,7 +68,7 @@ __device__ __forceinline__ void set_err(const StageParams& p, int code) {
     if (p.err_plain)
         *reinterpret_cast<volatile int*>(p.err) = code;
     else
-        atomicCAS(p.err, 0, code);
+        report(p.err, code);
 }
 
 // acc + X0 * b0 + X1 * b1 + X2 * b2 + X3 * b3: the 4 unsigned byte codes of

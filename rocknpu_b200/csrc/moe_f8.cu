@@ -149,7 +149,7 @@ struct Tables {
 };
 
 __device__ __forceinline__ void fail(int* err, volatile uint32_t* abort, int code) {
-    atomicCAS(err, 0, code);
+    report(err, code);
     *abort = 1u;
 }
 
@@ -311,7 +311,7 @@ __device__ __forceinline__ void layout_x(const MoeParams& p, int half, int halve
             if (l == 0) *reinterpret_cast<float*>(blk + ActBlock<LO>::kScaleAt) = s;
         }
     }
-    if (!mag_finite(most)) atomicExch(p.err, kErrNonFinite);
+    if (!mag_finite(most)) report(p.err, kErrNonFinite);
 }
 
 // Sums over k0..k1 of one expert's row with kRouterTokens tokens.
@@ -414,7 +414,7 @@ __device__ __forceinline__ void choose(const MoeParams& p, const Tables& tb, int
         key[j] = ex < p.e ? sort_key(v[j]) : 0u;
         vmax = fmaxf(vmax, v[j]);
     }
-    if (!finite) atomicExch(p.err, kErrNonFinite);
+    if (!finite) report(p.err, kErrNonFinite);
     vmax = warp_max(vmax);
     float ev[PER], sum = 0.0f;
 #pragma unroll
@@ -975,7 +975,7 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
             for (int i = threadIdx.x; i < p.t * p.top; i += kThreads) {
                 int ex = p.ids[i];
                 if (ex >= p.e) {
-                    if (blockIdx.x == 0) atomicCAS(p.err, 0, kErrBadIndex);
+                    if (blockIdx.x == 0) report(p.err, kErrBadIndex);
                     ex = -1;
                 }
                 tb.pair_e[i] = static_cast<short>(ex < 0 ? -1 : ex);
@@ -1101,7 +1101,7 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
             if (lane == 0)
                 for (int i = max(0, g - S); i < g; ++i)
                     if (!mbar_wait(&full[i % S], (i / S) & 1)) {
-                        atomicCAS(p.err, 0, kErrTimeoutDrain);
+                        report(p.err, kErrTimeoutDrain);
                         break;
                     }
             __syncwarp();

@@ -27,6 +27,20 @@ enum DeviceError : int {
 // wait is 2 s, rocknpu-matmul/src/int8_decode.rs:13).
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
 
+// Records an error in a status word.  The first one stays, except that a wait
+// that ran out replaces what an operand caused: it may have left a workspace's
+// counters at other values than zero, which the host has to learn.  (At most
+// two replacements: 0, an operand's code, a wait's.)
+__device__ __forceinline__ void report(int* err, int code) {
+    int seen = atomicCAS(err, kErrNone, code);
+    if (code == kErrNonFinite || code == kErrBadIndex) return;
+    for (int i = 0; i < 2 && (seen == kErrNonFinite || seen == kErrBadIndex); ++i) {
+        const int was = seen;
+        seen = atomicCAS(err, was, code);
+        if (seen == was) return;
+    }
+}
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }

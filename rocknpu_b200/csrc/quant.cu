@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kRowThreads) prep_w8_kernel(const uint8_t* __r
         });
     }
     if (__syncthreads_or(!finite)) {
-        if (threadIdx.x == 0) atomicExch(err, kErrNonFinite);
+        if (threadIdx.x == 0) report(err, kErrNonFinite);
         return;
     }
     const float scale = row_scale(block_max(amax, red));
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(kRowThreads) prep_w8_reg_kernel(const uint8_t*
         }
     }
     if (__syncthreads_or(!finite)) {
-        if (threadIdx.x == 0) atomicExch(err, kErrNonFinite);
+        if (threadIdx.x == 0) report(err, kErrNonFinite);
         return;
     }
     const float scale = row_scale(block_max(amax, red));
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(kRowThreads) prep_w8_q4k_lut_kernel(const uint
         amax = fmaxf(amax, fmaxf(fabsf(vlo), fabsf(vhi)));
     }
     if (__any_sync(0xffffffffu, !finite)) {
-        if (lane == 0) atomicExch(err, kErrNonFinite);
+        if (lane == 0) report(err, kErrNonFinite);
         return;
     }
     const float scale = row_scale(warp_max(amax));
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(kRowThreads) quant_rows_kernel(const float* __
     }
     for (int i = k + threadIdx.x; i < k16; i += kRowThreads) srow[i] = 0.0f;
     if (__syncthreads_or(!finite)) {
-        if (threadIdx.x == 0) atomicExch(err, kErrNonFinite);
+        if (threadIdx.x == 0) report(err, kErrNonFinite);
         return;
     }
     const float scale = row_scale(block_max(amax, red));
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kRegRowThreads) quant_rows_reg_kernel(const fl
         amax = fmaxf(fmaxf(amax, fmaxf(fabsf(v[j].x), fabsf(v[j].y))), fmaxf(fabsf(v[j].z), fabsf(v[j].w)));
     }
     if (__syncthreads_or(!finite)) {
-        if (threadIdx.x == 0) atomicExch(err, kErrNonFinite);
+        if (threadIdx.x == 0) report(err, kErrNonFinite);
         return;
     }
     const float scale = row_scale(block_max(amax, red));
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(kRowThreads) hilo_residual_kernel(const float*
         amax = fmaxf(amax, fabsf(v));
     }
     if (__syncthreads_or(!finite)) {
-        if (threadIdx.x == 0) atomicExch(err, kErrNonFinite);
+        if (threadIdx.x == 0) report(err, kErrNonFinite);
         return;
     }
     const float scale = row_scale(block_max(amax, red));

@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kRowsThreads, kRowsCtas)
         }
         at = then;
     }
-    if (!mag_finite(most)) atomicExch(err, kErrNonFinite);
+    if (!mag_finite(most)) report(err, kErrNonFinite);
 }
 
 template <class T>
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kPrepThreads, sizeof(T) == 4 ? 2 : WHOLE ? 3 :
     m = cta_max<kPrepThreads>(m, red);
     const float s = f8_scale(__uint_as_float(m));
     if (threadIdx.x == 0) {
-        if (!mag_finite(m)) atomicExch(err, kErrNonFinite);
+        if (!mag_finite(m)) report(err, kErrNonFinite);
         scales[blockIdx.x] = s;
     }
 #pragma unroll
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kKqThreads, KIND == kQ6K ? 3 : 2)
     m = cta_max<kKqThreads>(m, red);
     const float s = f8_scale(__uint_as_float(m));
     if (threadIdx.x == 0) {
-        if (!mag_finite(m)) atomicExch(err, kErrNonFinite);
+        if (!mag_finite(m)) report(err, kErrNonFinite);
         scales[blockIdx.x] = s;
     }
 #pragma unroll

@@ -80,7 +80,7 @@ __global__ void peer_barrier_kernel(PeerPtrs peers, unsigned* local_sig, int ran
             asm volatile("ld.acquire.sys.global.u32 %0, [%1];" : "=r"(v) : "l"(mine) : "memory");
             if (static_cast<int>(v - e) >= 0) break;
             if (rk::globaltimer_ns() - t0 > limit_ns) {
-                atomicCAS(err, 0, rk::kErrTimeoutPeer);
+                rk::report(err, rk::kErrTimeoutPeer);
                 break;
             }
             __nanosleep(200);
