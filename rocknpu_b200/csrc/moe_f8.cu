@@ -974,12 +974,14 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
         } else {
             for (int i = threadIdx.x; i < p.t * p.top; i += kThreads) {
                 int ex = p.ids[i];
+                const float w = p.weights[i];
                 if (ex >= p.e) {
                     if (blockIdx.x == 0) report(p.err, kErrBadIndex);
                     ex = -1;
                 }
+                if (ex >= 0 && !isfinite(w) && blockIdx.x == 0) report(p.err, kErrNonFinite);
                 tb.pair_e[i] = static_cast<short>(ex < 0 ? -1 : ex);
-                tb.pair_w[i] = p.weights[i];
+                tb.pair_w[i] = w;
             }
         }
         __syncthreads();

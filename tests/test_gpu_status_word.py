@@ -89,3 +89,25 @@ def test_a_wait_replaces_an_operands_code(before, after):
         lib().rocknpu_b200_set_peer_wait_limit_ms(0)
         for h, _ in handles:
             lib().rocknpu_b200_peer_buffer_destroy(h)
+
+
+@pytest.mark.parametrize("bad", [NAN, float("inf"), -float("inf")])
+def test_a_weight_of_a_live_slot_is_an_input(bad):
+    """Given routing weights: a non-finite one sets the word, except in an empty slot."""
+    from rocknpu_b200 import device as dev
+    t, h, f, e, top = 5, 256, 128, 3, 2
+    status = dev.new_status()
+    x = torch.randn((t, h), device="cuda")
+    gate, up = (dev.prepare_f8(torch.randn((e, f, h), device="cuda"), status) for _ in range(2))
+    down = dev.prepare_f8(torch.randn((e, h, f), device="cuda"), status)
+    ws = dev.new_workspace(dev.moe_f8_workspace_bytes(t, h, f, e, top, x.dtype))
+    ids = torch.randint(0, e, (t, top), dtype=torch.int32, device="cuda")
+    weights = torch.rand((t, top), device="cuda")
+    weights[3, 1] = bad
+    ids[3, 1] = -1
+    dev.moe_f8(x, gate, up, down, status, ws, ids=ids, weights=weights)
+    assert status.item() == 0
+    ids[3, 1] = 2
+    dev.moe_f8(x, gate, up, down, status, ws, ids=ids, weights=weights)
+    assert status.item() == 1
+    assert not ws[:65536].any()
