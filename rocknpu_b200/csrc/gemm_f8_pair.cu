@@ -251,8 +251,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             // while one is added, the next block's first piece included.
             auto ready = [&](int i) {
                 if (!wait_or_abort(&done[i % S], (i / S) & 1, abort)) {
-                    if (lane == 0 && !*abort) fail(p.err, abort, kErrTimeoutAccum);
-                    ok = false;
+                    if (!*abort) fail(p.err, abort, kErrTimeoutAccum);
+                    ok = false;  // of this lane; the others' may still have come
                 }
                 __syncwarp();
                 tc_fence_after();
@@ -305,6 +305,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 a1 = a2;
                 w1 = w2;
             }
+            ok = __all_sync(0xffffffffu, ok);  // the stores have barriers of the warp
             if (ok) {
                 if (p.out_type == kTypeF32)
                     store_rows<float>(p, acc, m0, n0, staging, lane);

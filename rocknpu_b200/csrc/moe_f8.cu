@@ -1151,7 +1151,7 @@ __global__ void __launch_bounds__(MoeCfg<NG, LO>::kThreads, 1) moe_f8_kernel(con
                     for (int kb = s.k0; kb < s.k1; ++kb, ++stage) {
                         const int st = stage % S;
                         if (!wait_or_abort(&full[st], (stage / S) & 1, abort)) {
-                            if (lane == 0 && !*abort) fail(p.err, abort, kErrTimeoutFull);
+                            if (!*abort) fail(p.err, abort, kErrTimeoutFull);  // any lane's wait
                             ok = false;
                         }
                         ok = __all_sync(0xffffffffu, ok);
