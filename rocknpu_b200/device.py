@@ -199,6 +199,14 @@ def _status_ptr(status: torch.Tensor) -> int:
     return status.data_ptr()
 
 
+def _workspace(workspace: torch.Tensor):
+    """(address, bytes); the bytes are the workspace's own, so no expanded or
+    strided view."""
+    if not workspace.is_contiguous():
+        raise ValueError("workspace is contiguous (new_workspace)")
+    return workspace.data_ptr(), workspace.nbytes
+
+
 def _f8_empty(like: torch.Tensor, *shape) -> torch.Tensor:
     """e4m3 tensor on `like`'s device whose rows start at multiples of 16 bytes."""
     k = shape[-1]
@@ -339,8 +347,7 @@ def gemm_f8(a8: torch.Tensor, a_scales: torch.Tensor, w8: torch.Tensor, w_scales
     out, out_type, ldo = _dense_out(out, m, n, out_dtype, a8)
     _launch("gemm_f8", dev, a8.data_ptr(), lda, a_scales.data_ptr(), _row_scales(a_scales, m, k, "a_scales"),
             w8.data_ptr(), ldw, w_scales.data_ptr(), out.data_ptr(), out_type, ldo, m, k, n,
-            None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.nbytes,
-            _status_ptr(status))
+            *((None, 0) if workspace is None else _workspace(workspace)), _status_ptr(status))
     return out
 
 
@@ -362,7 +369,7 @@ def matmul_f8(a: torch.Tensor, w8: torch.Tensor, w_scales: torch.Tensor, status:
     _weight_scales(w_scales, (_f8_blocks(n), _f8_blocks(k)), "w8")
     out, out_type, ldo = _dense_out(out, m, n, out_dtype or a.dtype, a)
     _launch("matmul_f8", dev, a.data_ptr(), type_, lda, w8.data_ptr(), ldw, w_scales.data_ptr(),
-            out.data_ptr(), out_type, ldo, m, k, n, workspace.data_ptr(), workspace.nbytes, _status_ptr(status))
+            out.data_ptr(), out_type, ldo, m, k, n, *_workspace(workspace), _status_ptr(status))
     return out
 
 
@@ -435,5 +442,5 @@ def moe_f8(x: torch.Tensor, gate, up, down, status: torch.Tensor, workspace: tor
                           *_experts(gate, (e, f, h), "gate"), *_experts(up, (e, f, h), "up"),
                           *_experts(down, (e, h, f), "down"), 0 if router is None else router.data_ptr(), router_type,
                           ld_router, 1 if renormalize else 0, ids.data_ptr(), weights.data_ptr())
-    _launch("moe_f8", dev, args, workspace.data_ptr(), workspace.nbytes, _status_ptr(status))
+    _launch("moe_f8", dev, args, *_workspace(workspace), _status_ptr(status))
     return out, ids, weights
