@@ -314,14 +314,15 @@ __device__ __forceinline__ void layout_x(const MoeParams& p, int half, int halve
     if (!mag_finite(most)) report(p.err, kErrNonFinite);
 }
 
-// Sums over k0..k1 of one expert's row with kRouterTokens tokens.
-__device__ __forceinline__ void router_dot(const MoeParams& p, int ex, int tok0, int k0, int k1, int lane,
+// This lane's sums of one expert's row with kRouterTokens tokens, over every
+// kRouterWarps-th stretch of k from stretch `from`.
+__device__ __forceinline__ void router_dot(const MoeParams& p, int ex, int tok0, int from, int lane,
                                            float (&s)[kRouterTokens]) {
 #pragma unroll
     for (int i = 0; i < kRouterTokens; ++i) s[i] = 0.0f;
-    if (p.wide) {  // k0 and k1 are multiples of 8
+    if (p.wide) {  // h is a multiple of 8
 #pragma unroll 2
-        for (int k = k0 + lane * 8; k < k1; k += 256) {
+        for (int k = from * 256 + lane * 8; k < p.h; k += kRouterWarps * 256) {
             float r[8];
             load_dense8(p.router, p.router_type, ex * p.ld_router + k, r);
 #pragma unroll
@@ -335,51 +336,61 @@ __device__ __forceinline__ void router_dot(const MoeParams& p, int ex, int tok0,
         }
     } else {
 #pragma unroll 4
-        for (int k = k0 + lane; k < k1; k += 32) {
+        for (int k = from * 32 + lane; k < p.h; k += kRouterWarps * 32) {
             const float r = load_dense(p.router, p.router_type, ex * p.ld_router + k);
 #pragma unroll
             for (int i = 0; i < kRouterTokens; ++i)
                 if (tok0 + i < p.t) s[i] = fmaf(r, load_dense(p.x, p.type, (tok0 + i) * p.ldx + k), s[i]);
         }
     }
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
-    for (int i = 0; i < kRouterTokens; ++i)
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
 }
 
 // Part `part` of the router products.  Few tasks: warps of a CTA share a
-// task's k range; many: a warp each.
+// task's stretches of k; many: a warp takes a task's one after the other.  The
+// sums are added in one order, lane by lane over the stretches and then over
+// the lanes, so a token's logits do not depend on the tokens beside it.
 __device__ __forceinline__ void router_products(const MoeParams& p, const Tables& tb, int part, int warp, int warps, int lane) {
     const int groups = (p.t + kRouterTokens - 1) / kRouterTokens, tasks = p.e * groups;
     float s[kRouterTokens];
     if (tasks <= 2 * static_cast<int>(gridDim.x)) {
-        const int per = (p.h / 8 + kRouterWarps - 1) / kRouterWarps * 8;
+        static_assert(kRouterWarps * kRouterTokens * 32 * 4 <= 8192, "sums in tb.red");
         for (int task = part; task < tasks; task += gridDim.x) {
             const int ex = task / groups, tok0 = (task - ex * groups) * kRouterTokens;
             if (warp < kRouterWarps) {
-                router_dot(p, ex, tok0, warp * per, min(p.h, (warp + 1) * per), lane, s);
-                if (lane == 0)
+                router_dot(p, ex, tok0, warp, lane, s);
 #pragma unroll
-                    for (int i = 0; i < kRouterTokens; ++i) tb.red[warp * kRouterTokens + i] = s[i];
+                for (int i = 0; i < kRouterTokens; ++i) tb.red[(warp * kRouterTokens + i) * 32 + lane] = s[i];
             }
             __syncthreads();
-            if (threadIdx.x < kRouterTokens && tok0 + static_cast<int>(threadIdx.x) < p.t) {
+            if (warp < kRouterTokens && tok0 + warp < p.t) {
                 float sum = 0.0f;
 #pragma unroll
-                for (int w = 0; w < kRouterWarps; ++w) sum += tb.red[w * kRouterTokens + threadIdx.x];
-                __stcg(p.logits + (tok0 + threadIdx.x) * p.e + ex, sum);
+                for (int w = 0; w < kRouterWarps; ++w) sum += tb.red[(w * kRouterTokens + warp) * 32 + lane];
+                sum = warp_sum(sum);
+                if (lane == 0) __stcg(p.logits + (tok0 + warp) * p.e + ex, sum);
             }
             __syncthreads();
         }
     } else {
         for (int task = part * warps + warp; task < tasks; task += gridDim.x * warps) {
             const int ex = task / groups, tok0 = (task - ex * groups) * kRouterTokens;
-            router_dot(p, ex, tok0, 0, p.h, lane, s);
-            if (lane == 0)
+            float sum[kRouterTokens] = {};
+            for (int from = 0; from < kRouterWarps; ++from) {
+                router_dot(p, ex, tok0, from, lane, s);
 #pragma unroll
-                for (int i = 0; i < kRouterTokens; ++i)
-                    if (tok0 + i < p.t) __stcg(p.logits + (tok0 + i) * p.e + ex, s[i]);
+                for (int i = 0; i < kRouterTokens; ++i) sum[i] += s[i];
+            }
+#pragma unroll
+            for (int i = 0; i < kRouterTokens; ++i) {
+                sum[i] = warp_sum(sum[i]);
+                if (lane == 0 && tok0 + i < p.t) __stcg(p.logits + (tok0 + i) * p.e + ex, sum[i]);
+            }
         }
     }
 }
