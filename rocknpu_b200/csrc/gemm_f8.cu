@@ -394,7 +394,7 @@ F8Plan plan_f8(int m, int n, int k) {
     const int kb = (k + kF8Block - 1) / kF8Block, sms = sm_count();
     double best = 1e300;
     for (int bt : {16, 32, 64, 128}) {
-        if (bt > 16 && bt >= 2 * m) break;
+        if (bt > 16 && bt / 2 >= m) break;
         const long long tiles =  // more are refused at the launch
             std::min<long long>(static_cast<long long>((n + kWRows - 1) / kWRows) * ((m + bt - 1) / bt), 0x7fffffff);
         const double block = std::max(4.0 * std::max(55.0, bt / 2.0) + 150.0, (kWRows + bt) * 128 / 60.0);
