@@ -335,7 +335,9 @@ int rocknpu_b200_gemv_kq(uint32_t kind, const uint8_t *layout, size_t k, size_t 
  * `type` / `out_type` are ggml ids: ROCKNPU_GGML_F32, _F16 or _BF16; dense
  * pointers are aligned to their elements (16-byte aligned rows are faster),
  * scales and status words to 4 bytes.
- * A non-finite input sets *status to 1 and leaves the outputs unspecified. */
+ * A non-finite input (dense values, K-quant blocks, routers, routing weights)
+ * sets *status to 1 and leaves the outputs unspecified; codes and block scales
+ * are taken as they are. */
 
 /* Activation rows a[m][lda] -> a_f8[m][ld_f8] + scales[m][ld_scales]; columns
  * k..ld_f8 of a_f8 are left as they are. */
@@ -408,7 +410,9 @@ typedef struct rocknpu_b200_f8_experts {
  * be x.
  * Activations are not quantised: f32 ones, and the hidden values of every
  * type, enter the products with 22 bits relative to the largest of their block
- * of 128 (hidden values: of 16), f16 and bf16 ones exactly; sums are f32.
+ * of 128 (hidden values: of 16), f16 and bf16 ones exactly but for what is
+ * below 2^-39 of that; sums are f32, those of the router too.  A token's
+ * choice and weights do not depend on the tokens beside it.
  * hidden and ffn are multiples of 16, top_k <= 16, experts <= 256. */
 typedef struct rocknpu_b200_moe_f8_args {
     size_t tokens, hidden, ffn, experts, top_k;

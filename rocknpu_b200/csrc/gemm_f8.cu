@@ -383,12 +383,14 @@ struct F8Plan {
     size_t scratch = 0;
 };
 
-// Tile height and distribution.  A block costs a CTA the larger of its MMAs
-// (four of at least 55 cycles, and about 150 of barriers and commits) and its
-// bytes from L2 at about 60 per cycle.  Whole tiles take ceil(tiles / SMs)
-// rounds; cut evenly the blocks divide without a remainder, but a CTA then
-// writes (and its neighbour reads) up to two partial tiles at about 30 bytes
-// per cycle.
+// Tile height and distribution, by costs in one unit.  They are fitted so that
+// the faster form is chosen and are not the cycles a form takes (a pair's
+// block is priced 600 and takes about 890 of them).  A block costs a CTA the
+// larger of its MMAs (four of at least 55, and about 150 of barriers and
+// commits) and its bytes from L2 at about 60 per unit.  Whole tiles take
+// ceil(tiles / SMs) rounds; cut evenly the blocks divide without a remainder,
+// but a CTA then writes (and its neighbour reads) up to two partial tiles at
+// about 30 bytes per unit.
 F8Plan plan_f8(int m, int n, int k) {
     F8Plan pl;
     const int kb = (k + kF8Block - 1) / kF8Block, sms = sm_count();
@@ -413,7 +415,8 @@ F8Plan plan_f8(int m, int n, int k) {
             pl.scratch = stream ? static_cast<size_t>(pl.grid) * 2 * kWRows * bt * sizeof(float) : 0;
         }
     }
-    // two-SM tiles: 512 cycles of MMAs per block and 256 x 256 outputs
+    // two-SM tiles: 512 cycles of MMAs per block and 256 x 256 outputs; 4000 for
+    // a tile's start and its stores
     const long long pairs = static_cast<long long>((n + 255) / 256) * ((m + 255) / 256);
     const int slots = m > 128 ? f8_detail::pair_slots() : 0;
     if (slots > 0) {

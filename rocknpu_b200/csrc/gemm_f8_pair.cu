@@ -29,7 +29,10 @@
 // that its sums are in TMEM; the epilogue is never more than the two TMEM
 // buffers behind, less than the stages, so it cannot miss a phase.
 //
-// Measured: 4096 x 8192 x 28672 bf16 1015 us with the quantiser, 1.9 PFLOP/s.
+// Measured: 4096 x 8192 x 28672 bf16 1030 us with the quantiser, 1.9 PFLOP/s, at
+// the power limit's clocks; 910 us and 2.1 PFLOP/s for a call after idling.  A block
+// takes about 890 cycles where its MMAs take 512: an epilogue warp has one TMEM
+// load in flight, waits for four of them, and frees the buffer after the last.
 //
 // Bounded waits as in the int8 pair kernel (gemm_pair.cu).
 #include <algorithm>

@@ -49,11 +49,11 @@
 // cooperative launch cost 16 us more per call).  The weight copies of phase 2
 // start before its wait.  Every wait is bounded.
 //
-// Measured: one token, 2 of 8 experts, 2048 / 5632, f32: 38.7 us, 69 MB of
+// Measured: one token, 2 of 8 experts, 2048 / 5632, f32: 37.5 us, 69 MB of
 // weights (10.6 us at HBM's rate; half is the latency of the phases); 13
-// tokens, 4 of 16, 1536 / 2240, f16: 53.6 us, 3.1 TB/s; 64 tokens, 2 of 8, 4096 /
-// 8192, bf16: 298 us, 2.7 TB/s, bound by the consumers, two warps per scheduler
-// (copies alone: 204 us).
+// tokens, 4 of 16, 1536 / 2240, f16: 56.5 us, 2.9 TB/s; 64 tokens, 2 of 8, 4096 /
+// 8192, bf16: 329 us, 2.5 TB/s, bound by the consumers, two warps per scheduler
+// (the hidden values' second term about 20 us, the look for far groups 10).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -1251,7 +1251,10 @@ bool make_expert_map(CUtensorMap* map, const MoeWeight& w, int k, int rows, int 
 }
 
 // Token groups of 8 per expert and entry: twice the mean number of tokens per
-// expert, at most all.  An expert with more is read twice.
+// expert, at most all.  An expert with n pairs is n / (8 groups) entries,
+// rounded up, and its weights are copied for each: with even routing once, for
+// all of 64 tokens on one of 64 experts eight times (2048 / 1024, bf16, 1 of
+// 64, launch included: even 123 us, 40 of the tokens on one expert 80, all 49).
 int token_groups(int t, int e, int top) {
     const int cap = std::min(t, 2 * ((t * top + e - 1) / e));
     return cap <= 8 ? 1 : cap <= 16 ? 2 : cap <= 32 ? 4 : 8;
