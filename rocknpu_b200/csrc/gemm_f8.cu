@@ -285,9 +285,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_f8_kernel(const __grid_const
 #pragma unroll
             for (int i = 0; i < kPer; ++i) as[i] = p.a_scale + static_cast<long long>(min(m0 + lane + 32 * i, p.m - 1)) * p.ld_as;
             // the next block's scales are loaded one block ahead
-            float sa[kPer], sw = __ldg(ws + t.kb0);
+            float sa[kPer], sw = ld_global(ws + t.kb0);
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) sa[i] = __ldg(as[i] + t.kb0);
+            for (int i = 0; i < kPer; ++i) sa[i] = ld_global(as[i] + t.kb0);
             float acc[COLS];
 #pragma unroll
             for (int c = 0; c < COLS; ++c) acc[c] = 0.0f;
@@ -298,9 +298,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_f8_kernel(const __grid_const
                 for (int i = 0; i < kPer; ++i)
                     if (lane + 32 * i < COLS) sc[lane + 32 * i] = sa[i] * sw;
                 const int nkb = min(kb + 1, t.kb1 - 1);
-                sw = __ldg(ws + nkb);
+                sw = ld_global(ws + nkb);
 #pragma unroll
-                for (int i = 0; i < kPer; ++i) sa[i] = __ldg(as[i] + nkb);
+                for (int i = 0; i < kPer; ++i) sa[i] = ld_global(as[i] + nkb);
                 __syncwarp();
                 int ready = 0;
                 if (lane == 0) ready = wait_or_abort(&tfull[b], (g / B) & 1, abort) ? 1 : 0;

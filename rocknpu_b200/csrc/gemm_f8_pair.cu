@@ -270,7 +270,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             };
             // scales two blocks ahead
             const int last = p.num_kb - 1;
-            float s = __ldg(as) * __ldg(ws), a1 = __ldg(as + min(1, last)), w1 = __ldg(ws + min(1, last));
+            float s = ld_global(as) * ld_global(ws), a1 = ld_global(as + min(1, last)), w1 = ld_global(ws + min(1, last));
             uint32_t r0[32], r1[32];
             ready(g);
             tmem_ld32(lane_base + (g & 1) * kTile, r0);
@@ -278,7 +278,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             // 4096 x 28672 x 8192)
 #pragma unroll 4
             for (int kb = 0; kb < p.num_kb; ++kb, ++g) {
-                const float a2 = __ldg(as + min(kb + 2, last)), w2 = __ldg(ws + min(kb + 2, last));
+                const float a2 = ld_global(as + min(kb + 2, last)), w2 = ld_global(ws + min(kb + 2, last));
                 const uint32_t base = lane_base + (g & 1) * kTile;
                 tmem_ld_wait();
                 tmem_ld32(base + 32, r1);

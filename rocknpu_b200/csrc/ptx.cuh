@@ -94,6 +94,15 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// A read of what a preceding kernel may still have been writing when this one
+// began (griddep_wait() lies between): not through the non-coherent path, which is
+// for data that nobody writes during the kernel.
+__device__ __forceinline__ float ld_global(const float* p) {
+    float v;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    return v;
+}
+
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Bounded wait that also gives up once another role of the CTA has aborted.
